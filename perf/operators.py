@@ -143,8 +143,6 @@ def prepare(case, seed):
             # quantised once, before the layer runs: whole rows to [-127, 127] by their largest magnitude
             state['x'] = (x * (127.0 / x.abs().amax(1, keepdim=True))).round().to(torch.int8)
             state['row_scale'] = (x.abs().amax(1) / 127.0)
-            if case['gather']:
-                state['row_scale'] = state['row_scale'][state['rows'].long()]
             state['weight'] = torch.randint(-127, 128, shape_w, generator=gen, device='cuda', dtype=torch.int8)
             state['channel_scale'] = (0.5 + torch.rand(shape_w[:2], generator=gen, device='cuda')) / (73.0 * math.sqrt(case['inner']))
         else:
@@ -214,7 +212,8 @@ def _plain_grouped(state):
     expert = torch.searchsorted(offsets[1:].contiguous(), at, right=True)
     v = product[expert, at - offsets[expert]]
     if state['row_scale'] is not None:
-        v = v * state['row_scale'][:, None] * state['channel_scale'][expert]
+        scale = state['row_scale'] if state['rows'] is None else state['row_scale'][state['rows'].long()]
+        v = v * scale[:, None] * state['channel_scale'][expert]
     if state['bias'] is not None:
         v = v + state['bias'][expert]
     if case['gated']:
@@ -335,7 +334,8 @@ def exact(case, seed):
             mine = state['x'][b:t] if state['rows'] is None else state['x'].index_select(0, state['rows'][b:t].long())
             v = mine.double() @ state['weight'][e].double().mT
             if state['row_scale'] is not None:
-                v = v * torch.outer(state['row_scale'][b:t].double(), state['channel_scale'][e].double())
+                token_scale = state['row_scale'][b:t] if state['rows'] is None else state['row_scale'].index_select(0, state['rows'][b:t].long())
+                v = v * torch.outer(token_scale.double(), state['channel_scale'][e].double())
             if state['bias'] is not None:
                 v = v + state['bias'][e].double()
             if case['gated']:
