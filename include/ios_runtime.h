@@ -229,6 +229,67 @@ IOS_API int ios_pointwise_conv_static_scratch(const float *x, const float *w, co
  * call is then incomplete; the word and the counters are cleared), IOS_OK otherwise. */
 IOS_API int ios_static_scratch_status(void *cuda_stream);
 
+/* ---- operators on device tensors: a mixture-of-experts layer and its 8-bit products (no counterpart in the
+ *      reference, whose operators are those of convolution networks) -------------------------------------------
+ * All pointers are DEVICE pointers of one device, which need not be the current one; matrices are row-major with a
+ * row stride in elements and unit column stride, any alignment of the element type.  The work is enqueued on
+ * cuda_stream (a cudaStream_t of that device, NULL = default stream) and NOT synchronised; nothing is allocated or
+ * kept between calls, so calls may overlap and may be captured into graphs.  Outputs must not overlap inputs.
+ * Sums, softmax terms and scales are float32 (8-bit products: int32).  Everything runs in a fixed order: the same
+ * inputs give the same bits.  Zero rows are no error. */
+enum { IOS_F32 = 0, IOS_F16 = 1, IOS_BF16 = 2, IOS_S8 = 3 };   /* element types */
+
+/* The router.  For each token the k experts with the largest logits (equal logits: the lower index first; -inf and
+ * NaN are never chosen, so a token may get fewer than k or none), their gates
+ *     gates[t, j] = exp(l_j - max) / sum     over the chosen (renormalize != 0) or over all experts of the token,
+ * and the plan that orders the (token, expert) pairs by expert, inside an expert by token:
+ *     chosen[tokens, k]   expert of each pair, best first; -1 where none was left (its gate is 0)
+ *     offsets[experts+1]  expert e owns the sorted rows offsets[e] .. offsets[e+1] - 1
+ *     rows[tokens * k]    token of each sorted row; -1 behind the last one
+ *     slots[tokens, k]    sorted row of each pair, -1 for none
+ * type: IOS_F32 / IOS_F16 / IOS_BF16; experts <= 1024, k <= 32 and k <= experts.  workspace: at least the bytes that
+ * ios_route_experts_workspace names (0 for small calls, then NULL is fine), 4-byte aligned, contents irrelevant; it
+ * must not be shared by calls that overlap. */
+IOS_API int ios_route_experts_workspace(int tokens, int experts, size_t *bytes);
+IOS_API int ios_route_experts(const void *logits, int type, int tokens, int experts, long long stride, int k,
+                              int renormalize, int *chosen, float *gates, int *offsets, int *rows, int *slots,
+                              void *workspace, size_t workspace_bytes, void *cuda_stream);
+
+/* Ragged products: for every row r of group g, offsets[g] <= r < offsets[g + 1],
+ *     y[r, n] = act(row_scale[src] * channel_scale[g, n] * sum_k x[src, k] * w[g, n, k] + bias[g, n]),
+ * src = rows[r] if rows is given, else r.  gated != 0: w, channel_scale and bias have 2 * channels rows per group and
+ *     y[r, n] = act(v[n]) * v[channels + n]          (v: the value inside act(...) above).
+ * x[x_rows, inner] and w[groups, channels (* 2), inner] have one type (IOS_F32: three TF32 products, fp32-grade;
+ * IOS_F16, IOS_BF16; IOS_S8: inner < 131072), y[total_rows, channels] is IOS_F32 / IOS_F16 / IOS_BF16.  row_scale[x_rows],
+ * channel_scale and bias (groups x channels or 2 * channels, dense) are float32 or NULL.  act: 0 identity, 1 relu,
+ * 2 sigmoid, 3 tanh, 4 silu.  offsets[groups + 1] is read on the device and must not decrease; it may stop short of
+ * total_rows, rows of y behind the last group are left as they were.  An entry of rows outside [0, x_rows) reads as a row
+ * of zeros.  groups <= 1024. */
+IOS_API int ios_grouped_matmul(const void *x, int type, long long x_rows, long long x_stride, const void *w, int groups,
+                               int channels, int inner, long long w_stride, long long w_group_stride, const int *offsets,
+                               const int *rows, int total_rows, const float *row_scale, const float *channel_scale,
+                               const float *bias, int act, int gated, void *y, int y_type, long long y_stride,
+                               void *cuda_stream);
+
+/* y[m, n] = act(row_scale[m] * channel_scale[n] * sum_k a[m, k] * b[n, k] + bias[n]) with 8-bit integers a, b and exact
+ * sums (inner < 131072); row_scale, channel_scale, bias float32 or NULL, act as above. */
+IOS_API int ios_matmul_int8(const signed char *a, long long a_stride, const signed char *b, long long b_stride, int rows,
+                            int channels, int inner, const float *row_scale, const float *channel_scale,
+                            const float *bias, int act, void *y, int y_type, long long y_stride, void *cuda_stream);
+
+/* Rows to 8-bit integers with a scale each: scale[r] = max |x[src]| / 127 over the finite values,
+ * q[r, k] = 127 x[src, k] / max |x[src]| rounded to the nearest whole number, halves to even (exactly: no rounding of the
+ * quotient comes first).  A row of zeros gets scale 0; NaN becomes 0, an infinity +-127.  src as above.  The same call
+ * quantises a weight matrix [channels, inner] with a scale per channel. */
+IOS_API int ios_quantize_rows(const void *x, int type, long long x_rows, long long x_stride, int inner, const int *rows,
+                              long long total_rows, signed char *q, long long q_stride, float *scale, void *cuda_stream);
+
+/* out[t, :] = sum over j < k of gates[t, j] * y[slots[t, j], :], in the order of j; a slot outside [0, y_rows) adds
+ * nothing, a token without any gets zeros. */
+IOS_API int ios_combine_experts(const void *y, int type, long long y_rows, long long y_stride, const float *gates,
+                                const int *slots, long long tokens, int k, int channels, void *out, int out_type,
+                                long long out_stride, void *cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,7 +11,8 @@ Same functions, arguments and return shapes as the reference's
   raw buffer of whatever array it is given, ``ios_runtime.py:126``);
 * there is no CPU path: without a CUDA device every call raises.
 
-``Engine`` is the build-once / run-many handle used for serving and benchmarking.
+``Engine`` is the build-once / run-many handle used for serving and benchmarking.  ``route_experts``, ``grouped_matmul``,
+``matmul_int8``, ``quantize_rows`` and ``combine_experts`` work on GPU tensors (``device_ops.py``).
 """
 import ctypes
 import json
@@ -22,6 +23,8 @@ import numpy as np
 
 from ios.ir import Conv, Graph, Block, Node
 from .ctypes_utils import c_string, c_string_list, c_ndarray_list, get_nodes_by_type
+from . import device_ops
+from .device_ops import Routing, combine_experts, grouped_matmul, matmul_int8, quantize_rows, route_experts  # noqa: F401
 
 cur_dir = os.path.dirname(os.path.abspath(os.path.realpath(__file__)))
 
@@ -77,6 +80,7 @@ def load_ios_library():
         handle.ios_host_register.argtypes = [ctypes.c_void_p, ctypes.c_size_t]
         handle.ios_host_unregister.argtypes = [ctypes.c_void_p]
         handle.ios_conv2d.argtypes = [ctypes.c_void_p] * 4 + [_INT] * 14
+        device_ops.declare(handle)
         return handle
     raise FileNotFoundError('IOS Backend library not found (build it with inter-operator-scheduler_b200/build.py)')
 
