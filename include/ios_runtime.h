@@ -239,6 +239,10 @@ IOS_API int ios_static_scratch_status(void *cuda_stream);
  * inputs give the same bits.  Zero rows are no error. */
 enum { IOS_F32 = 0, IOS_F16 = 1, IOS_BF16 = 2, IOS_S8 = 3 };   /* element types */
 
+/* Waits for cuda_stream, then tells whether a bounded wait inside a product on `device` ran out since the last call of
+ * this function (IOS_ERR_TIMEOUT: an output is incomplete) -- the calls below return before their work is done. */
+IOS_API int ios_device_ops_status(int device, void *cuda_stream);
+
 /* The router.  For each token the k experts with the largest logits (equal logits: the lower index first; -inf and
  * NaN are never chosen, so a token may get fewer than k or none), their gates
  *     gates[t, j] = exp(l_j - max) / sum     over the chosen (renormalize != 0) or over all experts of the token,

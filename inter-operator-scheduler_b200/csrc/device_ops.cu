@@ -86,6 +86,7 @@ int check_grouped(const GroupedParams &p, const char *what) {
     if (p.y_stride < p.channels) return fail(IOS_ERR_ARGUMENT, "%s: rows of y overlap (stride %lld, %d channels)", what, p.y_stride, p.channels);
     if (p.type == Elem::S8 && p.inner >= 131072)
         return fail(IOS_ERR_LIMIT, "%s: 8-bit products of 131072 or more elements can pass the 32 bits of their sum", what);
+    if (grouped_too_large(p)) return fail(IOS_ERR_LIMIT, "%s: %d rows of %d channels are too many for one call", what, p.total, p.channels);
     if (!p.rows && p.x_rows < p.total) return fail(IOS_ERR_ARGUMENT, "%s: x has %lld rows, y %d", what, p.x_rows, p.total);
     return IOS_OK;
 }
@@ -285,4 +286,16 @@ extern "C" int ios_combine_experts(const void *y, int type, long long y_rows, lo
     p.out_type = Elem(out_type);
     p.out_stride = out_stride;
     return finish("combine_experts", launch_combine(p, static_cast<cudaStream_t>(cuda_stream)));
+}
+
+extern "C" int ios_device_ops_status(int device, void *cuda_stream) {
+    int current = 0, code = 0;
+    if (cudaError_t err = cudaGetDevice(&current)) return DeviceScope::cuda("cudaGetDevice", err);
+    if (cudaError_t err = cudaSetDevice(device)) return DeviceScope::cuda("cudaSetDevice", err);
+    const cudaError_t err = expert_mm_status(static_cast<cudaStream_t>(cuda_stream), &code);
+    cudaSetDevice(current);
+    if (err != cudaSuccess) return DeviceScope::cuda("reading the time-out word", err);
+    if (code != 0) return fail(IOS_ERR_TIMEOUT, "a bounded wait inside a product ran out (code %d): its output is incomplete", code);
+    record_error("");
+    return IOS_OK;
 }

@@ -1,121 +1,781 @@
-// Matrix products over ragged groups of rows: y[r, :] = act(x[src(r), :] w[g]^T ...) for the rows r of group g.
+// Matrix products over ragged groups of rows on the 5th-generation tensor cores (sm_100a):
 //
-// A 64 x 64 output tile per block, operands staged in shared memory, float (8-bit: int) sums in registers.  The group
-// sizes are only known on the device, so the grid covers the most tiles any distribution of the rows can need and
-// every block finds its own tile from the offsets.
+//     y[r, n] = act(row_scale[src] channel_scale[g, n] sum_k x[src, k] w[g, n, k] + bias[g, n]),   r in group g
+//
+// * The weights' channels are the 128 rows of a tcgen05.mma (TMEM lanes), a group's rows are its columns: N may be any
+//   multiple of 16 up to 256, so a group of one row costs a 16-column instruction instead of a 128-row one, and a
+//   group's end needs no masked store -- the epilogue writes whole columns, one row of y each.  K advances one 128-byte
+//   swizzle row per step (64 elements of 16 bits, 128 of 8 bits, 32 of float32).
+// * The group sizes are only known on the device.  Every CTA works out the same list of tiles from the offsets (one
+//   scan) and resident CTAs walk it; a group's rows are dealt evenly to its tiles.
+// * Products too small to fill the GPU split K over a thread-block cluster: the CTAs deal the tile's columns among
+//   themselves, push their partial sums into the shared memory of the CTA that finishes a column, and that CTA adds them
+//   in rank order.  No workspace, no counters, the same bits every time.
+// * Operands arrive by TMA where their rows start on 16-byte boundaries -- rows gathered by index through
+//   tile::gather4 -- and through registers of eight loader warps otherwise.
+// * float32: every operand is split into two TF32 numbers on its way into shared memory (loader warps); three products
+//   a_hi b_hi + a_hi b_lo + a_lo b_hi.  The tensor core truncates where it adds, so the sum over more than 128 elements is
+//   formed in registers, rounded to nearest, from partial sums over 128.
+// * gated: 16 rows of the gate half and the 16 rows of the same channels of the other half alternate in the tile, so that
+//   a lane and the lane 16 further on hold the two factors of one result.
+//
+// Warp roles: 0 = weight loads, 1 = MMA issuer, 2 = tensor memory, 3 = row loads, 4..7 = epilogue, 8..15 = loaders (only
+// where TMA cannot be used).  Every wait is bounded; on a time-out the device's error word is set, loads in flight are
+// waited for, tensor memory is freed and the kernel returns.
 #include "expert_ops.h"
+#include "kernels.h"
+#include "tc_device.h"
 
-#include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <algorithm>
+#include <climits>
 
 namespace ios {
 namespace {
 
-constexpr int kTile = 64, kStep = 16, kThreads = 256;
+enum Kind { kF16 = 0, kI8 = 1, kX3 = 2 };       // instruction: 16-bit floats, 8-bit integers, three TF32 products
 
-template <class T> struct Arith { using Sum = float; };
-template <> struct Arith<signed char> { using Sum = int; };
-__device__ __forceinline__ float widen(float v) { return v; }
-__device__ __forceinline__ float widen(__half v) { return __half2float(v); }
-__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ int widen(signed char v) { return v; }
+constexpr int kEpilogueWarps = 4, kLoaderWarps = 8;
+constexpr int kTmaThreads = 256, kLoadThreads = 512;
+constexpr int kLoaderCols = 128;                // widest tile of the loader warps (their registers hold a step)
+constexpr int kChunkSteps = 4;                  // float32: K steps per partial sum
+constexpr int kMaxStages = 12;
+constexpr int kMaxGroupTiles = INT_MAX / kMaxExperts - 1;    // tiles of a group: their sum over all groups fits an int
+constexpr size_t kSmemLimit = 227 * 1024;
 
-__device__ __forceinline__ float apply_act(float v, int act) {
-    switch (act) {
-        case 1: return fmaxf(v, 0.0f);
-        case 2: return 1.0f / (1.0f + __expf(-v));
-        case 3: return tanhf(v);
-        case 4: return v / (1.0f + __expf(-v));
-        default: return v;
-    }
-}
+__device__ int g_expert_error;                  // set by a wait that ran out, read by expert_mm_status
+
+struct MmGeom {
+    int tn;             // columns a tile may have
+    int n_tiles;        // channel tiles of a group
+    int tile_channels;  // output channels per channel tile: 128, gated 64
+    int k_steps;
+    int cluster;        // CTAs that share a tile's K range
+    int stages;
+    int box_rows;       // rows per TMA box of x
+    int tmem_cols;
+    uint32_t format;    // operand format field of the instruction descriptor
+    int esize;
+    int stage_off, recv_off, table_off, bar_off;   // byte offsets in shared memory
+};
+
+struct Tile {
+    int group, row0, valid, cols, channel0;
+};
 
 // offsets come from the device: whatever they hold, a group stays inside [0, total]
-__device__ __forceinline__ void group_rows(const GroupedParams &p, int g, int *begin, int *end) {
-    if (!p.offsets) { *begin = 0; *end = p.total; return; }
+__device__ __forceinline__ void group_rows(const GroupedParams &p, int g, int *begin, int *count) {
+    if (!p.offsets) { *begin = 0; *count = p.total; return; }
     *begin = min(max(p.offsets[g], 0), p.total);
-    *end = min(max(p.offsets[g + 1], *begin), p.total);
+    *count = min(max(p.offsets[g + 1], *begin), p.total) - *begin;
+}
+// Columns per tile of a group: its rows dealt evenly to the fewest tiles, in multiples of 16.
+__device__ __forceinline__ int even_cols(int count, int tn) {
+    const int tiles = (count + tn - 1) / tn;
+    return ((count + tiles - 1) / tiles + 15) & ~15;
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads) grouped_kernel(const GroupedParams p) {
-    using Sum = typename Arith<T>::Sum;
-    __shared__ Sum xs[kStep][kTile + 4], ws[2][kStep][kTile + 4];
-    int tile = blockIdx.x, g = 0, begin = 0, end = 0;
-    for (;; ++g) {
-        if (g == p.groups) return;
-        group_rows(p, g, &begin, &end);
-        const int tiles = (end - begin + kTile - 1) / kTile;
-        if (tile < tiles) break;
-        tile -= tiles;
+// first[g] = tiles before group g, for all groups; all threads call it
+__device__ void build_table(const GroupedParams &p, const MmGeom &t, int *first, int threads) {
+    __shared__ int warp_total[kLoadThreads / 32];
+    constexpr int kPer = kMaxExperts / kTmaThreads;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int mine[kPer], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int g = int(threadIdx.x) * kPer + i;
+        int count = 0, begin;
+        if (g < p.groups) group_rows(p, g, &begin, &count);
+        const int c = count > 0 ? even_cols(count, t.tn) : 1;
+        mine[i] = int(min((long long)((count + c - 1) / c) * t.n_tiles, (long long)kMaxGroupTiles));
+        sum += mine[i];
     }
-    const int row0 = begin + tile * kTile, n0 = blockIdx.y * kTile;
-    const int halves = p.gated ? 2 : 1;
-    const T *w = static_cast<const T *>(p.w) + (long long)g * p.w_group_stride;
-    const int tr = threadIdx.x / 16 * 4, tc = threadIdx.x % 16 * 4;
-    Sum acc[2][4][4] = {};
-    for (int k0 = 0; k0 < p.inner; k0 += kStep) {
-        for (int i = threadIdx.x; i < kTile * kStep; i += kThreads) {
-            const int r = i / kStep, k = i % kStep;
-            Sum v = 0;
-            if (row0 + r < end && k0 + k < p.inner) {
-                const long long src = p.rows ? p.rows[row0 + r] : row0 + r;
-                if (src >= 0 && src < p.x_rows) v = widen(static_cast<const T *>(p.x)[src * p.x_stride + k0 + k]);
+    int run = sum;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, run, s);
+        if (lane >= s) run += v;
+    }
+    if (lane == 31) warp_total[warp] = run;
+    __syncthreads();
+    int start = run - sum;
+    for (int w = 0; w < warp; ++w) start += warp_total[w];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int g = int(threadIdx.x) * kPer + i;
+        if (g < p.groups) first[g] = start;
+        start += mine[i];
+        if (g == p.groups - 1) first[p.groups] = start;
+    }
+}
+
+// Tiles of a group: up to 8 column tiles side by side, then the next channels, so that neighbours in the list share
+// weights and rows in L2.
+__device__ __forceinline__ Tile find_tile(const GroupedParams &p, const MmGeom &t, const int *first, int index) {
+    int lo = 0, hi = p.groups;                    // first[lo] <= index < first[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first[mid] <= index) lo = mid;
+        else hi = mid;
+    }
+    int begin, count;
+    group_rows(p, lo, &begin, &count);
+    const int cols = even_cols(count, t.tn);
+    const int col_tiles = (count + cols - 1) / cols;
+    const int at = index - first[lo];
+    const int band = at / (8 * t.n_tiles);
+    const int wide = min(8, col_tiles - band * 8);
+    const int inside = at - band * 8 * t.n_tiles;
+    Tile tile;
+    tile.group = lo;
+    const int col0 = (band * 8 + inside % wide) * cols;
+    tile.row0 = begin + col0;
+    tile.valid = min(cols, count - col0);
+    tile.cols = (tile.valid + 15) & ~15;
+    tile.channel0 = inside / wide * t.tile_channels;
+    return tile;
+}
+
+// Row of the weights (inside its group) that tile row r holds
+__device__ __forceinline__ int weight_row(const GroupedParams &p, const Tile &tile, int r) {
+    if (!p.gated) return tile.channel0 + r;
+    return ((r >> 4) & 1) * p.channels + tile.channel0 + (r >> 5) * 16 + (r & 15);
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void *tmap, uint32_t bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+// four rows of the matrix, any four, behind one another
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const void *tmap, uint32_t bar, int c0, int4 rows) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+        ::"r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w)
+        : "memory");
+}
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void store_cluster(uint32_t dst, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(v) : "memory");
+}
+__device__ __forceinline__ void time_out(int code) { atomicExch(&g_expert_error, code); }
+
+// ---- loader warps: 16 bytes of a row, zeros behind its end, for any alignment ----------------------
+__device__ __noinline__ uint4 load_chunk_edge(const uint8_t *row, long long byte0, long long row_bytes, int esize) {
+    uint4 out = make_uint4(0, 0, 0, 0);
+    uint32_t *words = reinterpret_cast<uint32_t *>(&out);
+    for (int b = 0; b < 16; b += esize) {
+        if (byte0 + b >= row_bytes) break;
+        uint32_t v;
+        if (esize == 1) v = row[byte0 + b];
+        else if (esize == 2) v = *reinterpret_cast<const uint16_t *>(row + byte0 + b);
+        else v = *reinterpret_cast<const uint32_t *>(row + byte0 + b);
+        words[b >> 2] |= v << (8 * (b & 3));
+    }
+    return out;
+}
+__device__ __forceinline__ uint4 load_chunk(const uint8_t *row, long long byte0, long long row_bytes, int esize) {
+    const uint8_t *at = row + byte0;
+    const uint32_t skew = uint32_t(reinterpret_cast<uintptr_t>(at)) & 15u;
+    if (skew == 0 && byte0 + 16 <= row_bytes) return __ldg(reinterpret_cast<const uint4 *>(at));
+    if (byte0 >= row_bytes) return make_uint4(0, 0, 0, 0);
+    // aligned words around the chunk, shifted into place; all of them inside the row
+    if (byte0 >= 4 && byte0 + 20 <= row_bytes) {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(at - (skew & 3u));
+        const uint32_t shift = 8 * (skew & 3u);
+        const uint32_t a = __ldg(w), b = __ldg(w + 1), c = __ldg(w + 2), d = __ldg(w + 3), e = __ldg(w + 4);
+        return make_uint4(__funnelshift_r(a, b, shift), __funnelshift_r(b, c, shift), __funnelshift_r(c, d, shift),
+                          __funnelshift_r(d, e, shift));
+    }
+    return load_chunk_edge(row, byte0, row_bytes, esize);
+}
+
+// x = hi + lo + (less than 2^-22 |x|), both TF32.  An infinity or NaN is all in hi.
+__device__ __forceinline__ void split_tf32(float x, float *hi, float *lo) {
+    float h = round_tf32(x);
+    if (!(fabsf(h) <= 3.402823466e38f)) h = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u);
+    *hi = h;
+    *lo = fabsf(h) <= 3.402823466e38f ? round_tf32(x - h) : 0.0f;
+}
+
+__device__ __noinline__ float act_far(float v, int act) {
+    if (act == 2) return 1.0f / (1.0f + __expf(-v));
+    return tanhf(v);
+}
+__device__ __forceinline__ float apply_act(float v, int act) {
+    if (act == 0) return v;
+    if (act == 1) return fmaxf(v, 0.0f);
+    if (act == 4) return __fdividef(v, 1.0f + __expf(-v));
+    return act_far(v, act);
+}
+
+__device__ __forceinline__ void store_out(void *y, Elem type, long long at, float v) {
+    if (type == Elem::BF16) static_cast<__nv_bfloat16 *>(y)[at] = __float2bfloat16_rn(v);
+    else if (type == Elem::F16) static_cast<__half *>(y)[at] = __float2half_rn(v);
+    else static_cast<float *>(y)[at] = v;
+}
+
+template <int KIND, bool TMA>
+__global__ void __launch_bounds__(TMA ? kTmaThreads : kLoadThreads, 1)
+expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const GroupedParams p,
+                 const MmGeom t) {
+    constexpr int kThreadCount = TMA ? kTmaThreads : kLoadThreads;
+    constexpr int kPlanes = KIND == kX3 ? 2 : 1;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ float row_scale_s[2][256];
+    __shared__ uint32_t live_s[2][8];
+    __shared__ uint32_t tmem_slot;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *generic = smem_raw + (base - smem_u32(smem_raw));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t b_bytes = uint32_t(t.tn) * kRowBytes;
+    const uint32_t stage_bytes = kPlanes * (kATileBytes + b_bytes);
+    const uint32_t full0 = base + t.bar_off, empty0 = full0 + 8u * t.stages;
+    const uint32_t acc_full0 = empty0 + 8u * t.stages, acc_empty0 = acc_full0 + 16u;
+    const uint32_t recv_full = acc_empty0 + 16u, recv_free = recv_full + 8u;
+    int *first = reinterpret_cast<int *>(generic + t.table_off);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < t.stages; ++s) {
+            mbar_init(full0 + 8u * s, TMA ? 2 : kLoaderWarps);
+            mbar_init(empty0 + 8u * s, 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(acc_full0 + 8u * a, 1);
+            mbar_init(acc_empty0 + 8u * a, kEpilogueWarps);
+        }
+        mbar_init(recv_full, uint32_t(kEpilogueWarps * t.cluster));
+        mbar_init(recv_free, uint32_t(kEpilogueWarps * t.cluster));
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 2) {
+        tmem_alloc(smem_u32(&tmem_slot), uint32_t(t.tmem_cols));
+        tmem_relinquish();
+    }
+    grid_dependency_entry();
+    build_table(p, t, first, kThreadCount);
+    tc_fence_before();
+    __syncthreads();
+    if (t.cluster > 1) cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const int total_tiles = first[p.groups];
+    const int rank = t.cluster > 1 ? int(cluster_cta_rank()) : 0;
+    const int tile0 = int(blockIdx.x) / t.cluster, tile_step = int(gridDim.x) / t.cluster;
+    const int k_begin = t.k_steps * rank / t.cluster, k_end = t.k_steps * (rank + 1) / t.cluster;
+    const int k_elems = kRowBytes / t.esize;
+
+    if (TMA && warp == 0) {
+        // ---------------- weights ----------------
+        if (lane == 0) {
+            int s = 0;
+            uint32_t phase = 1;
+            int armed = 0;
+            bool ok = true;
+            for (int i = tile0; i < total_tiles && ok; i += tile_step) {
+                const Tile tile = find_tile(p, t, first, i);
+                for (int k = k_begin; k < k_end; ++k) {
+                    ok = mbar_wait(empty0 + 8u * s, phase, nullptr);
+                    if (!ok) break;
+                    const uint32_t dst = base + t.stage_off + uint32_t(s) * stage_bytes, bar = full0 + 8u * s;
+                    mbar_expect_tx(bar, kATileBytes);
+                    if (!p.gated) {
+                        tma_load_3d(dst, &map_w, bar, k * k_elems, tile.channel0, tile.group);
+                    } else {
+#pragma unroll
+                        for (int b = 0; b < 8; ++b)
+                            tma_load_3d(dst + uint32_t(b) * 16u * kRowBytes, &map_w, bar, k * k_elems, weight_row(p, tile, b * 16), tile.group);
+                    }
+                    ++armed;
+                    if (++s == t.stages) { s = 0; phase ^= 1u; }
+                }
             }
-            xs[k][r] = v;
-            for (int h = 0; h < halves; ++h) {
-                Sum u = 0;
-                if (n0 + r < p.channels && k0 + k < p.inner)
-                    u = widen(w[((long long)h * p.channels + n0 + r) * p.w_stride + k0 + k]);
-                ws[h][k][r] = u;
+            if (!ok) {
+                time_out(1);
+                for (int j = armed - 1, n = 0; j >= 0 && n < t.stages; --j, ++n)
+                    mbar_wait(full0 + 8u * (j % t.stages), uint32_t((j / t.stages) & 1), nullptr);
             }
         }
-        __syncthreads();
-        for (int k = 0; k < kStep; ++k)
-            for (int h = 0; h < halves; ++h)
+    } else if (TMA && warp == 3) {
+        // ---------------- rows ----------------
+        int s = 0;
+        uint32_t phase = 1;
+        int armed = 0;
+        bool ok = true;
+        for (int i = tile0; i < total_tiles && ok; i += tile_step) {
+            const Tile tile = find_tile(p, t, first, i);
+            const int loads = p.rows ? (tile.valid + 3) / 4 : (tile.valid + t.box_rows - 1) / t.box_rows;
+            const uint32_t bytes = uint32_t(loads) * (p.rows ? 4 : t.box_rows) * kRowBytes;
+            int4 src[2];
+            if (p.rows) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int j = 0; j < 2; ++j) {
+                    int at[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[h][i][j] += xs[k][tr + i] * ws[h][k][tc + j];
-        __syncthreads();
-    }
-    const int per_group = halves * p.channels;
-    for (int i = 0; i < 4; ++i) {
-        const int r = row0 + tr + i;
-        if (r >= end) continue;
-        const long long src = p.rows ? p.rows[r] : r;
-        const float rs = p.row_scale && src >= 0 && src < p.x_rows ? p.row_scale[src] : 1.0f;
-        for (int j = 0; j < 4; ++j) {
-            const int n = n0 + tc + j;
-            if (n >= p.channels) continue;
-            float v[2] = {0.0f, 1.0f};
-            for (int h = 0; h < halves; ++h) {
-                const long long at = (long long)g * per_group + h * p.channels + n;
-                v[h] = float(acc[h][i][j]) * rs;
-                if (p.channel_scale) v[h] *= p.channel_scale[at];
-                if (p.bias) v[h] += p.bias[at];
+                    for (int q = 0; q < 4; ++q) {
+                        const int c = min((j * 32 + lane) * 4 + q, tile.valid - 1);
+                        const int r = p.rows[tile.row0 + c];
+                        at[q] = r >= 0 && r < p.x_rows ? r : 0;      // a missing row is zeroed by the epilogue
+                    }
+                    src[j] = make_int4(at[0], at[1], at[2], at[3]);
+                }
             }
-            const float out = apply_act(v[0], p.act) * v[1];
-            const long long at = (long long)r * p.y_stride + n;
-            if (p.out_type == Elem::F32) static_cast<float *>(p.y)[at] = out;
-            else if (p.out_type == Elem::F16) static_cast<__half *>(p.y)[at] = __float2half_rn(out);
-            else static_cast<__nv_bfloat16 *>(p.y)[at] = __float2bfloat16_rn(out);
+            for (int k = k_begin; k < k_end; ++k) {
+                ok = mbar_wait(empty0 + 8u * s, phase, nullptr);
+                ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
+                if (!ok) break;
+                const uint32_t dst = base + t.stage_off + uint32_t(s) * stage_bytes + kATileBytes, bar = full0 + 8u * s;
+                if (lane == 0) mbar_expect_tx(bar, bytes);
+                __syncwarp();
+                if (p.rows) {
+                    if (lane < loads) tma_gather4(dst + uint32_t(lane) * 4u * kRowBytes, &map_x, bar, k * k_elems, src[0]);
+                    if (lane + 32 < loads) tma_gather4(dst + uint32_t(lane + 32) * 4u * kRowBytes, &map_x, bar, k * k_elems, src[1]);
+                } else if (lane < loads) {
+                    tma_load_2d(dst + uint32_t(lane) * uint32_t(t.box_rows) * kRowBytes, &map_x, bar, k * k_elems, tile.row0 + lane * t.box_rows);
+                }
+                ++armed;
+                if (++s == t.stages) { s = 0; phase ^= 1u; }
+            }
         }
+        if (!ok) {
+            if (lane == 0) time_out(2);
+            for (int j = armed - 1, n = 0; j >= 0 && n < t.stages; --j, ++n)
+                mbar_wait(full0 + 8u * (j % t.stages), uint32_t((j / t.stages) & 1), nullptr);
+        }
+    } else if (!TMA && warp >= 8) {
+        // ---------------- loader warps ----------------
+        // thread i of 256 moves 16-byte column i % 8 of rows i / 8, i / 8 + 32, ...: four of the weights, up to four of x
+        const int tid = int(threadIdx.x) - 256, c16 = tid & 7, r0 = tid >> 3;
+        const long long row_bytes = (long long)p.inner * t.esize;
+        int s = 0;
+        uint32_t phase = 1;
+        bool ok = true;
+        for (int i = tile0; i < total_tiles && ok; i += tile_step) {
+            const Tile tile = find_tile(p, t, first, i);
+            const int wide = p.gated ? 2 * p.channels : p.channels;
+            const uint8_t *src[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int r = weight_row(p, tile, r0 + 32 * j);
+                const uint8_t *w = static_cast<const uint8_t *>(p.w) + ((long long)tile.group * p.w_group_stride + (long long)r * p.w_stride) * t.esize;
+                src[j] = r < wide ? w : nullptr;
+                const int c = r0 + 32 * j;
+                src[4 + j] = nullptr;
+                if (c < tile.valid) {
+                    const int at = p.rows ? p.rows[tile.row0 + c] : tile.row0 + c;
+                    if (at >= 0 && at < p.x_rows) src[4 + j] = static_cast<const uint8_t *>(p.x) + (long long)at * p.x_stride * t.esize;
+                }
+            }
+            uint4 now[8], next[8];
+            auto fetch = [&](uint4 *v, int k) {
+                const long long byte0 = (long long)k * kRowBytes + c16 * 16;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = src[j] ? load_chunk(src[j], byte0, row_bytes, t.esize) : make_uint4(0, 0, 0, 0);
+            };
+            fetch(now, k_begin);
+            for (int k = k_begin; k < k_end; ++k) {
+                if (k + 1 < k_end) fetch(next, k + 1);
+                ok = mbar_wait(empty0 + 8u * s, phase, nullptr);
+                ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
+                if (!ok) break;
+                uint8_t *stage = generic + t.stage_off + size_t(s) * stage_bytes;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int r = r0 + 32 * (j & 3);
+                    if (j >= 4 && r >= tile.cols) continue;
+                    uint8_t *dst = stage + (j < 4 ? 0 : kPlanes * kATileBytes) + sw128_offset(r, c16);
+                    if (KIND != kX3) {
+                        *reinterpret_cast<uint4 *>(dst) = now[j];
+                    } else {
+                        float4 hi, lo;
+                        split_tf32(__uint_as_float(now[j].x), &hi.x, &lo.x);
+                        split_tf32(__uint_as_float(now[j].y), &hi.y, &lo.y);
+                        split_tf32(__uint_as_float(now[j].z), &hi.z, &lo.z);
+                        split_tf32(__uint_as_float(now[j].w), &hi.w, &lo.w);
+                        *reinterpret_cast<float4 *>(dst) = hi;
+                        *reinterpret_cast<float4 *>(dst + (j < 4 ? uint32_t(kATileBytes) : b_bytes)) = lo;
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full0 + 8u * s);
+                if (++s == t.stages) { s = 0; phase ^= 1u; }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) now[j] = next[j];
+            }
+        }
+        if (!ok && lane == 0) time_out(3);
+    } else if (warp == 1) {
+        // ---------------- MMA issuer ----------------
+        if (lane == 0) {
+            int s = 0;
+            uint32_t phase = 0;
+            int turn = 0;                                       // accumulator hand-overs so far
+            bool ok = true;
+            for (int i = tile0; i < total_tiles && ok; i += tile_step) {
+                const Tile tile = find_tile(p, t, first, i);
+                // sums in float32 / int32 (bit 4 / 5), operand formats, both K-major, N and M
+                const uint32_t idesc = (KIND == kI8 ? 2u << 4 : 1u << 4) | (t.format << 7) | (t.format << 10) |
+                                       (uint32_t(tile.cols >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
+                uint32_t acc = 0;
+                for (int k = k_begin; k < k_end && ok; ++k) {
+                    const bool opens = KIND == kX3 ? (k - k_begin) % kChunkSteps == 0 : k == k_begin;
+                    const bool closes = k + 1 == k_end || (KIND == kX3 && (k - k_begin) % kChunkSteps == kChunkSteps - 1);
+                    const uint32_t a = uint32_t(turn) & 1u;
+                    const uint32_t d = tmem + a * uint32_t(t.tn);
+                    if (opens) {
+                        ok = mbar_wait(acc_empty0 + 8u * a, ((uint32_t(turn) >> 1) & 1u) ^ 1u, nullptr);
+                        tc_fence_after();
+                        acc = 0;
+                    }
+                    if (ok) ok = mbar_wait(full0 + 8u * s, phase, nullptr);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t stage = base + t.stage_off + uint32_t(s) * stage_bytes;
+                    const uint64_t da = smem_desc_kmajor(stage, 128), db = smem_desc_kmajor(stage + kPlanes * kATileBytes, 128);
+                    const uint64_t da_lo = smem_desc_kmajor(stage + kATileBytes, 128);
+                    const uint64_t db_lo = smem_desc_kmajor(stage + kPlanes * kATileBytes + b_bytes, 128);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const uint64_t o = uint64_t(q * 2);
+                        if (KIND == kF16) umma_f16(d, da + o, db + o, idesc, acc);
+                        else if (KIND == kI8) umma_i8(d, da + o, db + o, idesc, acc);
+                        else {
+                            umma_tf32(d, da_lo + o, db + o, idesc, acc);
+                            umma_tf32(d, da + o, db_lo + o, idesc, 1u);
+                            umma_tf32(d, da + o, db + o, idesc, 1u);
+                        }
+                        acc = 1;
+                    }
+                    umma_commit(empty0 + 8u * s);
+                    if (closes) {
+                        umma_commit(acc_full0 + 8u * a);
+                        ++turn;
+                    }
+                    if (++s == t.stages) { s = 0; phase ^= 1u; }
+                }
+            }
+            if (!ok) time_out(4);
+        }
+    } else if (warp >= 4 && warp < 8) {
+        // ---------------- epilogue ----------------
+        const int quad = warp & 3, tid = int(threadIdx.x) - 128, lane_row = quad * 32 + lane;
+        const uint32_t lane_tmem = tmem + (uint32_t(quad * 32) << 16);
+        const uint32_t recv = base + t.recv_off;
+        float *recv_generic = reinterpret_cast<float *>(generic + t.recv_off);
+        const bool per_row = p.row_scale || p.rows;
+        int turn = 0, round = 0;
+        bool ok = true;
+        for (int i = tile0; i < total_tiles && ok; i += tile_step, ++round) {
+            const Tile tile = find_tile(p, t, first, i);
+            const int half = p.gated ? (lane >> 4) : 0;
+            const int channel = p.gated ? tile.channel0 + quad * 16 + (lane & 15) : tile.channel0 + lane_row;
+            const bool in_channels = channel < p.channels;
+            const long long per_channel = (long long)tile.group * (p.gated ? 2 : 1) * p.channels + (long long)half * p.channels + channel;
+            const float channel_scale = p.channel_scale && in_channels ? p.channel_scale[per_channel] : 1.0f;
+            const float bias = p.bias && in_channels ? p.bias[per_channel] : 0.0f;
+            const int slot = round & 1;
+            if (per_row) {
+                for (int c = tid; c < max(t.tn, 32); c += 128) {           // whole warps
+                    const int src = c < tile.valid ? (p.rows ? p.rows[tile.row0 + c] : tile.row0 + c) : -1;
+                    const bool live = src >= 0 && src < p.x_rows;
+                    row_scale_s[slot][c] = live && p.row_scale ? p.row_scale[src] : 1.0f;
+                    const uint32_t mask = __ballot_sync(0xffffffffu, live);
+                    if (lane == 0) live_s[slot][c >> 5] = mask;
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+            }
+            // a finished sum of column c: scales, bias, activation, store
+            auto value = [&](float raw, int c) {
+                float v = KIND == kI8 ? float(__float_as_int(raw)) : raw;
+                if (per_row) {
+                    if (!((live_s[slot][c >> 5] >> (c & 31)) & 1u)) v = 0.0f;
+                    v *= row_scale_s[slot][c];
+                }
+                return v * channel_scale + bias;
+            };
+            auto put = [&](int c, float v) {
+                if (in_channels && c < tile.valid) store_out(p.y, p.out_type, (long long)(tile.row0 + c) * p.y_stride + channel, v);
+            };
+            // two neighbouring columns c, c + 1
+            auto finish = [&](float raw0, float raw1, int c) {
+                if (c >= tile.valid) return;
+                const float v0 = value(raw0, c), v1 = value(raw1, c + 1);
+                if (!p.gated) {
+                    put(c, apply_act(v0, p.act));
+                    put(c + 1, apply_act(v1, p.act));
+                } else {
+                    // the lower half of the warp finishes column c, the upper half column c + 1
+                    const float other = __shfl_xor_sync(0xffffffffu, half ? v0 : v1, 16);
+                    const float gate = half ? other : v0, up = half ? v1 : other;
+                    put(c + half, apply_act(gate, p.act) * up);
+                }
+            };
+            if (KIND == kX3) {
+                float sum[kLoaderCols];
+#pragma unroll
+                for (int c = 0; c < kLoaderCols; ++c) sum[c] = 0.0f;
+                for (int k = k_begin; k < k_end && ok; k += kChunkSteps, ++turn) {
+                    const uint32_t a = uint32_t(turn) & 1u;
+                    ok = mbar_wait(acc_full0 + 8u * a, (uint32_t(turn) >> 1) & 1u, nullptr);
+                    ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int c0 = 0; c0 < kLoaderCols; c0 += 16)
+                        if (c0 < tile.cols) {
+                            float v[16];
+                            tmem_ld16(lane_tmem + a * uint32_t(t.tn) + c0, v);
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) sum[c0 + c] += v[c];
+                        }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(acc_empty0 + 8u * a);
+                }
+                if (!ok) break;
+                if (t.cluster == 1) {
+#pragma unroll
+                    for (int c = 0; c < kLoaderCols; c += 2)
+                        if (c < tile.cols) finish(sum[c], sum[c + 1], c);
+                } else {
+                    ok = round == 0 || mbar_wait_cluster(recv_free, uint32_t(round - 1) & 1u, nullptr);
+                    ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
+                    if (!ok) break;
+                    const int per = tile.cols / t.cluster;
+#pragma unroll
+                    for (int c = 0; c < kLoaderCols; ++c)
+                        if (c < tile.cols)
+                            store_cluster(cluster_map(recv + uint32_t((rank * per + c % per) * kTileM + lane_row) * 4u, uint32_t(c / per)), sum[c]);
+                }
+            } else {
+                const uint32_t a = uint32_t(turn) & 1u;
+                ok = mbar_wait(acc_full0 + 8u * a, (uint32_t(turn) >> 1) & 1u, nullptr);
+                if (ok && t.cluster > 1 && round > 0) ok = mbar_wait_cluster(recv_free, uint32_t(round - 1) & 1u, nullptr);
+                ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
+                if (!ok) break;
+                tc_fence_after();
+                const int per = tile.cols / t.cluster;
+                for (int c0 = 0; c0 < tile.cols; c0 += 16) {
+                    float v[16];
+                    tmem_ld16(lane_tmem + a * uint32_t(t.tn) + c0, v);
+                    if (t.cluster == 1) {
+#pragma unroll
+                        for (int c = 0; c < 16; c += 2) finish(v[c], v[c + 1], c0 + c);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) {
+                            const int d = (c0 + c) / per;
+                            store_cluster(cluster_map(recv + uint32_t((rank * per + c0 + c - d * per) * kTileM + lane_row) * 4u, uint32_t(d)), v[c]);
+                        }
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty0 + 8u * a);
+                ++turn;
+            }
+            if (t.cluster > 1) {
+                // this CTA's columns: the partial sums of all ranks, added in rank order
+                const int per = tile.cols / t.cluster;
+                __syncwarp();
+                if (lane < t.cluster) mbar_arrive_cluster(cluster_map(recv_full, uint32_t(lane)));
+                ok = mbar_wait_cluster(recv_full, uint32_t(round) & 1u, nullptr);
+                ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
+                if (!ok) break;
+                for (int c = 0; c < per; c += 2) {
+                    float v[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float f = 0.0f;
+                        int n = 0;
+                        for (int q = 0; q < t.cluster; ++q) {
+                            const float part = recv_generic[(q * per + c + j) * kTileM + lane_row];
+                            if (KIND == kI8) n += __float_as_int(part);
+                            else f += part;
+                        }
+                        v[j] = KIND == kI8 ? __int_as_float(n) : f;
+                    }
+                    finish(v[0], v[1], rank * per + c);
+                }
+                __syncwarp();
+                if (lane < t.cluster) mbar_arrive_cluster(cluster_map(recv_free, uint32_t(lane)));
+            }
+        }
+        if (!ok && lane == 0) time_out(5);
     }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (t.cluster > 1) cluster_sync_all();       // nobody may still push into the shared memory of a CTA that has gone
+    if (warp == 2) {
+        tc_fence_after();
+        tmem_dealloc(tmem, uint32_t(t.tmem_cols));
+    }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+    static const EncodeTiledFn fn = [] {
+        void *sym = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            sym = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(sym);
+    }();
+    return fn;
+}
+
+// A tensor map of a matrix (or a stack of them) with rows of `inner` elements; boxes of one swizzle row x box_rows.
+bool encode(CUtensorMap *map, Elem type, const void *base, long long inner, long long rows, long long row_bytes, long long stack,
+            long long stack_bytes, int box_rows, int rank) {
+    const CUtensorMapDataType types[] = {CU_TENSOR_MAP_DATA_TYPE_FLOAT32, CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                                         CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_DATA_TYPE_UINT8};
+    const cuuint64_t dims[3] = {cuuint64_t(inner), cuuint64_t(rows), cuuint64_t(stack)};
+    const cuuint64_t strides[2] = {cuuint64_t(row_bytes), cuuint64_t(stack_bytes)};
+    const cuuint32_t box[3] = {cuuint32_t(kRowBytes / elem_size(type)), cuuint32_t(box_rows), 1};
+    const cuuint32_t steps[3] = {1, 1, 1};
+    return encode_fn()(map, types[int(type)], cuuint32_t(rank), const_cast<void *>(base), dims, strides, box, steps,
+                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// May TMA read rows of this stride?  (16-byte aligned rows that do not overlap, strides below 2^40 bytes)
+bool tma_rows(const void *base, long long stride, int inner, int esize) {
+    const long long bytes = stride * esize;
+    return reinterpret_cast<uintptr_t>(base) % 16 == 0 && bytes % 16 == 0 && stride >= inner && bytes < (1LL << 40);
+}
+
+int ceil_div(long long a, long long b) { return int((a + b - 1) / b); }
+
+bool tma_able(const GroupedParams &p) {
+    const int esize = elem_size(p.type);
+    const long long wide = p.gated ? 2 * p.channels : p.channels, group_bytes = p.w_group_stride * esize;
+    return p.type != Elem::F32 && p.x_rows > 0 && tma_rows(p.x, p.x_stride, p.inner, esize) && tma_rows(p.w, p.w_stride, p.inner, esize) &&
+           (p.groups == 1 || (group_bytes % 16 == 0 && p.w_group_stride >= wide * p.w_stride && group_bytes < (1LL << 40)));
+}
+
+// Columns of a tile: the smallest power of two that holds an average group, so that most groups read their weights once.
+int columns_for(const GroupedParams &p, int most) {
+    const int average = ceil_div(p.total, std::min(p.groups, p.total));
+    int tn = 16;
+    while (tn < average && tn < most) tn *= 2;
+    return tn;
+}
+
+// Chooses the tiling; touches no device.  Returns the CTAs to launch.
+int choose(const GroupedParams &p, int sm_count, bool tma, MmGeom *t) {
+    const int esize = elem_size(p.type);
+    t->esize = esize;
+    t->format = p.type == Elem::BF16 ? 1u : p.type == Elem::F16 ? 0u : p.type == Elem::S8 ? 1u : 2u;
+    t->tile_channels = p.gated ? kTileM / 2 : kTileM;
+    t->n_tiles = ceil_div(p.channels, t->tile_channels);
+    t->k_steps = ceil_div((long long)p.inner * esize, kRowBytes);
+    const int busy = std::min(p.groups, p.total);
+    t->tn = columns_for(p, tma ? 256 : kLoaderCols);
+    auto tiles = [&]() { return (long long)t->n_tiles * std::max<long long>(busy, ceil_div(p.total, t->tn)); };
+    if (tiles() < sm_count && t->tn > 128) t->tn = 128;
+    // K split: as long as it fills SMs that would idle and leaves every CTA two K steps
+    t->cluster = 1;
+    while (t->cluster < 8 && t->tn <= 128 && tiles() * t->cluster * 2 <= sm_count && t->k_steps >= 4 * t->cluster) t->cluster *= 2;
+    t->box_rows = std::min(t->tn, 64);
+    t->tmem_cols = std::max(32, 2 * t->tn);
+    const int planes = p.type == Elem::F32 ? 2 : 1;
+    const size_t stage = size_t(planes) * (kATileBytes + t->tn * kRowBytes);
+    const size_t recv = t->cluster > 1 ? size_t(t->tn) * kTileM * sizeof(float) : 0;
+    const size_t table = (size_t(p.groups + 1) * sizeof(int) + 15) / 16 * 16;
+    const size_t fixed = 1024 + recv + table + 2 * kMaxStages * 8 + 64 + 4096;       // 4096: the kernel's static shared memory
+    t->stages = int(std::min<size_t>(kMaxStages, (kSmemLimit - fixed) / stage));
+    t->stage_off = 0;
+    t->recv_off = int(t->stages * stage);
+    t->table_off = int(t->recv_off + recv);
+    t->bar_off = int(t->table_off + table);
+    const long long most = (long long)t->n_tiles * (p.total / t->tn + busy);         // no distribution needs more
+    return int(std::min<long long>(sm_count / t->cluster, most)) * t->cluster;
+}
+
+template <int KIND, bool TMA>
+cudaError_t run(const GroupedParams &p, const MmGeom &t, int ctas, const CUtensorMap &map_w, const CUtensorMap &map_x, cudaStream_t stream) {
+    const int smem = t.bar_off + 2 * kMaxStages * 8 + 64 + 1024;
+    const auto kernel = expert_mm_kernel<KIND, TMA>;
+    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (err != cudaSuccess) return err;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(unsigned(ctas));
+    config.blockDim = dim3(TMA ? kTmaThreads : kLoadThreads);
+    config.dynamicSmemBytes = size_t(smem);
+    config.stream = stream;
+    cudaLaunchAttribute attribute = {};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = unsigned(t.cluster);
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, map_w, map_x, p, t);
 }
 
 }  // namespace
 
-cudaError_t launch_grouped(const GroupedParams &p, cudaStream_t stream) {
-    const long long tiles = (p.total + kTile - 1) / kTile + (p.offsets ? p.groups : 0);
-    const dim3 grid(unsigned(tiles), unsigned((p.channels + kTile - 1) / kTile));
-    switch (p.type) {
-        case Elem::F32: grouped_kernel<float><<<grid, kThreads, 0, stream>>>(p); break;
-        case Elem::F16: grouped_kernel<__half><<<grid, kThreads, 0, stream>>>(p); break;
-        case Elem::BF16: grouped_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(p); break;
-        case Elem::S8: grouped_kernel<signed char><<<grid, kThreads, 0, stream>>>(p); break;
+bool grouped_too_large(const GroupedParams &p) {
+    return p.total > 0 && (long long)ceil_div(p.total, columns_for(p, kLoaderCols)) * ceil_div(p.channels, kTileM / 2) > kMaxGroupTiles;
+}
+
+cudaError_t launch_grouped(const GroupedParams &given, cudaStream_t stream) {
+    int device = 0, sm_count = 0;
+    cudaError_t err = cudaGetDevice(&device);
+    if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, device);
+    if (err != cudaSuccess) return err;
+    GroupedParams p = given;
+    const int wide = p.gated ? 2 * p.channels : p.channels;
+    // a stride that separates nothing may hold anything
+    const int apart = (p.inner + 15) / 16 * 16;
+    if (p.x_rows <= 1) p.x_stride = apart;
+    if (wide == 1) p.w_stride = apart;
+    MmGeom t = {};
+    bool tma = tma_able(p) && encode_fn();
+    int ctas = choose(p, sm_count, tma, &t);
+    alignas(64) CUtensorMap map_w = {}, map_x = {};
+    if (tma) {
+        const long long stack_bytes = p.groups == 1 ? 16 : p.w_group_stride * t.esize;
+        if (!encode(&map_w, p.type, p.w, p.inner, wide, p.w_stride * t.esize, p.groups, stack_bytes, p.gated ? 16 : kTileM, 3) ||
+            !encode(&map_x, p.type, p.x, p.inner, p.x_rows, p.x_stride * t.esize, 1, 0, p.rows ? 1 : t.box_rows, 2)) {
+            tma = false;                             // a shape that no tensor map describes
+            ctas = choose(p, sm_count, tma, &t);
+        }
     }
-    return cudaGetLastError();
+    if (p.type == Elem::F32) return run<kX3, false>(p, t, ctas, map_w, map_x, stream);
+    if (p.type == Elem::S8)
+        return tma ? run<kI8, true>(p, t, ctas, map_w, map_x, stream) : run<kI8, false>(p, t, ctas, map_w, map_x, stream);
+    return tma ? run<kF16, true>(p, t, ctas, map_w, map_x, stream) : run<kF16, false>(p, t, ctas, map_w, map_x, stream);
+}
+
+cudaError_t expert_mm_status(cudaStream_t stream, int *code) {
+    cudaError_t err = cudaMemcpyFromSymbolAsync(code, g_expert_error, sizeof *code, 0, cudaMemcpyDeviceToHost, stream);
+    if (err == cudaSuccess) err = cudaStreamSynchronize(stream);
+    if (err == cudaSuccess && *code != 0) {
+        const int zero = 0;
+        err = cudaMemcpyToSymbol(g_expert_error, &zero, sizeof zero);
+    }
+    return err;
 }
 
 }  // namespace ios

@@ -80,5 +80,9 @@ struct GroupedParams {
     long long y_stride;
 };
 cudaError_t launch_grouped(const GroupedParams &p, cudaStream_t stream);
+// more tiles than the kernel's table counts
+bool grouped_too_large(const GroupedParams &p);
+// Waits for the stream; *code: the wait that ran out in a product on the current device since the last call, 0 for none.
+cudaError_t expert_mm_status(cudaStream_t stream, int *code);
 
 }  // namespace ios

@@ -34,6 +34,7 @@ def declare(handle):
     handle.ios_matmul_int8.argtypes = [_PTR, _LONG, _PTR, _LONG, _INT, _INT, _INT, _PTR, _PTR, _PTR, _INT, _PTR, _INT,
                                        _LONG, _PTR]
     handle.ios_quantize_rows.argtypes = [_PTR, _INT, _LONG, _LONG, _INT, _PTR, _LONG, _PTR, _LONG, _PTR, _PTR]
+    handle.ios_device_ops_status.argtypes = [_INT, _PTR]
     handle.ios_combine_experts.argtypes = [_PTR, _INT, _LONG, _LONG, _PTR, _PTR, _LONG, _INT, _INT, _PTR, _INT, _LONG, _PTR]
 
 
@@ -259,3 +260,10 @@ def combine_experts(y, gates, slots, out_dtype=None, out=None):
     _call('ios_combine_experts', y.data_ptr(), code, y.shape[0], y.stride(0), gates_at, slots_at, tokens, k, y.shape[1],
           out.data_ptr(), _Torch.codes[out_dtype], out.stride(0), _stream(device))
     return out
+
+
+def device_ops_status(device=None):
+    """Waits for torch's current stream of ``device`` and raises if a bounded wait inside a product ran out since the last call."""
+    torch = _Torch.get()
+    index = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    _call('ios_device_ops_status', index, _stream(index))

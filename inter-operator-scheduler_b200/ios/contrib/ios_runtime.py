@@ -24,7 +24,8 @@ import numpy as np
 from ios.ir import Conv, Graph, Block, Node
 from .ctypes_utils import c_string, c_string_list, c_ndarray_list, get_nodes_by_type
 from . import device_ops
-from .device_ops import Routing, combine_experts, grouped_matmul, matmul_int8, quantize_rows, route_experts  # noqa: F401
+from .device_ops import (Routing, combine_experts, device_ops_status, grouped_matmul, matmul_int8,  # noqa: F401
+                         quantize_rows, route_experts)
 
 cur_dir = os.path.dirname(os.path.abspath(os.path.realpath(__file__)))
 
