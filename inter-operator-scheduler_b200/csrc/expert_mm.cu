@@ -11,16 +11,17 @@
 // * Products too small to fill the GPU split K over a thread-block cluster: the CTAs deal the tile's columns among
 //   themselves, push their partial sums into the shared memory of the CTA that finishes a column, and that CTA adds them
 //   in rank order.  No workspace, no counters, the same bits every time.
-// * Operands arrive by TMA where their rows start on 16-byte boundaries -- rows gathered by index through
-//   tile::gather4 -- and through registers of eight loader warps otherwise.
+// * Operands arrive by TMA where their rows start on 16-byte boundaries; rows gathered by index then by cp.async of four
+//   warps (tile::gather4 moves 512 bytes per instruction and took 68 cycles for each: 1480 us where this takes @GATHER@ us, 4096
+//   tokens x 8 of 64 experts, gated, 2048 -> 1280).  Anything else goes through registers of eight loader warps.
 // * float32: every operand is split into two TF32 numbers on its way into shared memory (loader warps); three products
 //   a_hi b_hi + a_hi b_lo + a_lo b_hi.  The tensor core truncates where it adds, so the sum over more than 128 elements is
 //   formed in registers, rounded to nearest, from partial sums over 128.
 // * gated: 16 rows of the gate half and the 16 rows of the same channels of the other half alternate in the tile, so that
 //   a lane and the lane 16 further on hold the two factors of one result.
 //
-// Warp roles: 0 = weight loads, 1 = MMA issuer, 2 = tensor memory, 3 = row loads, 4..7 = epilogue, 8..15 = loaders (only
-// where TMA cannot be used).  Every wait is bounded; on a time-out the device's error word is set, loads in flight are
+// Warp roles: 0 = weight loads, 1 = MMA issuer, 2 = tensor memory, 3 = row loads, 4..11 (4..7) = epilogue, then
+// gathering or loader warps.  Every wait is bounded; on a time-out the device's error word is set, loads in flight are
 // waited for, tensor memory is freed and the kernel returns.
 #include "expert_ops.h"
 #include "kernels.h"
@@ -35,10 +36,18 @@ namespace ios {
 namespace {
 
 enum Kind { kF16 = 0, kI8 = 1, kX3 = 2 };       // instruction: 16-bit floats, 8-bit integers, three TF32 products
+enum Loads { kTma = 0, kGather = 1, kRegs = 2 };  // operands by TMA / gathered rows by cp.async warps / all through registers
 
-constexpr int kEpilogueWarps = 4, kLoaderWarps = 8;
-constexpr int kTmaThreads = 256, kLoadThreads = 512;
+constexpr int kGatherWarps = 4, kLoaderWarps = 8;
+constexpr int kMaxThreads = 512;
+// Two epilogue warps per lane quarter share a tile's columns; one beside the loader warps, which need the registers.
+__host__ __device__ constexpr int epilogue_warps(int loads) { return loads == kRegs ? 4 : 8; }
+__host__ __device__ constexpr int threads_of(int loads) {
+    return 32 * (4 + epilogue_warps(loads) + (loads == kTma ? 0 : loads == kGather ? kGatherWarps : kLoaderWarps));
+}
 constexpr int kLoaderCols = 128;                // widest tile of the loader warps (their registers hold a step)
+constexpr int kStageCols = 32;                  // columns an epilogue warp turns round at a time
+constexpr int kTurnBytes = kStageCols * 32 * 2; // ... in this much shared memory (float32: in two halves)
 constexpr int kChunkSteps = 4;                  // float32: K steps per partial sum
 constexpr int kMaxStages = 12;
 constexpr int kMaxGroupTiles = INT_MAX / kMaxExperts - 1;    // tiles of a group: their sum over all groups fits an int
@@ -57,7 +66,7 @@ struct MmGeom {
     int tmem_cols;
     uint32_t format;    // operand format field of the instruction descriptor
     int esize;
-    int stage_off, recv_off, table_off, bar_off;   // byte offsets in shared memory
+    int recv_off, turn_off, table_off, bar_off;   // byte offsets in shared memory
 };
 
 struct Tile {
@@ -77,9 +86,9 @@ __device__ __forceinline__ int even_cols(int count, int tn) {
 }
 
 // first[g] = tiles before group g, for all groups; all threads call it
-__device__ void build_table(const GroupedParams &p, const MmGeom &t, int *first, int threads) {
-    __shared__ int warp_total[kLoadThreads / 32];
-    constexpr int kPer = kMaxExperts / kTmaThreads;
+__device__ void build_table(const GroupedParams &p, const MmGeom &t, int *first) {
+    __shared__ int warp_total[kMaxThreads / 32];
+    constexpr int kPer = (kMaxExperts + threads_of(kTma) - 1) / threads_of(kTma);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int mine[kPer], sum = 0;
 #pragma unroll
@@ -149,12 +158,9 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void *tmap, uint
         ::"r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
         : "memory");
 }
-// four rows of the matrix, any four, behind one another
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const void *tmap, uint32_t bar, int c0, int4 rows) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-        ::"r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w)
-        : "memory");
+// 16 bytes into shared memory of which `bytes` come from memory, the rest are zeros
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -217,28 +223,79 @@ __device__ __noinline__ float act_far(float v, int act) {
     if (act == 2) return 1.0f / (1.0f + __expf(-v));
     return tanhf(v);
 }
-__device__ __forceinline__ float apply_act(float v, int act) {
-    if (act == 0) return v;
-    if (act == 1) return fmaxf(v, 0.0f);
-    if (act == 4) return __fdividef(v, 1.0f + __expf(-v));
-    return act_far(v, act);
+// the activation of N values; one branch for all of them
+template <int N>
+__device__ __forceinline__ void activate(float *v, int act) {
+    if (act == 0) return;
+    if (act == 1) {
+#pragma unroll
+        for (int c = 0; c < N; ++c) v[c] = fmaxf(v[c], 0.0f);
+    } else if (act == 4) {
+#pragma unroll
+        for (int c = 0; c < N; ++c) v[c] = __fdividef(v[c], 1.0f + __expf(-v[c]));
+    } else {
+#pragma unroll
+        for (int c = 0; c < N; ++c) v[c] = act_far(v[c], act);
+    }
 }
 
-__device__ __forceinline__ void store_out(void *y, Elem type, long long at, float v) {
-    if (type == Elem::BF16) static_cast<__nv_bfloat16 *>(y)[at] = __float2bfloat16_rn(v);
-    else if (type == Elem::F16) static_cast<__half *>(y)[at] = __float2half_rn(v);
-    else static_cast<float *>(y)[at] = v;
+template <class T> __device__ __forceinline__ T narrow(float v);
+template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// What an epilogue warp needs to write the results of its lanes' channels.
+struct Out {
+    uint8_t *turn;              // shared memory of this warp, kTurnBytes
+    uint8_t *first;             // &y[tile.row0][first channel of this warp]
+    long long row_bytes;
+    int rows, channels;         // valid rows of the tile, valid channels of this warp
+    int vectors;                // rows may be written 16 bytes at a time
+};
+
+// v[c] (gated: v[c / 2], the lanes' halves holding alternate columns) are the results of columns c0 .. c0 + 31 of this
+// lane's channel.  The warp turns them round in shared memory and writes whole segments of rows, 64 bytes or more.
+template <class T, bool GATED>
+__device__ __forceinline__ void write_columns(const Out &o, const float *v, int c0, int lane) {
+    constexpr int kWidth = GATED ? 16 : 32;                           // channels of the warp
+    constexpr int kCols = kTurnBytes / (32 * int(sizeof(T)));         // columns per turn
+    constexpr int kPieces = kWidth * int(sizeof(T)) / 16;             // 16-byte pieces of a row
+    T *turn = reinterpret_cast<T *>(o.turn);
+#pragma unroll
+    for (int h = 0; h < kStageCols; h += kCols) {
+        if (GATED) {
+#pragma unroll
+            for (int c = 0; c < kCols / 2; ++c) turn[(2 * c + (lane >> 4)) * 16 + (lane & 15)] = narrow<T>(v[h / 2 + c]);
+        } else {
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) turn[c * 32 + lane] = narrow<T>(v[h + c]);
+        }
+        __syncwarp();
+        const int count = o.rows - c0 - h;
+        if (o.vectors) {
+            const int row = lane / kPieces;
+            uint8_t *to = o.first + (c0 + h + row) * o.row_bytes + (lane % kPieces) * 16;
+#pragma unroll
+            for (int q = 0; q < kCols * kPieces / 32; ++q) {
+                if (row + q * (32 / kPieces) < count) *reinterpret_cast<uint4 *>(to) = reinterpret_cast<const uint4 *>(turn)[q * 32 + lane];
+                to += (32 / kPieces) * o.row_bytes;
+            }
+        } else {
+            for (int i = lane; i < min(kCols, count) * kWidth; i += 32)
+                if (i % kWidth < o.channels) reinterpret_cast<T *>(o.first + (c0 + h + i / kWidth) * o.row_bytes)[i % kWidth] = turn[i];
+        }
+        __syncwarp();
+    }
 }
 
-template <int KIND, bool TMA>
-__global__ void __launch_bounds__(TMA ? kTmaThreads : kLoadThreads, 1)
+template <int KIND, int LOADS>
+__global__ void __launch_bounds__(threads_of(LOADS), 1)
 expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const GroupedParams p,
                  const MmGeom t) {
-    constexpr int kThreadCount = TMA ? kTmaThreads : kLoadThreads;
     constexpr int kPlanes = KIND == kX3 ? 2 : 1;
+    constexpr int kEpilogueWarps = epilogue_warps(LOADS), kLoadWarp0 = 4 + kEpilogueWarps;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ float row_scale_s[2][256];
-    __shared__ uint32_t live_s[2][8];
+    __shared__ __align__(16) float row_scale_s[2][256];
     __shared__ uint32_t tmem_slot;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *generic = smem_raw + (base - smem_u32(smem_raw));
@@ -252,7 +309,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < t.stages; ++s) {
-            mbar_init(full0 + 8u * s, TMA ? 2 : kLoaderWarps);
+            mbar_init(full0 + 8u * s, LOADS == kTma ? 2 : LOADS == kGather ? 1 + kGatherWarps : kLoaderWarps);
             mbar_init(empty0 + 8u * s, 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -269,7 +326,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         tmem_relinquish();
     }
     grid_dependency_entry();
-    build_table(p, t, first, kThreadCount);
+    build_table(p, t, first);
     tc_fence_before();
     __syncthreads();
     if (t.cluster > 1) cluster_sync_all();
@@ -281,7 +338,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     const int k_begin = t.k_steps * rank / t.cluster, k_end = t.k_steps * (rank + 1) / t.cluster;
     const int k_elems = kRowBytes / t.esize;
 
-    if (TMA && warp == 0) {
+    if (LOADS != kRegs && warp == 0) {
         // ---------------- weights ----------------
         if (lane == 0) {
             int s = 0;
@@ -293,7 +350,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 for (int k = k_begin; k < k_end; ++k) {
                     ok = mbar_wait(empty0 + 8u * s, phase, nullptr);
                     if (!ok) break;
-                    const uint32_t dst = base + t.stage_off + uint32_t(s) * stage_bytes, bar = full0 + 8u * s;
+                    const uint32_t dst = base + uint32_t(s) * stage_bytes, bar = full0 + 8u * s;
                     mbar_expect_tx(bar, kATileBytes);
                     if (!p.gated) {
                         tma_load_3d(dst, &map_w, bar, k * k_elems, tile.channel0, tile.group);
@@ -312,56 +369,92 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                     mbar_wait(full0 + 8u * (j % t.stages), uint32_t((j / t.stages) & 1), nullptr);
             }
         }
-    } else if (TMA && warp == 3) {
+    } else if (LOADS == kTma && warp == 3) {
         // ---------------- rows ----------------
-        int s = 0;
+        if (lane == 0) {
+            int s = 0;
+            uint32_t phase = 1;
+            int armed = 0;
+            bool ok = true;
+            for (int i = tile0; i < total_tiles && ok; i += tile_step) {
+                const Tile tile = find_tile(p, t, first, i);
+                const int loads = (tile.valid + t.box_rows - 1) / t.box_rows;
+                const uint32_t bytes = uint32_t(loads * t.box_rows) * kRowBytes;
+                for (int k = k_begin; k < k_end; ++k) {
+                    ok = mbar_wait(empty0 + 8u * s, phase, nullptr);
+                    if (!ok) break;
+                    const uint32_t dst = base + uint32_t(s) * stage_bytes + kATileBytes, bar = full0 + 8u * s;
+                    mbar_expect_tx(bar, bytes);
+                    for (int b = 0; b < loads; ++b)
+                        tma_load_2d(dst + uint32_t(b * t.box_rows) * kRowBytes, &map_x, bar, k * k_elems, tile.row0 + b * t.box_rows);
+                    ++armed;
+                    if (++s == t.stages) { s = 0; phase ^= 1u; }
+                }
+            }
+            if (!ok) {
+                time_out(2);
+                for (int j = armed - 1, n = 0; j >= 0 && n < t.stages; --j, ++n)
+                    mbar_wait(full0 + 8u * (j % t.stages), uint32_t((j / t.stages) & 1), nullptr);
+            }
+        }
+    } else if (LOADS == kGather && warp >= kLoadWarp0) {
+        // ---------------- gathered rows ----------------
+        // thread i of 128 moves 16-byte column i % 8 of columns i / 8, i / 8 + 16, ... of the tile.  A step is handed over
+        // once it has landed, `lag` steps after it was asked for (narrow tiles have many stages, and need them: a step is
+        // then a few KiB).
+        constexpr int kMost = 16;
+        const int lag = t.stages >= 8 ? 6 : 2;
+        const int tid = int(threadIdx.x) - 32 * kLoadWarp0, c16 = tid & 7, r0 = tid >> 3;
+        const long long row_bytes = (long long)p.inner * t.esize;
+        int s = 0, landed = 0, waiting = 0;
         uint32_t phase = 1;
-        int armed = 0;
         bool ok = true;
+        auto hand_over = [&]() {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full0 + 8u * landed);
+            if (++landed == t.stages) landed = 0;
+            --waiting;
+        };
         for (int i = tile0; i < total_tiles && ok; i += tile_step) {
             const Tile tile = find_tile(p, t, first, i);
-            const int loads = p.rows ? (tile.valid + 3) / 4 : (tile.valid + t.box_rows - 1) / t.box_rows;
-            const uint32_t bytes = uint32_t(loads) * (p.rows ? 4 : t.box_rows) * kRowBytes;
-            int4 src[2];
-            if (p.rows) {
+            int src[kMost];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    int at[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int c = min((j * 32 + lane) * 4 + q, tile.valid - 1);
-                        const int r = p.rows[tile.row0 + c];
-                        at[q] = r >= 0 && r < p.x_rows ? r : 0;      // a missing row is zeroed by the epilogue
-                    }
-                    src[j] = make_int4(at[0], at[1], at[2], at[3]);
-                }
+            for (int j = 0; j < kMost; ++j) {
+                const int c = r0 + 16 * j;
+                const int r = c < tile.valid ? p.rows[tile.row0 + c] : -1;
+                src[j] = r >= 0 && r < p.x_rows ? r : -1;
             }
             for (int k = k_begin; k < k_end; ++k) {
                 ok = mbar_wait(empty0 + 8u * s, phase, nullptr);
                 ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
                 if (!ok) break;
-                const uint32_t dst = base + t.stage_off + uint32_t(s) * stage_bytes + kATileBytes, bar = full0 + 8u * s;
-                if (lane == 0) mbar_expect_tx(bar, bytes);
-                __syncwarp();
-                if (p.rows) {
-                    if (lane < loads) tma_gather4(dst + uint32_t(lane) * 4u * kRowBytes, &map_x, bar, k * k_elems, src[0]);
-                    if (lane + 32 < loads) tma_gather4(dst + uint32_t(lane + 32) * 4u * kRowBytes, &map_x, bar, k * k_elems, src[1]);
-                } else if (lane < loads) {
-                    tma_load_2d(dst + uint32_t(lane) * uint32_t(t.box_rows) * kRowBytes, &map_x, bar, k * k_elems, tile.row0 + lane * t.box_rows);
-                }
-                ++armed;
+                const uint32_t dst = base + uint32_t(s) * stage_bytes + kATileBytes;
+                const long long byte0 = (long long)k * kRowBytes + c16 * 16;
+                const int left = int(min(max(row_bytes - byte0, 0LL), 16LL));
+#pragma unroll
+                for (int j = 0; j < kMost; ++j)
+                    if (16 * j < tile.cols) {
+                        const bool live = src[j] >= 0 && left > 0;
+                        const uint8_t *from = static_cast<const uint8_t *>(p.x) + (live ? (long long)src[j] * p.x_stride * t.esize + byte0 : 0);
+                        cp_async16(dst + sw128_offset(r0 + 16 * j, c16), from, live ? left : 0);
+                    }
+                asm volatile("cp.async.commit_group;" ::: "memory");
                 if (++s == t.stages) { s = 0; phase ^= 1u; }
+                if (++waiting > lag) {
+                    if (lag == 6) asm volatile("cp.async.wait_group 6;" ::: "memory");
+                    else asm volatile("cp.async.wait_group 2;" ::: "memory");
+                    hand_over();
+                }
             }
         }
-        if (!ok) {
-            if (lane == 0) time_out(2);
-            for (int j = armed - 1, n = 0; j >= 0 && n < t.stages; --j, ++n)
-                mbar_wait(full0 + 8u * (j % t.stages), uint32_t((j / t.stages) & 1), nullptr);
-        }
-    } else if (!TMA && warp >= 8) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        while (waiting > 0) hand_over();
+        if (!ok && lane == 0) time_out(2);
+    } else if (LOADS == kRegs && warp >= kLoadWarp0) {
         // ---------------- loader warps ----------------
         // thread i of 256 moves 16-byte column i % 8 of rows i / 8, i / 8 + 32, ...: four of the weights, up to four of x
-        const int tid = int(threadIdx.x) - 256, c16 = tid & 7, r0 = tid >> 3;
+        const int tid = int(threadIdx.x) - 32 * kLoadWarp0, c16 = tid & 7, r0 = tid >> 3;
         const long long row_bytes = (long long)p.inner * t.esize;
         int s = 0;
         uint32_t phase = 1;
@@ -394,7 +487,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 ok = mbar_wait(empty0 + 8u * s, phase, nullptr);
                 ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
                 if (!ok) break;
-                uint8_t *stage = generic + t.stage_off + size_t(s) * stage_bytes;
+                uint8_t *stage = generic + size_t(s) * stage_bytes;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int r = r0 + 32 * (j & 3);
@@ -447,7 +540,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                     if (ok) ok = mbar_wait(full0 + 8u * s, phase, nullptr);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t stage = base + t.stage_off + uint32_t(s) * stage_bytes;
+                    const uint32_t stage = base + uint32_t(s) * stage_bytes;
                     const uint64_t da = smem_desc_kmajor(stage, 128), db = smem_desc_kmajor(stage + kPlanes * kATileBytes, 128);
                     const uint64_t da_lo = smem_desc_kmajor(stage + kATileBytes, 128);
                     const uint64_t db_lo = smem_desc_kmajor(stage + kPlanes * kATileBytes + b_bytes, 128);
@@ -473,58 +566,84 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             }
             if (!ok) time_out(4);
         }
-    } else if (warp >= 4 && warp < 8) {
+    } else if (warp >= 4 && warp < kLoadWarp0) {
         // ---------------- epilogue ----------------
-        const int quad = warp & 3, tid = int(threadIdx.x) - 128, lane_row = quad * 32 + lane;
+        // warps 4 + q and 8 + q read lanes 32 q .. 32 q + 31 of tensor memory and alternate in the columns
+        constexpr int kShare = kEpilogueWarps / 4;
+        const int quad = warp & 3, share = (warp >> 2) - 1, tid = int(threadIdx.x) - 128, lane_row = quad * 32 + lane;
         const uint32_t lane_tmem = tmem + (uint32_t(quad * 32) << 16);
         const uint32_t recv = base + t.recv_off;
         float *recv_generic = reinterpret_cast<float *>(generic + t.recv_off);
-        const bool per_row = p.row_scale || p.rows;
+        const int out_size = elem_size(p.out_type);
+        Out o;
+        o.turn = generic + t.turn_off + (warp - 4) * kTurnBytes;
+        o.row_bytes = p.y_stride * out_size;
         int turn = 0, round = 0;
         bool ok = true;
         for (int i = tile0; i < total_tiles && ok; i += tile_step, ++round) {
             const Tile tile = find_tile(p, t, first, i);
             const int half = p.gated ? (lane >> 4) : 0;
-            const int channel = p.gated ? tile.channel0 + quad * 16 + (lane & 15) : tile.channel0 + lane_row;
+            const int warp_channel = tile.channel0 + quad * (p.gated ? 16 : 32);
+            const int channel = warp_channel + (p.gated ? (lane & 15) : lane);
             const bool in_channels = channel < p.channels;
             const long long per_channel = (long long)tile.group * (p.gated ? 2 : 1) * p.channels + (long long)half * p.channels + channel;
             const float channel_scale = p.channel_scale && in_channels ? p.channel_scale[per_channel] : 1.0f;
             const float bias = p.bias && in_channels ? p.bias[per_channel] : 0.0f;
-            const int slot = round & 1;
-            if (per_row) {
-                for (int c = tid; c < max(t.tn, 32); c += 128) {           // whole warps
+            o.first = static_cast<uint8_t *>(p.y) + (tile.row0 * p.y_stride + warp_channel) * out_size;
+            o.rows = tile.valid;
+            o.channels = max(0, min(p.gated ? 16 : 32, p.channels - warp_channel));
+            o.vectors = ((reinterpret_cast<uintptr_t>(o.first) | uintptr_t(o.row_bytes)) & 15) == 0 && o.channels == (p.gated ? 16 : 32);
+            const float *row_scale = row_scale_s[round & 1];
+            if (p.row_scale) {
+                for (int c = tid; c < t.tn; c += 32 * kEpilogueWarps) {
                     const int src = c < tile.valid ? (p.rows ? p.rows[tile.row0 + c] : tile.row0 + c) : -1;
-                    const bool live = src >= 0 && src < p.x_rows;
-                    row_scale_s[slot][c] = live && p.row_scale ? p.row_scale[src] : 1.0f;
-                    const uint32_t mask = __ballot_sync(0xffffffffu, live);
-                    if (lane == 0) live_s[slot][c >> 5] = mask;
+                    row_scale_s[round & 1][c] = src >= 0 && src < p.x_rows ? p.row_scale[src] : 1.0f;
                 }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory");
             }
-            // a finished sum of column c: scales, bias, activation, store
-            auto value = [&](float raw, int c) {
-                float v = KIND == kI8 ? float(__float_as_int(raw)) : raw;
-                if (per_row) {
-                    if (!((live_s[slot][c >> 5] >> (c & 31)) & 1u)) v = 0.0f;
-                    v *= row_scale_s[slot][c];
+            // finished sums of columns c0 .. c0 + 31 (those behind the tile's last are not used): scales, bias, activation, store
+            auto finish = [&](float *v, int c0) {
+                if (c0 >= tile.valid || o.channels == 0) return;
+                if (KIND == kI8) {
+#pragma unroll
+                    for (int c = 0; c < kStageCols; ++c) v[c] = float(__float_as_int(v[c]));
                 }
-                return v * channel_scale + bias;
-            };
-            auto put = [&](int c, float v) {
-                if (in_channels && c < tile.valid) store_out(p.y, p.out_type, (long long)(tile.row0 + c) * p.y_stride + channel, v);
-            };
-            // two neighbouring columns c, c + 1
-            auto finish = [&](float raw0, float raw1, int c) {
-                if (c >= tile.valid) return;
-                const float v0 = value(raw0, c), v1 = value(raw1, c + 1);
+                if (p.row_scale) {
+                    if (t.cluster == 1) {                     // c0 is a multiple of 32, t.tn of 16
+#pragma unroll
+                        for (int c = 0; c < kStageCols; c += 4)
+                            if (c0 + c < t.tn) {
+                                const float4 f = *reinterpret_cast<const float4 *>(row_scale + c0 + c);
+                                v[c] *= f.x; v[c + 1] *= f.y; v[c + 2] *= f.z; v[c + 3] *= f.w;
+                            }
+                    } else {                                  // a rank's columns may start at any even one
+#pragma unroll
+                        for (int c = 0; c < kStageCols; ++c)
+                            if (c0 + c < t.tn) v[c] *= row_scale[c0 + c];
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < kStageCols; ++c) v[c] = v[c] * channel_scale + bias;
                 if (!p.gated) {
-                    put(c, apply_act(v0, p.act));
-                    put(c + 1, apply_act(v1, p.act));
+                    activate<kStageCols>(v, p.act);
+                    if (p.out_type == Elem::BF16) write_columns<__nv_bfloat16, false>(o, v, c0, lane);
+                    else if (p.out_type == Elem::F16) write_columns<__half, false>(o, v, c0, lane);
+                    else write_columns<float, false>(o, v, c0, lane);
                 } else {
-                    // the lower half of the warp finishes column c, the upper half column c + 1
-                    const float other = __shfl_xor_sync(0xffffffffu, half ? v0 : v1, 16);
-                    const float gate = half ? other : v0, up = half ? v1 : other;
-                    put(c + half, apply_act(gate, p.act) * up);
+                    // the lower half of the warp finishes the even columns, the upper half the odd ones
+                    float up[kStageCols / 2];
+#pragma unroll
+                    for (int c = 0; c < kStageCols / 2; ++c) {
+                        const float other = __shfl_xor_sync(0xffffffffu, half ? v[2 * c] : v[2 * c + 1], 16);
+                        up[c] = half ? v[2 * c + 1] : other;
+                        v[c] = half ? other : v[2 * c];
+                    }
+                    activate<kStageCols / 2>(v, p.act);
+#pragma unroll
+                    for (int c = 0; c < kStageCols / 2; ++c) v[c] *= up[c];
+                    if (p.out_type == Elem::BF16) write_columns<__nv_bfloat16, true>(o, v, c0, lane);
+                    else if (p.out_type == Elem::F16) write_columns<__half, true>(o, v, c0, lane);
+                    else write_columns<float, true>(o, v, c0, lane);
                 }
             };
             if (KIND == kX3) {
@@ -552,8 +671,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 if (!ok) break;
                 if (t.cluster == 1) {
 #pragma unroll
-                    for (int c = 0; c < kLoaderCols; c += 2)
-                        if (c < tile.cols) finish(sum[c], sum[c + 1], c);
+                    for (int c = 0; c < kLoaderCols; c += kStageCols) finish(sum + c, c);
                 } else {
                     ok = round == 0 || mbar_wait_cluster(recv_free, uint32_t(round - 1) & 1u, nullptr);
                     ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
@@ -571,14 +689,18 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
                 if (!ok) break;
                 tc_fence_after();
-                const int per = tile.cols / t.cluster;
-                for (int c0 = 0; c0 < tile.cols; c0 += 16) {
-                    float v[16];
-                    tmem_ld16(lane_tmem + a * uint32_t(t.tn) + c0, v);
-                    if (t.cluster == 1) {
-#pragma unroll
-                        for (int c = 0; c < 16; c += 2) finish(v[c], v[c + 1], c0 + c);
-                    } else {
+                if (t.cluster == 1) {
+                    for (int c0 = share * kStageCols; c0 < tile.valid; c0 += kShare * kStageCols) {
+                        float v[kStageCols];
+                        if (c0 + kStageCols <= t.tn) tmem_ld32(lane_tmem + a * uint32_t(t.tn) + c0, v);
+                        else tmem_ld16(lane_tmem + a * uint32_t(t.tn) + c0, v);
+                        finish(v, c0);
+                    }
+                } else {
+                    const int per = tile.cols / t.cluster;
+                    for (int c0 = share * 16; c0 < tile.cols; c0 += kShare * 16) {
+                        float v[16];
+                        tmem_ld16(lane_tmem + a * uint32_t(t.tn) + c0, v);
 #pragma unroll
                         for (int c = 0; c < 16; ++c) {
                             const int d = (c0 + c) / per;
@@ -599,20 +721,25 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 ok = mbar_wait_cluster(recv_full, uint32_t(round) & 1u, nullptr);
                 ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
                 if (!ok) break;
-                for (int c = 0; c < per; c += 2) {
-                    float v[2];
+                // (pairs of columns: a gated result takes two lanes' columns at once)
+                const int mine = kShare == 1 ? per : (per / 2 + 1) / 2 * 2;          // columns of the first warp of a quarter
+                const int from = share * mine, to = share == 0 ? mine : per;
+                o.rows = min(tile.valid, rank * per + to);
+                for (int c0 = from; c0 < to; c0 += kStageCols) {
+                    float v[kStageCols];
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
+                    for (int c = 0; c < kStageCols; ++c) {
                         float f = 0.0f;
                         int n = 0;
-                        for (int q = 0; q < t.cluster; ++q) {
-                            const float part = recv_generic[(q * per + c + j) * kTileM + lane_row];
-                            if (KIND == kI8) n += __float_as_int(part);
-                            else f += part;
-                        }
-                        v[j] = KIND == kI8 ? __int_as_float(n) : f;
+                        if (c0 + c < to)
+                            for (int q = 0; q < t.cluster; ++q) {
+                                const float part = recv_generic[(q * per + c0 + c) * kTileM + lane_row];
+                                if (KIND == kI8) n += __float_as_int(part);
+                                else f += part;
+                            }
+                        v[c] = KIND == kI8 ? __int_as_float(n) : f;
                     }
-                    finish(v[0], v[1], rank * per + c);
+                    finish(v, rank * per + c0);
                 }
                 __syncwarp();
                 if (lane < t.cluster) mbar_arrive_cluster(cluster_map(recv_free, uint32_t(lane)));
@@ -703,25 +830,26 @@ int choose(const GroupedParams &p, int sm_count, bool tma, MmGeom *t) {
     const size_t stage = size_t(planes) * (kATileBytes + t->tn * kRowBytes);
     const size_t recv = t->cluster > 1 ? size_t(t->tn) * kTileM * sizeof(float) : 0;
     const size_t table = (size_t(p.groups + 1) * sizeof(int) + 15) / 16 * 16;
-    const size_t fixed = 1024 + recv + table + 2 * kMaxStages * 8 + 64 + 4096;       // 4096: the kernel's static shared memory
+    const size_t turn = 8 * kTurnBytes;
+    const size_t fixed = 1024 + recv + turn + table + 2 * kMaxStages * 8 + 64 + 4096;       // 4096: the kernel's static shared memory
     t->stages = int(std::min<size_t>(kMaxStages, (kSmemLimit - fixed) / stage));
-    t->stage_off = 0;
     t->recv_off = int(t->stages * stage);
-    t->table_off = int(t->recv_off + recv);
+    t->turn_off = int(t->recv_off + recv);
+    t->table_off = int(t->turn_off + turn);
     t->bar_off = int(t->table_off + table);
     const long long most = (long long)t->n_tiles * (p.total / t->tn + busy);         // no distribution needs more
     return int(std::min<long long>(sm_count / t->cluster, most)) * t->cluster;
 }
 
-template <int KIND, bool TMA>
+template <int KIND, int LOADS>
 cudaError_t run(const GroupedParams &p, const MmGeom &t, int ctas, const CUtensorMap &map_w, const CUtensorMap &map_x, cudaStream_t stream) {
     const int smem = t.bar_off + 2 * kMaxStages * 8 + 64 + 1024;
-    const auto kernel = expert_mm_kernel<KIND, TMA>;
+    const auto kernel = expert_mm_kernel<KIND, LOADS>;
     cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (err != cudaSuccess) return err;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(unsigned(ctas));
-    config.blockDim = dim3(TMA ? kTmaThreads : kLoadThreads);
+    config.blockDim = dim3(threads_of(LOADS));
     config.dynamicSmemBytes = size_t(smem);
     config.stream = stream;
     cudaLaunchAttribute attribute = {};
@@ -757,15 +885,18 @@ cudaError_t launch_grouped(const GroupedParams &given, cudaStream_t stream) {
     if (tma) {
         const long long stack_bytes = p.groups == 1 ? 16 : p.w_group_stride * t.esize;
         if (!encode(&map_w, p.type, p.w, p.inner, wide, p.w_stride * t.esize, p.groups, stack_bytes, p.gated ? 16 : kTileM, 3) ||
-            !encode(&map_x, p.type, p.x, p.inner, p.x_rows, p.x_stride * t.esize, 1, 0, p.rows ? 1 : t.box_rows, 2)) {
+            (!p.rows && !encode(&map_x, p.type, p.x, p.inner, p.x_rows, p.x_stride * t.esize, 1, 0, t.box_rows, 2))) {
             tma = false;                             // a shape that no tensor map describes
             ctas = choose(p, sm_count, tma, &t);
         }
     }
-    if (p.type == Elem::F32) return run<kX3, false>(p, t, ctas, map_w, map_x, stream);
-    if (p.type == Elem::S8)
-        return tma ? run<kI8, true>(p, t, ctas, map_w, map_x, stream) : run<kI8, false>(p, t, ctas, map_w, map_x, stream);
-    return tma ? run<kF16, true>(p, t, ctas, map_w, map_x, stream) : run<kF16, false>(p, t, ctas, map_w, map_x, stream);
+    if (p.type == Elem::F32) return run<kX3, kRegs>(p, t, ctas, map_w, map_x, stream);
+    if (p.type == Elem::S8) {
+        if (!tma) return run<kI8, kRegs>(p, t, ctas, map_w, map_x, stream);
+        return p.rows ? run<kI8, kGather>(p, t, ctas, map_w, map_x, stream) : run<kI8, kTma>(p, t, ctas, map_w, map_x, stream);
+    }
+    if (!tma) return run<kF16, kRegs>(p, t, ctas, map_w, map_x, stream);
+    return p.rows ? run<kF16, kGather>(p, t, ctas, map_w, map_x, stream) : run<kF16, kTma>(p, t, ctas, map_w, map_x, stream);
 }
 
 cudaError_t expert_mm_status(cudaStream_t stream, int *code) {
