@@ -51,6 +51,7 @@ constexpr int kTurnBytes = kStageCols * 32 * 2; // ... in this much shared memor
 constexpr int kChunkSteps = 4;                  // float32: K steps per partial sum
 constexpr int kMaxStages = 12;
 constexpr int kMaxGroupTiles = INT_MAX / kMaxExperts - 1;    // tiles of a group: their sum over all groups fits an int
+constexpr int kBarBytes = 3 * kMaxStages * 8 + 48;    // mbarriers: three per stage, six more
 constexpr size_t kSmemLimit = 227 * 1024;
 
 __device__ int g_expert_error;                  // set by a wait that ran out, read by expert_mm_status
@@ -58,7 +59,8 @@ __device__ int g_expert_error;                  // set by a wait that ran out, r
 struct MmGeom {
     int tn;             // columns a tile may have
     int n_tiles;        // channel tiles of a group
-    int tile_channels;  // output channels per channel tile: 128, gated 64
+    int tile_channels;  // output channels per channel tile: 128 per CTA, gated 64
+    int grain;          // columns of a tile come in multiples of this: 16, pairs 32
     int k_steps;
     int cluster;        // CTAs that share a tile's K range
     int stages;
@@ -79,10 +81,10 @@ __device__ __forceinline__ void group_rows(const GroupedParams &p, int g, int *b
     *begin = min(max(p.offsets[g], 0), p.total);
     *count = min(max(p.offsets[g + 1], *begin), p.total) - *begin;
 }
-// Columns per tile of a group: its rows dealt evenly to the fewest tiles, in multiples of 16.
-__device__ __forceinline__ int even_cols(int count, int tn) {
-    const int tiles = (count + tn - 1) / tn;
-    return ((count + tiles - 1) / tiles + 15) & ~15;
+// Columns per tile of a group: its rows dealt evenly to the fewest tiles.
+__device__ __forceinline__ int even_cols(int count, const MmGeom &t) {
+    const int tiles = (count + t.tn - 1) / t.tn;
+    return ((count + tiles - 1) / tiles + t.grain - 1) & -t.grain;
 }
 
 // first[g] = tiles before group g, for all groups; all threads call it
@@ -96,7 +98,7 @@ __device__ void build_table(const GroupedParams &p, const MmGeom &t, int *first)
         const int g = int(threadIdx.x) * kPer + i;
         int count = 0, begin;
         if (g < p.groups) group_rows(p, g, &begin, &count);
-        const int c = count > 0 ? even_cols(count, t.tn) : 1;
+        const int c = count > 0 ? even_cols(count, t) : 1;
         mine[i] = int(min((long long)((count + c - 1) / c) * t.n_tiles, (long long)kMaxGroupTiles));
         sum += mine[i];
     }
@@ -121,7 +123,7 @@ __device__ void build_table(const GroupedParams &p, const MmGeom &t, int *first)
 
 // Tiles of a group: up to 8 column tiles side by side, then the next channels, so that neighbours in the list share
 // weights and rows in L2.
-__device__ __forceinline__ Tile find_tile(const GroupedParams &p, const MmGeom &t, const int *first, int index) {
+__device__ __forceinline__ Tile find_tile(const GroupedParams &p, const MmGeom &t, const int *first, int index, int cta_channel) {
     int lo = 0, hi = p.groups;                    // first[lo] <= index < first[hi]
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -130,7 +132,7 @@ __device__ __forceinline__ Tile find_tile(const GroupedParams &p, const MmGeom &
     }
     int begin, count;
     group_rows(p, lo, &begin, &count);
-    const int cols = even_cols(count, t.tn);
+    const int cols = even_cols(count, t);
     const int col_tiles = (count + cols - 1) / cols;
     const int at = index - first[lo];
     const int band = at / (8 * t.n_tiles);
@@ -141,8 +143,8 @@ __device__ __forceinline__ Tile find_tile(const GroupedParams &p, const MmGeom &
     const int col0 = (band * 8 + inside % wide) * cols;
     tile.row0 = begin + col0;
     tile.valid = min(cols, count - col0);
-    tile.cols = (tile.valid + 15) & ~15;
-    tile.channel0 = inside / wide * t.tile_channels;
+    tile.cols = (tile.valid + t.grain - 1) & -t.grain;
+    tile.channel0 = inside / wide * t.tile_channels + cta_channel;
     return tile;
 }
 
@@ -158,17 +160,72 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void *tmap, uint
         ::"r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
         : "memory");
 }
+// The same loads by one CTA of a pair: the bytes are counted on `bar`, which may be in either CTA's shared memory.
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void *tmap, uint32_t bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void *tmap, uint32_t bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+}
 // 16 bytes into shared memory of which `bytes` come from memory, the rest are zeros
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+// Low word of a K-major operand's descriptor (128-byte swizzle); the high word is the same for all.
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr) { return ((addr & 0x3FFFF) >> 4) | (1u << 16); }
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+// D += A B for one K block of 32 bytes, by one CTA or by a pair (whose halves of A, B and D lie at the same addresses).
+// The whole warp calls it with equal arguments, which then live in uniform registers, and one lane issues.
+#define IOS_UMMA(GROUP, KIND_NAME)                                                                             \
+    asm volatile(                                                                                              \
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"                                                         \
+        "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"                                                     \
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"                                                   \
+        "@q tcgen05.mma.cta_group::" GROUP ".kind::" KIND_NAME " [%0], a, b, %3, p;\n\t}"                       \
+        ::"r"(tmem_d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(kDescHigh), "r"(elected)       \
+        : "memory")
+template <int KIND, bool PAIR>
+__device__ __forceinline__ void umma(uint32_t elected, uint32_t tmem_d, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
+    if (KIND == kF16) {
+        if (PAIR) IOS_UMMA("2", "f16");
+        else IOS_UMMA("1", "f16");
+    } else if (KIND == kI8) {
+        if (PAIR) IOS_UMMA("2", "i8");
+        else IOS_UMMA("1", "i8");
+    } else {
+        IOS_UMMA("1", "tf32");
+    }
+}
+#undef IOS_UMMA
+// arrives at `bar` (of both CTAs of a pair) once the instructions issued so far have finished
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint32_t bar) {
+    if (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(bar), "h"(uint16_t(3))
+                     : "memory");
+    else
+        umma_commit(bar);
+}
+// mbar_wait for a barrier that other CTAs of the cluster may arrive at
+template <bool CLUSTER>
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
+    if (!CLUSTER) return mbar_wait(bar, parity, nullptr);
+    uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
         : "memory");
+    return done != 0 || mbar_wait_cluster(bar, parity, nullptr);
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -179,7 +236,13 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
 __device__ __forceinline__ void store_cluster(uint32_t dst, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(v) : "memory");
 }
-__device__ __forceinline__ void time_out(int code) { atomicExch(&g_expert_error, code); }
+// Records a wait that ran out.  The loads that this CTA has under way land within microseconds; those counted in another
+// CTA's barriers cannot be waited for from here, so a millisecond is let pass.
+__device__ __noinline__ void time_out(int code) {
+    atomicExch(&g_expert_error, code);
+    const uint64_t t0 = global_ns();
+    while (global_ns() - t0 < 1000000) __nanosleep(1000);
+}
 
 // ---- loader warps: 16 bytes of a row, zeros behind its end, for any alignment ----------------------
 __device__ __noinline__ uint4 load_chunk_edge(const uint8_t *row, long long byte0, long long row_bytes, int esize) {
@@ -288,7 +351,7 @@ __device__ __forceinline__ void write_columns(const Out &o, const float *v, int 
     }
 }
 
-template <int KIND, int LOADS>
+template <int KIND, int LOADS, bool PAIR>
 __global__ void __launch_bounds__(threads_of(LOADS), 1)
 expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const GroupedParams p,
                  const MmGeom t) {
@@ -300,21 +363,22 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *generic = smem_raw + (base - smem_u32(smem_raw));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t b_bytes = uint32_t(t.tn) * kRowBytes;
+    const uint32_t b_bytes = uint32_t(PAIR ? t.tn / 2 : t.tn) * kRowBytes;
     const uint32_t stage_bytes = kPlanes * (kATileBytes + b_bytes);
     const uint32_t full0 = base + t.bar_off, empty0 = full0 + 8u * t.stages;
     const uint32_t acc_full0 = empty0 + 8u * t.stages, acc_empty0 = acc_full0 + 16u;
-    const uint32_t recv_full = acc_empty0 + 16u, recv_free = recv_full + 8u;
+    const uint32_t recv_full = acc_empty0 + 16u, recv_free = recv_full + 8u, landed0 = recv_free + 8u;
     int *first = reinterpret_cast<int *>(generic + t.table_off);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < t.stages; ++s) {
-            mbar_init(full0 + 8u * s, LOADS == kTma ? 2 : LOADS == kGather ? 1 + kGatherWarps : kLoaderWarps);
+            mbar_init(full0 + 8u * s, LOADS == kTma ? 2 : LOADS == kGather ? (PAIR ? 3 : 2) : kLoaderWarps);
+            mbar_init(landed0 + 8u * s, 32 * kGatherWarps);
             mbar_init(empty0 + 8u * s, 1);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(acc_full0 + 8u * a, 1);
-            mbar_init(acc_empty0 + 8u * a, kEpilogueWarps);
+            mbar_init(acc_empty0 + 8u * a, (PAIR ? 2 : 1) * kEpilogueWarps);
         }
         mbar_init(recv_full, uint32_t(kEpilogueWarps * t.cluster));
         mbar_init(recv_free, uint32_t(kEpilogueWarps * t.cluster));
@@ -322,20 +386,29 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 2) {
-        tmem_alloc(smem_u32(&tmem_slot), uint32_t(t.tmem_cols));
-        tmem_relinquish();
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(t.tmem_cols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            tmem_alloc(smem_u32(&tmem_slot), uint32_t(t.tmem_cols));
+            tmem_relinquish();
+        }
     }
     grid_dependency_entry();
     build_table(p, t, first);
     tc_fence_before();
     __syncthreads();
-    if (t.cluster > 1) cluster_sync_all();
+    if (PAIR || t.cluster > 1) cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     const int total_tiles = first[p.groups];
-    const int rank = t.cluster > 1 ? int(cluster_cta_rank()) : 0;
-    const int tile0 = int(blockIdx.x) / t.cluster, tile_step = int(gridDim.x) / t.cluster;
-    const int k_begin = t.k_steps * rank / t.cluster, k_end = t.k_steps * (rank + 1) / t.cluster;
+    const int rank = PAIR || t.cluster > 1 ? int(cluster_cta_rank()) : 0;
+    const int sharing = PAIR ? 2 : t.cluster;                    // CTAs of a tile
+    const int tile0 = int(blockIdx.x) / sharing, tile_step = int(gridDim.x) / sharing;
+    const int k_begin = PAIR ? 0 : t.k_steps * rank / t.cluster, k_end = PAIR ? t.k_steps : t.k_steps * (rank + 1) / t.cluster;
+    const int cta_channel = PAIR ? rank * (t.tile_channels / 2) : 0;
+    // a pair's loads are counted in the CTA of rank 0, whose MMA issuer works for both
+    const uint32_t full_at = PAIR ? cluster_map(full0, 0) : full0;
     const int k_elems = kRowBytes / t.esize;
 
     if (LOADS != kRegs && warp == 0) {
@@ -346,18 +419,21 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             int armed = 0;
             bool ok = true;
             for (int i = tile0; i < total_tiles && ok; i += tile_step) {
-                const Tile tile = find_tile(p, t, first, i);
+                const Tile tile = find_tile(p, t, first, i, cta_channel);
                 for (int k = k_begin; k < k_end; ++k) {
                     ok = mbar_wait(empty0 + 8u * s, phase, nullptr);
                     if (!ok) break;
-                    const uint32_t dst = base + uint32_t(s) * stage_bytes, bar = full0 + 8u * s;
-                    mbar_expect_tx(bar, kATileBytes);
+                    const uint32_t dst = base + uint32_t(s) * stage_bytes, bar = full_at + 8u * s;
+                    if (!PAIR || rank == 0) mbar_expect_tx(full0 + 8u * s, (PAIR ? 2 : 1) * kATileBytes);
                     if (!p.gated) {
-                        tma_load_3d(dst, &map_w, bar, k * k_elems, tile.channel0, tile.group);
+                        if (PAIR) tma_load_3d_pair(dst, &map_w, bar, k * k_elems, tile.channel0, tile.group);
+                        else tma_load_3d(dst, &map_w, bar, k * k_elems, tile.channel0, tile.group);
                     } else {
 #pragma unroll
-                        for (int b = 0; b < 8; ++b)
-                            tma_load_3d(dst + uint32_t(b) * 16u * kRowBytes, &map_w, bar, k * k_elems, weight_row(p, tile, b * 16), tile.group);
+                        for (int b = 0; b < 8; ++b) {
+                            if (PAIR) tma_load_3d_pair(dst + uint32_t(b) * 16u * kRowBytes, &map_w, bar, k * k_elems, weight_row(p, tile, b * 16), tile.group);
+                            else tma_load_3d(dst + uint32_t(b) * 16u * kRowBytes, &map_w, bar, k * k_elems, weight_row(p, tile, b * 16), tile.group);
+                        }
                     }
                     ++armed;
                     if (++s == t.stages) { s = 0; phase ^= 1u; }
@@ -365,7 +441,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             }
             if (!ok) {
                 time_out(1);
-                for (int j = armed - 1, n = 0; j >= 0 && n < t.stages; --j, ++n)
+                for (int j = armed - 1, n = 0; j >= 0 && n < t.stages && (!PAIR || rank == 0); --j, ++n)
                     mbar_wait(full0 + 8u * (j % t.stages), uint32_t((j / t.stages) & 1), nullptr);
             }
         }
@@ -377,52 +453,49 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             int armed = 0;
             bool ok = true;
             for (int i = tile0; i < total_tiles && ok; i += tile_step) {
-                const Tile tile = find_tile(p, t, first, i);
-                const int loads = (tile.valid + t.box_rows - 1) / t.box_rows;
-                const uint32_t bytes = uint32_t(loads * t.box_rows) * kRowBytes;
+                const Tile tile = find_tile(p, t, first, i, cta_channel);
+                // a pair's CTAs hold half of the columns each
+                const int held = PAIR ? tile.cols / 2 : tile.cols, col0 = PAIR ? rank * held : 0;
+                const auto boxes = [&](int from) { return (max(0, min(held, tile.valid - from)) + t.box_rows - 1) / t.box_rows; };
+                const int loads = boxes(col0);
+                const uint32_t bytes = uint32_t((PAIR ? boxes(0) + boxes(held) : loads) * t.box_rows) * kRowBytes;
                 for (int k = k_begin; k < k_end; ++k) {
                     ok = mbar_wait(empty0 + 8u * s, phase, nullptr);
                     if (!ok) break;
-                    const uint32_t dst = base + uint32_t(s) * stage_bytes + kATileBytes, bar = full0 + 8u * s;
-                    mbar_expect_tx(bar, bytes);
-                    for (int b = 0; b < loads; ++b)
-                        tma_load_2d(dst + uint32_t(b * t.box_rows) * kRowBytes, &map_x, bar, k * k_elems, tile.row0 + b * t.box_rows);
+                    const uint32_t dst = base + uint32_t(s) * stage_bytes + kATileBytes, bar = full_at + 8u * s;
+                    if (!PAIR || rank == 0) mbar_expect_tx(full0 + 8u * s, bytes);
+                    for (int b = 0; b < loads; ++b) {
+                        const int row = tile.row0 + col0 + b * t.box_rows;
+                        if (PAIR) tma_load_2d_pair(dst + uint32_t(b * t.box_rows) * kRowBytes, &map_x, bar, k * k_elems, row);
+                        else tma_load_2d(dst + uint32_t(b * t.box_rows) * kRowBytes, &map_x, bar, k * k_elems, row);
+                    }
                     ++armed;
                     if (++s == t.stages) { s = 0; phase ^= 1u; }
                 }
             }
             if (!ok) {
                 time_out(2);
-                for (int j = armed - 1, n = 0; j >= 0 && n < t.stages; --j, ++n)
+                for (int j = armed - 1, n = 0; j >= 0 && n < t.stages && (!PAIR || rank == 0); --j, ++n)
                     mbar_wait(full0 + 8u * (j % t.stages), uint32_t((j / t.stages) & 1), nullptr);
             }
         }
     } else if (LOADS == kGather && warp >= kLoadWarp0) {
         // ---------------- gathered rows ----------------
-        // thread i of 128 moves 16-byte column i % 8 of columns i / 8, i / 8 + 16, ... of the tile.  A step is handed over
-        // once it has landed, `lag` steps after it was asked for (narrow tiles have many stages, and need them: a step is
-        // then a few KiB).
-        constexpr int kMost = 16;
-        const int lag = t.stages >= 8 ? 6 : 2;
+        // thread i of 128 moves 16-byte column i % 8 of columns i / 8, i / 8 + 16, ... of the tile
+        constexpr int kMost = PAIR ? 8 : 16;
         const int tid = int(threadIdx.x) - 32 * kLoadWarp0, c16 = tid & 7, r0 = tid >> 3;
         const long long row_bytes = (long long)p.inner * t.esize;
-        int s = 0, landed = 0, waiting = 0;
+        int s = 0;
         uint32_t phase = 1;
         bool ok = true;
-        auto hand_over = [&]() {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full0 + 8u * landed);
-            if (++landed == t.stages) landed = 0;
-            --waiting;
-        };
         for (int i = tile0; i < total_tiles && ok; i += tile_step) {
-            const Tile tile = find_tile(p, t, first, i);
+            const Tile tile = find_tile(p, t, first, i, cta_channel);
+            const int held = PAIR ? tile.cols / 2 : tile.cols, col0 = PAIR ? rank * held : 0;
             int src[kMost];
 #pragma unroll
             for (int j = 0; j < kMost; ++j) {
-                const int c = r0 + 16 * j;
-                const int r = c < tile.valid ? p.rows[tile.row0 + c] : -1;
+                const int c = col0 + r0 + 16 * j;
+                const int r = r0 + 16 * j < held && c < tile.valid ? p.rows[tile.row0 + c] : -1;
                 src[j] = r >= 0 && r < p.x_rows ? r : -1;
             }
             for (int k = k_begin; k < k_end; ++k) {
@@ -434,23 +507,37 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 const int left = int(min(max(row_bytes - byte0, 0LL), 16LL));
 #pragma unroll
                 for (int j = 0; j < kMost; ++j)
-                    if (16 * j < tile.cols) {
+                    if (16 * j < held) {
                         const bool live = src[j] >= 0 && left > 0;
                         const uint8_t *from = static_cast<const uint8_t *>(p.x) + (live ? (long long)src[j] * p.x_stride * t.esize + byte0 : 0);
                         cp_async16(dst + sw128_offset(r0 + 16 * j, c16), from, live ? left : 0);
                     }
-                asm volatile("cp.async.commit_group;" ::: "memory");
+                // arrives when this thread's copies have landed
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(landed0 + 8u * s) : "memory");
                 if (++s == t.stages) { s = 0; phase ^= 1u; }
-                if (++waiting > lag) {
-                    if (lag == 6) asm volatile("cp.async.wait_group 6;" ::: "memory");
-                    else asm volatile("cp.async.wait_group 2;" ::: "memory");
-                    hand_over();
-                }
             }
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        while (waiting > 0) hand_over();
+        asm volatile("cp.async.wait_all;" ::: "memory");
         if (!ok && lane == 0) time_out(2);
+    } else if (LOADS == kGather && warp == 3) {
+        // ---------------- hand-over of gathered rows ----------------
+        // The proxy fence between the copies and the tensor core is here and not in the gathering threads, where it would
+        // wait for every copy under way.
+        if (lane == 0) {
+            int s = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int i = tile0; i < total_tiles && ok; i += tile_step)
+                for (int k = k_begin; k < k_end; ++k) {
+                    ok = mbar_wait(landed0 + 8u * s, phase, nullptr);
+                    if (!ok) break;
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    if (PAIR) mbar_arrive_cluster(full_at + 8u * s);
+                    else mbar_arrive(full0 + 8u * s);
+                    if (++s == t.stages) { s = 0; phase ^= 1u; }
+                }
+            if (!ok) time_out(6);
+        }
     } else if (LOADS == kRegs && warp >= kLoadWarp0) {
         // ---------------- loader warps ----------------
         // thread i of 256 moves 16-byte column i % 8 of rows i / 8, i / 8 + 32, ...: four of the weights, up to four of x
@@ -460,7 +547,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         uint32_t phase = 1;
         bool ok = true;
         for (int i = tile0; i < total_tiles && ok; i += tile_step) {
-            const Tile tile = find_tile(p, t, first, i);
+            const Tile tile = find_tile(p, t, first, i, cta_channel);
             const int wide = p.gated ? 2 * p.channels : p.channels;
             const uint8_t *src[8];
 #pragma unroll
@@ -516,55 +603,56 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         if (!ok && lane == 0) time_out(3);
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
-        if (lane == 0) {
+        if (!PAIR || rank == 0) {
+            uint32_t elected;
+            asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.b32 %0, 1, 0, q;\n\t}" : "=r"(elected));
             int s = 0;
             uint32_t phase = 0;
             int turn = 0;                                       // accumulator hand-overs so far
             bool ok = true;
+            const uint32_t a_low0 = desc_low(base), stage_low = stage_bytes >> 4, b_low0 = kPlanes * kATileBytes >> 4;
             for (int i = tile0; i < total_tiles && ok; i += tile_step) {
-                const Tile tile = find_tile(p, t, first, i);
+                const Tile tile = find_tile(p, t, first, i, cta_channel);
                 // sums in float32 / int32 (bit 4 / 5), operand formats, both K-major, N and M
                 const uint32_t idesc = (KIND == kI8 ? 2u << 4 : 1u << 4) | (t.format << 7) | (t.format << 10) |
-                                       (uint32_t(tile.cols >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
+                                       (uint32_t(tile.cols >> 3) << 17) | (uint32_t((PAIR ? 2 : 1) * kTileM >> 4) << 24);
                 uint32_t acc = 0;
-                for (int k = k_begin; k < k_end && ok; ++k) {
+                for (int k = k_begin; k < k_end; ++k) {
                     const bool opens = KIND == kX3 ? (k - k_begin) % kChunkSteps == 0 : k == k_begin;
                     const bool closes = k + 1 == k_end || (KIND == kX3 && (k - k_begin) % kChunkSteps == kChunkSteps - 1);
                     const uint32_t a = uint32_t(turn) & 1u;
                     const uint32_t d = tmem + a * uint32_t(t.tn);
                     if (opens) {
-                        ok = mbar_wait(acc_empty0 + 8u * a, ((uint32_t(turn) >> 1) & 1u) ^ 1u, nullptr);
-                        tc_fence_after();
+                        ok = wait<PAIR>(acc_empty0 + 8u * a, ((uint32_t(turn) >> 1) & 1u) ^ 1u);
                         acc = 0;
                     }
-                    if (ok) ok = mbar_wait(full0 + 8u * s, phase, nullptr);
+                    if (ok) ok = wait<PAIR>(full0 + 8u * s, phase);
+                    ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t stage = base + uint32_t(s) * stage_bytes;
-                    const uint64_t da = smem_desc_kmajor(stage, 128), db = smem_desc_kmajor(stage + kPlanes * kATileBytes, 128);
-                    const uint64_t da_lo = smem_desc_kmajor(stage + kATileBytes, 128);
-                    const uint64_t db_lo = smem_desc_kmajor(stage + kPlanes * kATileBytes + b_bytes, 128);
+                    const uint32_t a_low = a_low0 + uint32_t(s) * stage_low, b_low = a_low + b_low0;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const uint64_t o = uint64_t(q * 2);
-                        if (KIND == kF16) umma_f16(d, da + o, db + o, idesc, acc);
-                        else if (KIND == kI8) umma_i8(d, da + o, db + o, idesc, acc);
-                        else {
-                            umma_tf32(d, da_lo + o, db + o, idesc, acc);
-                            umma_tf32(d, da + o, db_lo + o, idesc, 1u);
-                            umma_tf32(d, da + o, db + o, idesc, 1u);
+                    for (uint32_t q = 0; q < 8; q += 2) {
+                        if (KIND != kX3) {
+                            umma<KIND, PAIR>(elected, d, a_low + q, b_low + q, idesc, acc);
+                        } else {
+                            const uint32_t a_rest = a_low + (kATileBytes >> 4), b_rest = b_low + (b_bytes >> 4);
+                            umma<KIND, PAIR>(elected, d, a_rest + q, b_low + q, idesc, acc);
+                            umma<KIND, PAIR>(elected, d, a_low + q, b_rest + q, idesc, 1u);
+                            umma<KIND, PAIR>(elected, d, a_low + q, b_low + q, idesc, 1u);
                         }
                         acc = 1;
                     }
-                    umma_commit(empty0 + 8u * s);
-                    if (closes) {
-                        umma_commit(acc_full0 + 8u * a);
-                        ++turn;
+                    if (elected) {
+                        commit<PAIR>(empty0 + 8u * s);
+                        if (closes) commit<PAIR>(acc_full0 + 8u * a);
                     }
+                    __syncwarp();
+                    if (closes) ++turn;
                     if (++s == t.stages) { s = 0; phase ^= 1u; }
                 }
             }
-            if (!ok) time_out(4);
+            if (!ok && lane == 0) time_out(4);
         }
     } else if (warp >= 4 && warp < kLoadWarp0) {
         // ---------------- epilogue ----------------
@@ -581,7 +669,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         int turn = 0, round = 0;
         bool ok = true;
         for (int i = tile0; i < total_tiles && ok; i += tile_step, ++round) {
-            const Tile tile = find_tile(p, t, first, i);
+            const Tile tile = find_tile(p, t, first, i, cta_channel);
             const int half = p.gated ? (lane >> 4) : 0;
             const int warp_channel = tile.channel0 + quad * (p.gated ? 16 : 32);
             const int channel = warp_channel + (p.gated ? (lane & 15) : lane);
@@ -666,14 +754,14 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                         }
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(acc_empty0 + 8u * a);
+                    if (lane == 0) mbar_arrive(acc_empty0 + 8u * a);          // (no pairs)
                 }
                 if (!ok) break;
                 if (t.cluster == 1) {
 #pragma unroll
                     for (int c = 0; c < kLoaderCols; c += kStageCols) finish(sum + c, c);
                 } else {
-                    ok = round == 0 || mbar_wait_cluster(recv_free, uint32_t(round - 1) & 1u, nullptr);
+                    ok = round == 0 || wait<true>(recv_free, uint32_t(round - 1) & 1u);
                     ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
                     if (!ok) break;
                     const int per = tile.cols / t.cluster;
@@ -684,8 +772,8 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 }
             } else {
                 const uint32_t a = uint32_t(turn) & 1u;
-                ok = mbar_wait(acc_full0 + 8u * a, (uint32_t(turn) >> 1) & 1u, nullptr);
-                if (ok && t.cluster > 1 && round > 0) ok = mbar_wait_cluster(recv_free, uint32_t(round - 1) & 1u, nullptr);
+                ok = wait<PAIR>(acc_full0 + 8u * a, (uint32_t(turn) >> 1) & 1u);
+                if (ok && t.cluster > 1 && round > 0) ok = wait<true>(recv_free, uint32_t(round - 1) & 1u);
                 ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
                 if (!ok) break;
                 tc_fence_after();
@@ -710,7 +798,10 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(acc_empty0 + 8u * a);
+                if (lane == 0) {
+                    if (PAIR) mbar_arrive_cluster(cluster_map(acc_empty0 + 8u * a, 0));
+                    else mbar_arrive(acc_empty0 + 8u * a);
+                }
                 ++turn;
             }
             if (t.cluster > 1) {
@@ -718,7 +809,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 const int per = tile.cols / t.cluster;
                 __syncwarp();
                 if (lane < t.cluster) mbar_arrive_cluster(cluster_map(recv_full, uint32_t(lane)));
-                ok = mbar_wait_cluster(recv_full, uint32_t(round) & 1u, nullptr);
+                ok = wait<true>(recv_full, uint32_t(round) & 1u);
                 ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
                 if (!ok) break;
                 // (pairs of columns: a gated result takes two lanes' columns at once)
@@ -750,10 +841,12 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (t.cluster > 1) cluster_sync_all();       // nobody may still push into the shared memory of a CTA that has gone
+    // nobody may still push into, load into or multiply from the shared memory of a CTA that has gone
+    if (PAIR || t.cluster > 1) cluster_sync_all();
     if (warp == 2) {
         tc_fence_after();
-        tmem_dealloc(tmem, uint32_t(t.tmem_cols));
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(t.tmem_cols) : "memory");
+        else tmem_dealloc(tmem, uint32_t(t.tmem_cols));
     }
 }
 
@@ -810,7 +903,7 @@ int columns_for(const GroupedParams &p, int most) {
 }
 
 // Chooses the tiling; touches no device.  Returns the CTAs to launch.
-int choose(const GroupedParams &p, int sm_count, bool tma, MmGeom *t) {
+int choose(const GroupedParams &p, int sm_count, bool tma, MmGeom *t, bool *pair) {
     const int esize = elem_size(p.type);
     t->esize = esize;
     t->format = p.type == Elem::BF16 ? 1u : p.type == Elem::F16 ? 0u : p.type == Elem::S8 ? 1u : 2u;
@@ -824,27 +917,36 @@ int choose(const GroupedParams &p, int sm_count, bool tma, MmGeom *t) {
     // K split: as long as it fills SMs that would idle and leaves every CTA two K steps
     t->cluster = 1;
     while (t->cluster < 8 && t->tn <= 128 && tiles() * t->cluster * 2 <= sm_count && t->k_steps >= 4 * t->cluster) t->cluster *= 2;
-    t->box_rows = std::min(t->tn, 64);
+    // Pairs of CTAs share the rows of a tile of 256 channels: half of the loads of x per SM, and with them twice the K
+    // steps in flight.  Worth it once the tiles are wide and keep every pair busy.
+    *pair = tma && t->tn == 256 && (long long)ceil_div(p.channels, 2 * t->tile_channels) * ceil_div(p.total, t->tn) >= sm_count / 2;
+    t->grain = *pair ? 32 : 16;
+    if (*pair) {
+        t->tile_channels *= 2;
+        t->n_tiles = ceil_div(p.channels, t->tile_channels);
+    }
+    t->box_rows = std::min(*pair ? t->tn / 2 : t->tn, 64);
     t->tmem_cols = std::max(32, 2 * t->tn);
     const int planes = p.type == Elem::F32 ? 2 : 1;
-    const size_t stage = size_t(planes) * (kATileBytes + t->tn * kRowBytes);
+    const size_t stage = size_t(planes) * (kATileBytes + (*pair ? t->tn / 2 : t->tn) * kRowBytes);
     const size_t recv = t->cluster > 1 ? size_t(t->tn) * kTileM * sizeof(float) : 0;
     const size_t table = (size_t(p.groups + 1) * sizeof(int) + 15) / 16 * 16;
     const size_t turn = 8 * kTurnBytes;
-    const size_t fixed = 1024 + recv + turn + table + 2 * kMaxStages * 8 + 64 + 4096;       // 4096: the kernel's static shared memory
+    const size_t fixed = 1024 + recv + turn + table + kBarBytes + 4096;       // 4096: the kernel's static shared memory
     t->stages = int(std::min<size_t>(kMaxStages, (kSmemLimit - fixed) / stage));
     t->recv_off = int(t->stages * stage);
     t->turn_off = int(t->recv_off + recv);
     t->table_off = int(t->turn_off + turn);
     t->bar_off = int(t->table_off + table);
     const long long most = (long long)t->n_tiles * (p.total / t->tn + busy);         // no distribution needs more
-    return int(std::min<long long>(sm_count / t->cluster, most)) * t->cluster;
+    const int sharing = *pair ? 2 : t->cluster;
+    return int(std::min<long long>(sm_count / sharing, most)) * sharing;
 }
 
-template <int KIND, int LOADS>
+template <int KIND, int LOADS, bool PAIR>
 cudaError_t run(const GroupedParams &p, const MmGeom &t, int ctas, const CUtensorMap &map_w, const CUtensorMap &map_x, cudaStream_t stream) {
-    const int smem = t.bar_off + 2 * kMaxStages * 8 + 64 + 1024;
-    const auto kernel = expert_mm_kernel<KIND, LOADS>;
+    const int smem = t.bar_off + kBarBytes + 1024;
+    const auto kernel = expert_mm_kernel<KIND, LOADS, PAIR>;
     cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (err != cudaSuccess) return err;
     cudaLaunchConfig_t config = {};
@@ -854,7 +956,7 @@ cudaError_t run(const GroupedParams &p, const MmGeom &t, int ctas, const CUtenso
     config.stream = stream;
     cudaLaunchAttribute attribute = {};
     attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = unsigned(t.cluster);
+    attribute.val.clusterDim.x = unsigned(PAIR ? 2 : t.cluster);
     attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
     config.attrs = &attribute;
     config.numAttrs = 1;
@@ -879,24 +981,28 @@ cudaError_t launch_grouped(const GroupedParams &given, cudaStream_t stream) {
     if (p.x_rows <= 1) p.x_stride = apart;
     if (wide == 1) p.w_stride = apart;
     MmGeom t = {};
+    bool pair = false;
     bool tma = tma_able(p) && encode_fn();
-    int ctas = choose(p, sm_count, tma, &t);
+    int ctas = choose(p, sm_count, tma, &t, &pair);
     alignas(64) CUtensorMap map_w = {}, map_x = {};
     if (tma) {
         const long long stack_bytes = p.groups == 1 ? 16 : p.w_group_stride * t.esize;
         if (!encode(&map_w, p.type, p.w, p.inner, wide, p.w_stride * t.esize, p.groups, stack_bytes, p.gated ? 16 : kTileM, 3) ||
             (!p.rows && !encode(&map_x, p.type, p.x, p.inner, p.x_rows, p.x_stride * t.esize, 1, 0, t.box_rows, 2))) {
             tma = false;                             // a shape that no tensor map describes
-            ctas = choose(p, sm_count, tma, &t);
+            ctas = choose(p, sm_count, tma, &t, &pair);
         }
     }
-    if (p.type == Elem::F32) return run<kX3, kRegs>(p, t, ctas, map_w, map_x, stream);
+    const auto launch = [&](auto kernel) { return kernel(p, t, ctas, map_w, map_x, stream); };
+    if (p.type == Elem::F32) return launch(run<kX3, kRegs, false>);
     if (p.type == Elem::S8) {
-        if (!tma) return run<kI8, kRegs>(p, t, ctas, map_w, map_x, stream);
-        return p.rows ? run<kI8, kGather>(p, t, ctas, map_w, map_x, stream) : run<kI8, kTma>(p, t, ctas, map_w, map_x, stream);
+        if (!tma) return launch(run<kI8, kRegs, false>);
+        if (pair) return p.rows ? launch(run<kI8, kGather, true>) : launch(run<kI8, kTma, true>);
+        return p.rows ? launch(run<kI8, kGather, false>) : launch(run<kI8, kTma, false>);
     }
-    if (!tma) return run<kF16, kRegs>(p, t, ctas, map_w, map_x, stream);
-    return p.rows ? run<kF16, kGather>(p, t, ctas, map_w, map_x, stream) : run<kF16, kTma>(p, t, ctas, map_w, map_x, stream);
+    if (!tma) return launch(run<kF16, kRegs, false>);
+    if (pair) return p.rows ? launch(run<kF16, kGather, true>) : launch(run<kF16, kTma, true>);
+    return p.rows ? launch(run<kF16, kGather, false>) : launch(run<kF16, kTma, false>);
 }
 
 cudaError_t expert_mm_status(cudaStream_t stream, int *code) {

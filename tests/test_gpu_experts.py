@@ -239,6 +239,17 @@ def test_grouped_product_uneven_groups(dtype, counts):
     run_grouped(sum(counts), 4, 160, 144, dtype, counts=counts)
 
 
+# enough rows and channels that two CTAs work on a tile together
+@pytest.mark.parametrize('dtype', [BF16, F16, S8], ids=['bf16', 'fp16', 'int8'])
+@pytest.mark.parametrize('gather', [False, True])
+@pytest.mark.parametrize('counts,inner,channels', [
+    ([1700, 0, 3300], 192, 1100), ([256, 4097, 1, 31, 33, 600], 72, 1300), ([5000], 1000, 1030), ([130] * 40, 64, 513)])
+def test_grouped_product_in_pairs(dtype, gather, counts, inner, channels):
+    run_grouped(sum(counts), len(counts), inner, channels, dtype, counts=counts, gather=gather)
+    run_grouped(sum(counts), len(counts), inner, channels, dtype, counts=counts, gather=gather, gated=True, act='silu',
+                bias=True, scales=True, out_dtype=F32)
+
+
 def test_grouped_product_of_many_groups():
     run_grouped(4000, 1024, 64, 48, BF16, skew=0.3)
 
