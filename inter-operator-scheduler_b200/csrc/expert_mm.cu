@@ -51,7 +51,7 @@ constexpr int kTurnBytes = kStageCols * 32 * 2; // ... in this much shared memor
 constexpr int kChunkSteps = 4;                  // float32: K steps per partial sum
 constexpr int kMaxStages = 12;
 constexpr int kMaxGroupTiles = INT_MAX / kMaxExperts - 1;    // tiles of a group: their sum over all groups fits an int
-constexpr int kBarBytes = 3 * kMaxStages * 8 + 48;    // mbarriers: three per stage, six more
+constexpr int kBarBytes = 2 * kMaxStages * 8 + 48;    // mbarriers: two per stage, six more
 constexpr size_t kSmemLimit = 227 * 1024;
 
 __device__ int g_expert_error;                  // set by a wait that ran out, read by expert_mm_status
@@ -65,6 +65,7 @@ struct MmGeom {
     int cluster;        // CTAs that share a tile's K range
     int stages;
     int box_rows;       // rows per TMA box of x
+    int one_box;        // 1: (gated) the tile's alternating rows are one box of a five-dimensional view
     int tmem_cols;
     uint32_t format;    // operand format field of the instruction descriptor
     int esize;
@@ -154,28 +155,49 @@ __device__ __forceinline__ int weight_row(const GroupedParams &p, const Tile &ti
     return ((r >> 4) & 1) * p.channels + tile.channel0 + (r >> 5) * 16 + (r & 15);
 }
 
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void *tmap, uint32_t bar, int c0, int c1, int c2) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-        ::"r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
-        : "memory");
+// Loads into shared memory, counted on `bar` -- with PAIR that may be the other CTA's.  Like umma below they are called by
+// a whole warp with equal arguments and issued by one lane: from a branch that only one lane takes, every operand has to
+// be moved to a uniform register on the spot, which costs some 100 cycles per load.
+#define IOS_TMA(RANK, MODE, COORDS, ...)                                                                       \
+    do {                                                                                                       \
+        if (PAIR)                                                                                              \
+            asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t"                                       \
+                         "@q cp.async.bulk.tensor." RANK ".cta_group::2.shared::cluster.global" MODE             \
+                         ".mbarrier::complete_tx::bytes [%1], [%2, {" COORDS "}], [%3];\n\t}"                    \
+                         ::"r"(elected), "r"(dst), "l"(tmap), "r"(bar), __VA_ARGS__ : "memory");                \
+        else                                                                                                   \
+            asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t"                                       \
+                         "@q cp.async.bulk.tensor." RANK ".shared::cluster.global" MODE                          \
+                         ".mbarrier::complete_tx::bytes [%1], [%2, {" COORDS "}], [%3];\n\t}"                    \
+                         ::"r"(elected), "r"(dst), "l"(tmap), "r"(bar), __VA_ARGS__ : "memory");                \
+    } while (0)
+template <bool PAIR>
+__device__ __forceinline__ void load_2d(uint32_t elected, uint32_t dst, const void *tmap, uint32_t bar, int c0, int c1) {
+    IOS_TMA("2d", "", "%4, %5", "r"(c0), "r"(c1));
 }
-// The same loads by one CTA of a pair: the bytes are counted on `bar`, which may be in either CTA's shared memory.
-__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void *tmap, uint32_t bar, int c0, int c1, int c2) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-        ::"r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
-        : "memory");
+template <bool PAIR>
+__device__ __forceinline__ void load_3d(uint32_t elected, uint32_t dst, const void *tmap, uint32_t bar, int c0, int c1, int c2) {
+    IOS_TMA("3d", "", "%4, %5, %6", "r"(c0), "r"(c1), "r"(c2));
 }
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void *tmap, uint32_t bar, int c0, int c1) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-        ::"r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(c1)
-        : "memory");
+template <bool PAIR>
+__device__ __forceinline__ void load_5d(uint32_t elected, uint32_t dst, const void *tmap, uint32_t bar, int c0, int c3, int c4) {
+    IOS_TMA("5d", "", "%4, %7, %7, %5, %6", "r"(c0), "r"(c3), "r"(c4), "r"(0));
 }
-// 16 bytes into shared memory of which `bytes` come from memory, the rest are zeros
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// four rows of a matrix, any four, behind one another
+template <bool PAIR>
+__device__ __forceinline__ void load_rows4(uint32_t elected, uint32_t dst, const void *tmap, uint32_t bar, int c0, int4 rows) {
+    IOS_TMA("2d", ".tile::gather4", "%4, %5, %6, %7, %8", "r"(c0), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w));
+}
+#undef IOS_TMA
+// one arrival and `bytes` to come
+__device__ __forceinline__ void expect(uint32_t elected, uint32_t bar, uint32_t bytes) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t"
+                 "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%1], %2;\n\t}" ::"r"(elected), "r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint32_t elect() {
+    uint32_t elected;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.b32 %0, 1, 0, q;\n\t}" : "=r"(elected));
+    return elected;
 }
 // Low word of a K-major operand's descriptor (128-byte swizzle); the high word is the same for all.
 __device__ __forceinline__ uint32_t desc_low(uint32_t addr) { return ((addr & 0x3FFFF) >> 4) | (1u << 16); }
@@ -359,6 +381,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     constexpr int kEpilogueWarps = epilogue_warps(LOADS), kLoadWarp0 = 4 + kEpilogueWarps;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(16) float row_scale_s[2][256];
+    __shared__ uint32_t live_s[2][8];                            // one bit per column: its row exists
     __shared__ uint32_t tmem_slot;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *generic = smem_raw + (base - smem_u32(smem_raw));
@@ -367,13 +390,12 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     const uint32_t stage_bytes = kPlanes * (kATileBytes + b_bytes);
     const uint32_t full0 = base + t.bar_off, empty0 = full0 + 8u * t.stages;
     const uint32_t acc_full0 = empty0 + 8u * t.stages, acc_empty0 = acc_full0 + 16u;
-    const uint32_t recv_full = acc_empty0 + 16u, recv_free = recv_full + 8u, landed0 = recv_free + 8u;
+    const uint32_t recv_full = acc_empty0 + 16u, recv_free = recv_full + 8u;
     int *first = reinterpret_cast<int *>(generic + t.table_off);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < t.stages; ++s) {
-            mbar_init(full0 + 8u * s, LOADS == kTma ? 2 : LOADS == kGather ? (PAIR ? 3 : 2) : kLoaderWarps);
-            mbar_init(landed0 + 8u * s, 32 * kGatherWarps);
+            mbar_init(full0 + 8u * s, LOADS == kRegs ? kLoaderWarps : 1);
             mbar_init(empty0 + 8u * s, 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -411,133 +433,102 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     const uint32_t full_at = PAIR ? cluster_map(full0, 0) : full0;
     const int k_elems = kRowBytes / t.esize;
 
+    // Bytes that the rows of one K step bring into the CTA that holds columns from `col0` on.  Every warp that brings rows
+    // brings some, also where the tile needs none: otherwise the ring of stages could run on without it, and a wait by
+    // parity does not notice two rounds.
+    const auto row_bytes_of = [&](const Tile &tile, int col0) {
+        const int unit = LOADS == kGather ? 4 : t.box_rows, least = LOADS == kGather ? 4 * kGatherWarps : 1;
+        const int rows = max(least, min(PAIR ? tile.cols / 2 : tile.cols, tile.valid - col0));
+        return uint32_t((rows + unit - 1) / unit * unit) * kRowBytes;
+    };
     if (LOADS != kRegs && warp == 0) {
-        // ---------------- weights ----------------
-        if (lane == 0) {
-            int s = 0;
-            uint32_t phase = 1;
-            int armed = 0;
-            bool ok = true;
-            for (int i = tile0; i < total_tiles && ok; i += tile_step) {
-                const Tile tile = find_tile(p, t, first, i, cta_channel);
-                for (int k = k_begin; k < k_end; ++k) {
-                    ok = mbar_wait(empty0 + 8u * s, phase, nullptr);
-                    if (!ok) break;
-                    const uint32_t dst = base + uint32_t(s) * stage_bytes, bar = full_at + 8u * s;
-                    if (!PAIR || rank == 0) mbar_expect_tx(full0 + 8u * s, (PAIR ? 2 : 1) * kATileBytes);
-                    if (!p.gated) {
-                        if (PAIR) tma_load_3d_pair(dst, &map_w, bar, k * k_elems, tile.channel0, tile.group);
-                        else tma_load_3d(dst, &map_w, bar, k * k_elems, tile.channel0, tile.group);
-                    } else {
+        // ---------------- weights; arms the stage's barrier for the rows as well ----------------
+        const uint32_t elected = elect();
+        int s = 0;
+        uint32_t phase = 1;
+        int armed = 0;
+        bool ok = true;
+        for (int i = tile0; i < total_tiles && ok; i += tile_step) {
+            const Tile tile = find_tile(p, t, first, i, cta_channel);
+            const uint32_t bytes = (PAIR ? 2 : 1) * kATileBytes + row_bytes_of(tile, 0) + (PAIR ? row_bytes_of(tile, tile.cols / 2) : 0);
+            for (int k = k_begin; k < k_end; ++k) {
+                ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
+                if (!ok) break;
+                const uint32_t dst = base + uint32_t(s) * stage_bytes, bar = full_at + 8u * s;
+                if (!PAIR || rank == 0) expect(elected, full0 + 8u * s, bytes);
+                if (!p.gated) {
+                    load_3d<PAIR>(elected, dst, &map_w, bar, k * k_elems, tile.channel0, tile.group);
+                } else if (t.one_box) {
+                    load_5d<PAIR>(elected, dst, &map_w, bar, k * k_elems, tile.channel0 / 16, tile.group);
+                } else {
 #pragma unroll
-                        for (int b = 0; b < 8; ++b) {
-                            if (PAIR) tma_load_3d_pair(dst + uint32_t(b) * 16u * kRowBytes, &map_w, bar, k * k_elems, weight_row(p, tile, b * 16), tile.group);
-                            else tma_load_3d(dst + uint32_t(b) * 16u * kRowBytes, &map_w, bar, k * k_elems, weight_row(p, tile, b * 16), tile.group);
-                        }
-                    }
-                    ++armed;
-                    if (++s == t.stages) { s = 0; phase ^= 1u; }
+                    for (int b = 0; b < 8; ++b)
+                        load_3d<PAIR>(elected, dst + uint32_t(b) * 16u * kRowBytes, &map_w, bar, k * k_elems, weight_row(p, tile, b * 16), tile.group);
                 }
+                ++armed;
+                if (++s == t.stages) { s = 0; phase ^= 1u; }
             }
-            if (!ok) {
-                time_out(1);
-                for (int j = armed - 1, n = 0; j >= 0 && n < t.stages && (!PAIR || rank == 0); --j, ++n)
-                    mbar_wait(full0 + 8u * (j % t.stages), uint32_t((j / t.stages) & 1), nullptr);
-            }
+        }
+        if (!ok) {
+            if (lane == 0) time_out(1);
+            for (int j = armed - 1, n = 0; j >= 0 && n < t.stages && (!PAIR || rank == 0); --j, ++n)
+                mbar_wait(full0 + 8u * (j % t.stages), uint32_t((j / t.stages) & 1), nullptr);
         }
     } else if (LOADS == kTma && warp == 3) {
         // ---------------- rows ----------------
-        if (lane == 0) {
-            int s = 0;
-            uint32_t phase = 1;
-            int armed = 0;
-            bool ok = true;
-            for (int i = tile0; i < total_tiles && ok; i += tile_step) {
-                const Tile tile = find_tile(p, t, first, i, cta_channel);
-                // a pair's CTAs hold half of the columns each
-                const int held = PAIR ? tile.cols / 2 : tile.cols, col0 = PAIR ? rank * held : 0;
-                const auto boxes = [&](int from) { return (max(0, min(held, tile.valid - from)) + t.box_rows - 1) / t.box_rows; };
-                const int loads = boxes(col0);
-                const uint32_t bytes = uint32_t((PAIR ? boxes(0) + boxes(held) : loads) * t.box_rows) * kRowBytes;
-                for (int k = k_begin; k < k_end; ++k) {
-                    ok = mbar_wait(empty0 + 8u * s, phase, nullptr);
-                    if (!ok) break;
-                    const uint32_t dst = base + uint32_t(s) * stage_bytes + kATileBytes, bar = full_at + 8u * s;
-                    if (!PAIR || rank == 0) mbar_expect_tx(full0 + 8u * s, bytes);
-                    for (int b = 0; b < loads; ++b) {
-                        const int row = tile.row0 + col0 + b * t.box_rows;
-                        if (PAIR) tma_load_2d_pair(dst + uint32_t(b * t.box_rows) * kRowBytes, &map_x, bar, k * k_elems, row);
-                        else tma_load_2d(dst + uint32_t(b * t.box_rows) * kRowBytes, &map_x, bar, k * k_elems, row);
-                    }
-                    ++armed;
-                    if (++s == t.stages) { s = 0; phase ^= 1u; }
-                }
-            }
-            if (!ok) {
-                time_out(2);
-                for (int j = armed - 1, n = 0; j >= 0 && n < t.stages && (!PAIR || rank == 0); --j, ++n)
-                    mbar_wait(full0 + 8u * (j % t.stages), uint32_t((j / t.stages) & 1), nullptr);
-            }
-        }
-    } else if (LOADS == kGather && warp >= kLoadWarp0) {
-        // ---------------- gathered rows ----------------
-        // thread i of 128 moves 16-byte column i % 8 of columns i / 8, i / 8 + 16, ... of the tile
-        constexpr int kMost = PAIR ? 8 : 16;
-        const int tid = int(threadIdx.x) - 32 * kLoadWarp0, c16 = tid & 7, r0 = tid >> 3;
-        const long long row_bytes = (long long)p.inner * t.esize;
+        const uint32_t elected = elect();
         int s = 0;
         uint32_t phase = 1;
         bool ok = true;
         for (int i = tile0; i < total_tiles && ok; i += tile_step) {
             const Tile tile = find_tile(p, t, first, i, cta_channel);
-            const int held = PAIR ? tile.cols / 2 : tile.cols, col0 = PAIR ? rank * held : 0;
-            int src[kMost];
-#pragma unroll
-            for (int j = 0; j < kMost; ++j) {
-                const int c = col0 + r0 + 16 * j;
-                const int r = r0 + 16 * j < held && c < tile.valid ? p.rows[tile.row0 + c] : -1;
-                src[j] = r >= 0 && r < p.x_rows ? r : -1;
-            }
+            const int col0 = PAIR ? rank * (tile.cols / 2) : 0;              // a pair's CTAs hold half of the columns each
+            const int loads = int(row_bytes_of(tile, col0)) / (t.box_rows * kRowBytes);
             for (int k = k_begin; k < k_end; ++k) {
-                ok = mbar_wait(empty0 + 8u * s, phase, nullptr);
-                ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
+                ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
                 if (!ok) break;
-                const uint32_t dst = base + uint32_t(s) * stage_bytes + kATileBytes;
-                const long long byte0 = (long long)k * kRowBytes + c16 * 16;
-                const int left = int(min(max(row_bytes - byte0, 0LL), 16LL));
-#pragma unroll
-                for (int j = 0; j < kMost; ++j)
-                    if (16 * j < held) {
-                        const bool live = src[j] >= 0 && left > 0;
-                        const uint8_t *from = static_cast<const uint8_t *>(p.x) + (live ? (long long)src[j] * p.x_stride * t.esize + byte0 : 0);
-                        cp_async16(dst + sw128_offset(r0 + 16 * j, c16), from, live ? left : 0);
-                    }
-                // arrives when this thread's copies have landed
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(landed0 + 8u * s) : "memory");
+                const uint32_t dst = base + uint32_t(s) * stage_bytes + kATileBytes, bar = full_at + 8u * s;
+                for (int b = 0; b < loads; ++b)
+                    load_2d<PAIR>(elected, dst + uint32_t(b * t.box_rows) * kRowBytes, &map_x, bar, k * k_elems, tile.row0 + col0 + b * t.box_rows);
                 if (++s == t.stages) { s = 0; phase ^= 1u; }
             }
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
         if (!ok && lane == 0) time_out(2);
-    } else if (LOADS == kGather && warp == 3) {
-        // ---------------- hand-over of gathered rows ----------------
-        // The proxy fence between the copies and the tensor core is here and not in the gathering threads, where it would
-        // wait for every copy under way.
-        if (lane == 0) {
-            int s = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int i = tile0; i < total_tiles && ok; i += tile_step)
-                for (int k = k_begin; k < k_end; ++k) {
-                    ok = mbar_wait(landed0 + 8u * s, phase, nullptr);
-                    if (!ok) break;
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    if (PAIR) mbar_arrive_cluster(full_at + 8u * s);
-                    else mbar_arrive(full0 + 8u * s);
-                    if (++s == t.stages) { s = 0; phase ^= 1u; }
+    } else if (LOADS == kGather && warp >= kLoadWarp0) {
+        // ---------------- gathered rows: every fourth group of four to each of four warps ----------------
+        constexpr int kMost = (PAIR ? 128 : 256) / (4 * kGatherWarps);
+        const uint32_t elected = elect();
+        const int part = warp - kLoadWarp0;
+        int s = 0;
+        uint32_t phase = 1;
+        bool ok = true;
+        for (int i = tile0; i < total_tiles && ok; i += tile_step) {
+            const Tile tile = find_tile(p, t, first, i, cta_channel);
+            const int col0 = PAIR ? rank * (tile.cols / 2) : 0;
+            const int loads = int(row_bytes_of(tile, col0)) / (4 * kRowBytes);
+            int4 src[kMost];
+#pragma unroll
+            for (int j = 0; j < kMost; ++j) {
+                int at[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int r = p.rows[tile.row0 + min(col0 + (j * kGatherWarps + part) * 4 + q, tile.valid - 1)];
+                    at[q] = r >= 0 && r < p.x_rows ? r : 0;           // the epilogue makes zeros of a row that is none
                 }
-            if (!ok) time_out(6);
+                src[j] = make_int4(at[0], at[1], at[2], at[3]);
+            }
+            for (int k = k_begin; k < k_end; ++k) {
+                ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
+                if (!ok) break;
+                const uint32_t dst = base + uint32_t(s) * stage_bytes + kATileBytes, bar = full_at + 8u * s;
+#pragma unroll
+                for (int j = 0; j < kMost; ++j)
+                    if (j * kGatherWarps + part < loads)
+                        load_rows4<PAIR>(elected, dst + uint32_t(j * kGatherWarps + part) * 4u * kRowBytes, &map_x, bar, k * k_elems, src[j]);
+                if (++s == t.stages) { s = 0; phase ^= 1u; }
+            }
         }
+        if (!ok && lane == 0) time_out(3);
     } else if (LOADS == kRegs && warp >= kLoadWarp0) {
         // ---------------- loader warps ----------------
         // thread i of 256 moves 16-byte column i % 8 of rows i / 8, i / 8 + 32, ...: four of the weights, up to four of x
@@ -600,12 +591,11 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 for (int j = 0; j < 8; ++j) now[j] = next[j];
             }
         }
-        if (!ok && lane == 0) time_out(3);
+        if (!ok && lane == 0) time_out(6);
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
         if (!PAIR || rank == 0) {
-            uint32_t elected;
-            asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.b32 %0, 1, 0, q;\n\t}" : "=r"(elected));
+            const uint32_t elected = elect();
             int s = 0;
             uint32_t phase = 0;
             int turn = 0;                                       // accumulator hand-overs so far
@@ -682,10 +672,14 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             o.channels = max(0, min(p.gated ? 16 : 32, p.channels - warp_channel));
             o.vectors = ((reinterpret_cast<uintptr_t>(o.first) | uintptr_t(o.row_bytes)) & 15) == 0 && o.channels == (p.gated ? 16 : 32);
             const float *row_scale = row_scale_s[round & 1];
-            if (p.row_scale) {
-                for (int c = tid; c < t.tn; c += 32 * kEpilogueWarps) {
-                    const int src = c < tile.valid ? (p.rows ? p.rows[tile.row0 + c] : tile.row0 + c) : -1;
-                    row_scale_s[round & 1][c] = src >= 0 && src < p.x_rows ? p.row_scale[src] : 1.0f;
+            const uint32_t *live = live_s[round & 1];
+            if (p.row_scale || LOADS == kGather) {
+                for (int c = tid; c < max(t.tn, 32); c += 32 * kEpilogueWarps) {              // whole warps
+                    const int src = c >= tile.valid ? 0 : p.rows ? p.rows[tile.row0 + c] : tile.row0 + c;
+                    const bool known = src >= 0 && src < p.x_rows;
+                    row_scale_s[round & 1][c] = p.row_scale && known ? p.row_scale[src] : 1.0f;
+                    const uint32_t mask = __ballot_sync(0xffffffffu, known);
+                    if (lane == 0) live_s[round & 1][c >> 5] = mask;
                 }
                 asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory");
             }
@@ -695,6 +689,14 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 if (KIND == kI8) {
 #pragma unroll
                     for (int c = 0; c < kStageCols; ++c) v[c] = float(__float_as_int(v[c]));
+                }
+                if (LOADS == kGather) {                       // a row that is none was loaded as some other one
+                    const uint32_t mask = __funnelshift_r(live[c0 >> 5], live[min(c0 >> 5, 6) + 1], c0);
+                    if (mask != 0xffffffffu) {
+#pragma unroll
+                        for (int c = 0; c < kStageCols; ++c)
+                            if (!((mask >> c) & 1u)) v[c] = 0.0f;
+                    }
                 }
                 if (p.row_scale) {
                     if (t.cluster == 1) {                     // c0 is a multiple of 32, t.tn of 16
@@ -865,18 +867,39 @@ EncodeTiledFn encode_fn() {
     return fn;
 }
 
-// A tensor map of a matrix (or a stack of them) with rows of `inner` elements; boxes of one swizzle row x box_rows.
-bool encode(CUtensorMap *map, Elem type, const void *base, long long inner, long long rows, long long row_bytes, long long stack,
-            long long stack_bytes, int box_rows, int rank) {
+bool encode(CUtensorMap *map, Elem type, const void *base, int rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
     const CUtensorMapDataType types[] = {CU_TENSOR_MAP_DATA_TYPE_FLOAT32, CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                                          CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_DATA_TYPE_UINT8};
-    const cuuint64_t dims[3] = {cuuint64_t(inner), cuuint64_t(rows), cuuint64_t(stack)};
-    const cuuint64_t strides[2] = {cuuint64_t(row_bytes), cuuint64_t(stack_bytes)};
-    const cuuint32_t box[3] = {cuuint32_t(kRowBytes / elem_size(type)), cuuint32_t(box_rows), 1};
-    const cuuint32_t steps[3] = {1, 1, 1};
+    const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
     return encode_fn()(map, types[int(type)], cuuint32_t(rank), const_cast<void *>(base), dims, strides, box, steps,
                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The weights: boxes of one swizzle row x 128 rows of a group; gated: (element, channel of 16, half, block of 16 channels, group)
+// in boxes of 16 x 2 x 4 channels, or 16 rows at a time where the channels do not come in sixteens.
+bool encode_weights(CUtensorMap *map, const GroupedParams &p, const MmGeom &t) {
+    const cuuint64_t row = cuuint64_t(p.w_stride) * t.esize, wide = cuuint64_t(p.gated ? 2 : 1) * p.channels;
+    const cuuint64_t group = p.groups == 1 ? 16 : cuuint64_t(p.w_group_stride) * t.esize;      // (one group: no stride needed)
+    const cuuint32_t elems = cuuint32_t(kRowBytes / t.esize);
+    if (t.one_box) {
+        const cuuint64_t dims[5] = {cuuint64_t(p.inner), 16, 2, cuuint64_t(p.channels / 16), cuuint64_t(p.groups)};
+        const cuuint64_t strides[4] = {row, row * p.channels, row * 16, group};
+        const cuuint32_t box[5] = {elems, 16, 2, 4, 1};
+        return encode(map, p.type, p.w, 5, dims, strides, box);
+    }
+    const cuuint64_t dims[3] = {cuuint64_t(p.inner), wide, cuuint64_t(p.groups)};
+    const cuuint64_t strides[2] = {row, group};
+    const cuuint32_t box[3] = {elems, cuuint32_t(p.gated ? 16 : kTileM), 1};
+    return encode(map, p.type, p.w, 3, dims, strides, box);
+}
+
+// The rows: boxes of box_rows of them, or single ones to gather.
+bool encode_rows(CUtensorMap *map, const GroupedParams &p, const MmGeom &t) {
+    const cuuint64_t dims[2] = {cuuint64_t(p.inner), cuuint64_t(p.x_rows)};
+    const cuuint64_t strides[1] = {cuuint64_t(p.x_stride) * t.esize};
+    const cuuint32_t box[2] = {cuuint32_t(kRowBytes / t.esize), cuuint32_t(p.rows ? 1 : t.box_rows)};
+    return encode(map, p.type, p.x, 2, dims, strides, box);
 }
 
 // May TMA read rows of this stride?  (16-byte aligned rows that do not overlap, strides below 2^40 bytes)
@@ -925,6 +948,7 @@ int choose(const GroupedParams &p, int sm_count, bool tma, MmGeom *t, bool *pair
         t->tile_channels *= 2;
         t->n_tiles = ceil_div(p.channels, t->tile_channels);
     }
+    t->one_box = p.gated && p.channels % 16 == 0;
     t->box_rows = std::min(*pair ? t->tn / 2 : t->tn, 64);
     t->tmem_cols = std::max(32, 2 * t->tn);
     const int planes = p.type == Elem::F32 ? 2 : 1;
@@ -986,9 +1010,7 @@ cudaError_t launch_grouped(const GroupedParams &given, cudaStream_t stream) {
     int ctas = choose(p, sm_count, tma, &t, &pair);
     alignas(64) CUtensorMap map_w = {}, map_x = {};
     if (tma) {
-        const long long stack_bytes = p.groups == 1 ? 16 : p.w_group_stride * t.esize;
-        if (!encode(&map_w, p.type, p.w, p.inner, wide, p.w_stride * t.esize, p.groups, stack_bytes, p.gated ? 16 : kTileM, 3) ||
-            (!p.rows && !encode(&map_x, p.type, p.x, p.inner, p.x_rows, p.x_stride * t.esize, 1, 0, t.box_rows, 2))) {
+        if (!encode_weights(&map_w, p, t) || !encode_rows(&map_x, p, t)) {
             tma = false;                             // a shape that no tensor map describes
             ctas = choose(p, sm_count, tma, &t, &pair);
         }
