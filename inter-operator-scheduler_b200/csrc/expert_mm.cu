@@ -46,8 +46,9 @@ __host__ __device__ constexpr int threads_of(int loads) {
     return 32 * (4 + epilogue_warps(loads) + (loads == kTma ? 0 : loads == kGather ? kGatherWarps : kLoaderWarps));
 }
 constexpr int kLoaderCols = 128;                // widest tile of the loader warps (their registers hold a step)
-constexpr int kStageCols = 32;                  // columns an epilogue warp turns round at a time
-constexpr int kTurnBytes = kStageCols * 32 * 2; // ... in this much shared memory (float32: in two halves)
+constexpr int kTurnCols = 16;                   // columns an epilogue warp turns round at a time: few, because a small
+                                                // product runs this code once, and cold code costs more than it does
+constexpr int kTurnBytes = kTurnCols * 32 * 4;  // ... in this much shared memory
 constexpr int kChunkSteps = 4;                  // float32: K steps per partial sum
 constexpr int kMaxStages = 12;
 constexpr int kMaxGroupTiles = INT_MAX / kMaxExperts - 1;    // tiles of a group: their sum over all groups fits an int
@@ -76,32 +77,44 @@ struct Tile {
     int group, row0, valid, cols, channel0;
 };
 
-// offsets come from the device: whatever they hold, a group stays inside [0, total]
-__device__ __forceinline__ void group_rows(const GroupedParams &p, int g, int *begin, int *count) {
-    if (!p.offsets) { *begin = 0; *count = p.total; return; }
-    *begin = min(max(p.offsets[g], 0), p.total);
-    *count = min(max(p.offsets[g + 1], *begin), p.total) - *begin;
-}
 // Columns per tile of a group: its rows dealt evenly to the fewest tiles.
 __device__ __forceinline__ int even_cols(int count, const MmGeom &t) {
     const int tiles = (count + t.tn - 1) / t.tn;
     return ((count + tiles - 1) / tiles + t.grain - 1) & -t.grain;
 }
 
-// first[g] = tiles before group g, for all groups; all threads call it
-__device__ void build_table(const GroupedParams &p, const MmGeom &t, int *first) {
+// The list of tiles: bound[g] = first row of group g, first[g] = tiles before group g.  Offsets come from the device:
+// whatever they hold, a group stays inside [0, total].  All threads call it; a barrier has to follow.
+struct Table {
+    int *bound, *first;       // groups + 1 each, in shared memory
+};
+__device__ __forceinline__ int tiles_of(int count, const MmGeom &t) {
+    if (count <= 0) return 0;
+    const int cols = even_cols(count, t);
+    return int(min((long long)((count + cols - 1) / cols) * t.n_tiles, (long long)kMaxGroupTiles));
+}
+__device__ void build_table(const GroupedParams &p, const MmGeom &t, const Table &table, int threads) {
+    if (p.groups == 1) {
+        if (threadIdx.x == 0) {
+            const int begin = p.offsets ? min(max(p.offsets[0], 0), p.total) : 0;
+            const int end = p.offsets ? min(max(p.offsets[1], begin), p.total) : p.total;
+            table.bound[0] = begin;
+            table.bound[1] = end;
+            table.first[0] = 0;
+            table.first[1] = tiles_of(end - begin, t);
+        }
+        return;
+    }
     __shared__ int warp_total[kMaxThreads / 32];
-    constexpr int kPer = (kMaxExperts + threads_of(kTma) - 1) / threads_of(kTma);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int mine[kPer], sum = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int g = int(threadIdx.x) * kPer + i;
-        int count = 0, begin;
-        if (g < p.groups) group_rows(p, g, &begin, &count);
-        const int c = count > 0 ? even_cols(count, t) : 1;
-        mine[i] = int(min((long long)((count + c - 1) / c) * t.n_tiles, (long long)kMaxGroupTiles));
-        sum += mine[i];
+    for (int g = threadIdx.x; g <= p.groups; g += threads) table.bound[g] = min(max(p.offsets[g], 0), p.total);
+    __syncthreads();
+    const int per = (p.groups + threads - 1) / threads, g0 = min(int(threadIdx.x) * per, p.groups), g1 = min(g0 + per, p.groups);
+    int sum = 0;
+    for (int g = g0; g < g1; ++g) {
+        const int n = tiles_of(table.bound[g + 1] - table.bound[g], t);
+        table.first[g] = n;
+        sum += n;
     }
     int run = sum;
 #pragma unroll
@@ -113,29 +126,27 @@ __device__ void build_table(const GroupedParams &p, const MmGeom &t, int *first)
     __syncthreads();
     int start = run - sum;
     for (int w = 0; w < warp; ++w) start += warp_total[w];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int g = int(threadIdx.x) * kPer + i;
-        if (g < p.groups) first[g] = start;
-        start += mine[i];
-        if (g == p.groups - 1) first[p.groups] = start;
+    for (int g = g0; g < g1; ++g) {
+        const int n = table.first[g];
+        table.first[g] = start;
+        start += n;
     }
+    if (g0 < p.groups && g1 == p.groups) table.first[p.groups] = start;
 }
 
 // Tiles of a group: up to 8 column tiles side by side, then the next channels, so that neighbours in the list share
 // weights and rows in L2.
-__device__ __forceinline__ Tile find_tile(const GroupedParams &p, const MmGeom &t, const int *first, int index, int cta_channel) {
-    int lo = 0, hi = p.groups;                    // first[lo] <= index < first[hi]
+__device__ __forceinline__ Tile find_tile(const GroupedParams &p, const MmGeom &t, const Table &table, int index, int cta_channel) {
+    int lo = 0, hi = p.groups;                    // table.first[lo] <= index < table.first[hi]
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (first[mid] <= index) lo = mid;
+        if (table.first[mid] <= index) lo = mid;
         else hi = mid;
     }
-    int begin, count;
-    group_rows(p, lo, &begin, &count);
+    const int begin = table.bound[lo], count = table.bound[lo + 1] - begin;
     const int cols = even_cols(count, t);
     const int col_tiles = (count + cols - 1) / cols;
-    const int at = index - first[lo];
+    const int at = index - table.first[lo];
     const int band = at / (8 * t.n_tiles);
     const int wide = min(8, col_tiles - band * 8);
     const int inside = at - band * 8 * t.n_tiles;
@@ -150,8 +161,9 @@ __device__ __forceinline__ Tile find_tile(const GroupedParams &p, const MmGeom &
 }
 
 // Row of the weights (inside its group) that tile row r holds
+template <bool GATED>
 __device__ __forceinline__ int weight_row(const GroupedParams &p, const Tile &tile, int r) {
-    if (!p.gated) return tile.channel0 + r;
+    if (!GATED) return tile.channel0 + r;
     return ((r >> 4) & 1) * p.channels + tile.channel0 + (r >> 5) * 16 + (r & 15);
 }
 
@@ -324,11 +336,6 @@ __device__ __forceinline__ void activate(float *v, int act) {
     }
 }
 
-template <class T> __device__ __forceinline__ T narrow(float v);
-template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
 // What an epilogue warp needs to write the results of its lanes' channels.
 struct Out {
     uint8_t *turn;              // shared memory of this warp, kTurnBytes
@@ -337,43 +344,56 @@ struct Out {
     int rows, channels;         // valid rows of the tile, valid channels of this warp
     int vectors;                // rows may be written 16 bytes at a time
 };
-
-// v[c] (gated: v[c / 2], the lanes' halves holding alternate columns) are the results of columns c0 .. c0 + 31 of this
-// lane's channel.  The warp turns them round in shared memory and writes whole segments of rows, 64 bytes or more.
-template <class T, bool GATED>
-__device__ __forceinline__ void write_columns(const Out &o, const float *v, int c0, int lane) {
-    constexpr int kWidth = GATED ? 16 : 32;                           // channels of the warp
-    constexpr int kCols = kTurnBytes / (32 * int(sizeof(T)));         // columns per turn
-    constexpr int kPieces = kWidth * int(sizeof(T)) / 16;             // 16-byte pieces of a row
-    T *turn = reinterpret_cast<T *>(o.turn);
+// Rows c0 .. c0 + 15 of the results, from [column][WIDTH channels] in shared memory: whole segments of rows, 32 to 128 bytes.
+template <class T, int WIDTH>
+__device__ __forceinline__ void write_rows(const Out &o, int c0, int lane) {
+    constexpr int kPieces = WIDTH * int(sizeof(T)) / 16;              // 16-byte pieces of a row
+    const int count = min(kTurnCols, o.rows - c0);
+    if (o.vectors) {
+        const int row = lane / kPieces;
+        uint8_t *to = o.first + (c0 + row) * o.row_bytes + (lane % kPieces) * 16;
 #pragma unroll
-    for (int h = 0; h < kStageCols; h += kCols) {
-        if (GATED) {
-#pragma unroll
-            for (int c = 0; c < kCols / 2; ++c) turn[(2 * c + (lane >> 4)) * 16 + (lane & 15)] = narrow<T>(v[h / 2 + c]);
-        } else {
-#pragma unroll
-            for (int c = 0; c < kCols; ++c) turn[c * 32 + lane] = narrow<T>(v[h + c]);
+        for (int q = 0; q < kTurnCols * kPieces / 32; ++q) {
+            if (row + q * (32 / kPieces) < count) *reinterpret_cast<uint4 *>(to) = reinterpret_cast<const uint4 *>(o.turn)[q * 32 + lane];
+            to += (32 / kPieces) * o.row_bytes;
         }
-        __syncwarp();
-        const int count = o.rows - c0 - h;
-        if (o.vectors) {
-            const int row = lane / kPieces;
-            uint8_t *to = o.first + (c0 + h + row) * o.row_bytes + (lane % kPieces) * 16;
-#pragma unroll
-            for (int q = 0; q < kCols * kPieces / 32; ++q) {
-                if (row + q * (32 / kPieces) < count) *reinterpret_cast<uint4 *>(to) = reinterpret_cast<const uint4 *>(turn)[q * 32 + lane];
-                to += (32 / kPieces) * o.row_bytes;
-            }
-        } else {
-            for (int i = lane; i < min(kCols, count) * kWidth; i += 32)
-                if (i % kWidth < o.channels) reinterpret_cast<T *>(o.first + (c0 + h + i / kWidth) * o.row_bytes)[i % kWidth] = turn[i];
-        }
-        __syncwarp();
+    } else {
+        for (int i = lane; i < count * WIDTH; i += 32)
+            if (i % WIDTH < o.channels)
+                reinterpret_cast<T *>(o.first + (c0 + i / WIDTH) * o.row_bytes)[i % WIDTH] = reinterpret_cast<const T *>(o.turn)[i];
     }
 }
+// v[c] (gated: v[c / 2], the lanes' halves holding alternate columns) are the results of columns c0 .. c0 + 15 of this
+// lane's channel.  The warp turns them round in shared memory.
+template <bool GATED>
+__device__ __forceinline__ void write_columns(const Out &o, Elem type, const float *v, int c0, int lane) {
+    constexpr int kWidth = GATED ? 16 : 32;                           // channels of the warp
+    const int at = GATED ? (lane >> 4) * 16 + (lane & 15) : lane;
+    if (type == Elem::F32) {
+#pragma unroll
+        for (int c = 0; c < (GATED ? kTurnCols / 2 : kTurnCols); ++c) reinterpret_cast<float *>(o.turn)[c * 32 + at] = v[c];
+    } else if (type == Elem::BF16) {
+#pragma unroll
+        for (int c = 0; c < (GATED ? kTurnCols / 2 : kTurnCols); ++c) reinterpret_cast<__nv_bfloat16 *>(o.turn)[c * 32 + at] = __float2bfloat16_rn(v[c]);
+    } else {
+#pragma unroll
+        for (int c = 0; c < (GATED ? kTurnCols / 2 : kTurnCols); ++c) reinterpret_cast<__half *>(o.turn)[c * 32 + at] = __float2half_rn(v[c]);
+    }
+    __syncwarp();
+    if (type == Elem::F32) write_rows<float, kWidth>(o, c0, lane);
+    else write_rows<uint16_t, kWidth>(o, c0, lane);
+    __syncwarp();
+}
 
-template <int KIND, int LOADS, bool PAIR>
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float *v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+          "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
+        : "memory");
+}
+
+template <int KIND, int LOADS, bool PAIR, bool GATED>
 __global__ void __launch_bounds__(threads_of(LOADS), 1)
 expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const GroupedParams p,
                  const MmGeom t) {
@@ -391,8 +411,12 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     const uint32_t full0 = base + t.bar_off, empty0 = full0 + 8u * t.stages;
     const uint32_t acc_full0 = empty0 + 8u * t.stages, acc_empty0 = acc_full0 + 16u;
     const uint32_t recv_full = acc_empty0 + 16u, recv_free = recv_full + 8u;
-    int *first = reinterpret_cast<int *>(generic + t.table_off);
+    const Table table = {reinterpret_cast<int *>(generic + t.table_off), reinterpret_cast<int *>(generic + t.table_off) + p.groups + 1};
 
+    if (LOADS != kRegs && threadIdx.x == 32) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < t.stages; ++s) {
             mbar_init(full0 + 8u * s, LOADS == kRegs ? kLoaderWarps : 1);
@@ -417,13 +441,13 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         }
     }
     grid_dependency_entry();
-    build_table(p, t, first);
+    build_table(p, t, table, threads_of(LOADS));
     tc_fence_before();
     __syncthreads();
     if (PAIR || t.cluster > 1) cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    const int total_tiles = first[p.groups];
+    const int total_tiles = table.first[p.groups];
     const int rank = PAIR || t.cluster > 1 ? int(cluster_cta_rank()) : 0;
     const int sharing = PAIR ? 2 : t.cluster;                    // CTAs of a tile
     const int tile0 = int(blockIdx.x) / sharing, tile_step = int(gridDim.x) / sharing;
@@ -449,21 +473,21 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         int armed = 0;
         bool ok = true;
         for (int i = tile0; i < total_tiles && ok; i += tile_step) {
-            const Tile tile = find_tile(p, t, first, i, cta_channel);
+            const Tile tile = find_tile(p, t, table, i, cta_channel);
             const uint32_t bytes = (PAIR ? 2 : 1) * kATileBytes + row_bytes_of(tile, 0) + (PAIR ? row_bytes_of(tile, tile.cols / 2) : 0);
             for (int k = k_begin; k < k_end; ++k) {
                 ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
                 if (!ok) break;
                 const uint32_t dst = base + uint32_t(s) * stage_bytes, bar = full_at + 8u * s;
                 if (!PAIR || rank == 0) expect(elected, full0 + 8u * s, bytes);
-                if (!p.gated) {
+                if (!GATED) {
                     load_3d<PAIR>(elected, dst, &map_w, bar, k * k_elems, tile.channel0, tile.group);
                 } else if (t.one_box) {
                     load_5d<PAIR>(elected, dst, &map_w, bar, k * k_elems, tile.channel0 / 16, tile.group);
                 } else {
 #pragma unroll
                     for (int b = 0; b < 8; ++b)
-                        load_3d<PAIR>(elected, dst + uint32_t(b) * 16u * kRowBytes, &map_w, bar, k * k_elems, weight_row(p, tile, b * 16), tile.group);
+                        load_3d<PAIR>(elected, dst + uint32_t(b) * 16u * kRowBytes, &map_w, bar, k * k_elems, weight_row<GATED>(p, tile, b * 16), tile.group);
                 }
                 ++armed;
                 if (++s == t.stages) { s = 0; phase ^= 1u; }
@@ -481,7 +505,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         uint32_t phase = 1;
         bool ok = true;
         for (int i = tile0; i < total_tiles && ok; i += tile_step) {
-            const Tile tile = find_tile(p, t, first, i, cta_channel);
+            const Tile tile = find_tile(p, t, table, i, cta_channel);
             const int col0 = PAIR ? rank * (tile.cols / 2) : 0;              // a pair's CTAs hold half of the columns each
             const int loads = int(row_bytes_of(tile, col0)) / (t.box_rows * kRowBytes);
             for (int k = k_begin; k < k_end; ++k) {
@@ -503,7 +527,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         uint32_t phase = 1;
         bool ok = true;
         for (int i = tile0; i < total_tiles && ok; i += tile_step) {
-            const Tile tile = find_tile(p, t, first, i, cta_channel);
+            const Tile tile = find_tile(p, t, table, i, cta_channel);
             const int col0 = PAIR ? rank * (tile.cols / 2) : 0;
             const int loads = int(row_bytes_of(tile, col0)) / (4 * kRowBytes);
             int4 src[kMost];
@@ -538,12 +562,12 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         uint32_t phase = 1;
         bool ok = true;
         for (int i = tile0; i < total_tiles && ok; i += tile_step) {
-            const Tile tile = find_tile(p, t, first, i, cta_channel);
-            const int wide = p.gated ? 2 * p.channels : p.channels;
+            const Tile tile = find_tile(p, t, table, i, cta_channel);
+            const int wide = GATED ? 2 * p.channels : p.channels;
             const uint8_t *src[8];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int r = weight_row(p, tile, r0 + 32 * j);
+                const int r = weight_row<GATED>(p, tile, r0 + 32 * j);
                 const uint8_t *w = static_cast<const uint8_t *>(p.w) + ((long long)tile.group * p.w_group_stride + (long long)r * p.w_stride) * t.esize;
                 src[j] = r < wide ? w : nullptr;
                 const int c = r0 + 32 * j;
@@ -602,7 +626,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             bool ok = true;
             const uint32_t a_low0 = desc_low(base), stage_low = stage_bytes >> 4, b_low0 = kPlanes * kATileBytes >> 4;
             for (int i = tile0; i < total_tiles && ok; i += tile_step) {
-                const Tile tile = find_tile(p, t, first, i, cta_channel);
+                const Tile tile = find_tile(p, t, table, i, cta_channel);
                 // sums in float32 / int32 (bit 4 / 5), operand formats, both K-major, N and M
                 const uint32_t idesc = (KIND == kI8 ? 2u << 4 : 1u << 4) | (t.format << 7) | (t.format << 10) |
                                        (uint32_t(tile.cols >> 3) << 17) | (uint32_t((PAIR ? 2 : 1) * kTileM >> 4) << 24);
@@ -653,24 +677,25 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         const uint32_t recv = base + t.recv_off;
         float *recv_generic = reinterpret_cast<float *>(generic + t.recv_off);
         const int out_size = elem_size(p.out_type);
+        constexpr int kWidth = GATED ? 16 : 32;                       // channels of a warp
+        const int half = GATED ? lane >> 4 : 0;
         Out o;
         o.turn = generic + t.turn_off + (warp - 4) * kTurnBytes;
         o.row_bytes = p.y_stride * out_size;
         int turn = 0, round = 0;
         bool ok = true;
+#pragma unroll 1
         for (int i = tile0; i < total_tiles && ok; i += tile_step, ++round) {
-            const Tile tile = find_tile(p, t, first, i, cta_channel);
-            const int half = p.gated ? (lane >> 4) : 0;
-            const int warp_channel = tile.channel0 + quad * (p.gated ? 16 : 32);
-            const int channel = warp_channel + (p.gated ? (lane & 15) : lane);
-            const bool in_channels = channel < p.channels;
-            const long long per_channel = (long long)tile.group * (p.gated ? 2 : 1) * p.channels + (long long)half * p.channels + channel;
-            const float channel_scale = p.channel_scale && in_channels ? p.channel_scale[per_channel] : 1.0f;
-            const float bias = p.bias && in_channels ? p.bias[per_channel] : 0.0f;
+            const Tile tile = find_tile(p, t, table, i, cta_channel);
+            const int warp_channel = tile.channel0 + quad * kWidth;
+            const int channel = warp_channel + lane % kWidth;
+            const long long per_channel = (long long)tile.group * (GATED ? 2 : 1) * p.channels + (long long)half * p.channels + channel;
+            const float channel_scale = p.channel_scale && channel < p.channels ? p.channel_scale[per_channel] : 1.0f;
+            const float bias = p.bias && channel < p.channels ? p.bias[per_channel] : 0.0f;
             o.first = static_cast<uint8_t *>(p.y) + (tile.row0 * p.y_stride + warp_channel) * out_size;
             o.rows = tile.valid;
-            o.channels = max(0, min(p.gated ? 16 : 32, p.channels - warp_channel));
-            o.vectors = ((reinterpret_cast<uintptr_t>(o.first) | uintptr_t(o.row_bytes)) & 15) == 0 && o.channels == (p.gated ? 16 : 32);
+            o.channels = max(0, min(kWidth, p.channels - warp_channel));
+            o.vectors = ((reinterpret_cast<uintptr_t>(o.first) | uintptr_t(o.row_bytes)) & 15) == 0 && o.channels == kWidth;
             const float *row_scale = row_scale_s[round & 1];
             const uint32_t *live = live_s[round & 1];
             if (p.row_scale || LOADS == kGather) {
@@ -683,157 +708,134 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 }
                 asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory");
             }
-            // finished sums of columns c0 .. c0 + 31 (those behind the tile's last are not used): scales, bias, activation, store
-            auto finish = [&](float *v, int c0) {
-                if (c0 >= tile.valid || o.channels == 0) return;
-                if (KIND == kI8) {
-#pragma unroll
-                    for (int c = 0; c < kStageCols; ++c) v[c] = float(__float_as_int(v[c]));
-                }
-                if (LOADS == kGather) {                       // a row that is none was loaded as some other one
-                    const uint32_t mask = __funnelshift_r(live[c0 >> 5], live[min(c0 >> 5, 6) + 1], c0);
-                    if (mask != 0xffffffffu) {
-#pragma unroll
-                        for (int c = 0; c < kStageCols; ++c)
-                            if (!((mask >> c) & 1u)) v[c] = 0.0f;
-                    }
-                }
-                if (p.row_scale) {
-                    if (t.cluster == 1) {                     // c0 is a multiple of 32, t.tn of 16
-#pragma unroll
-                        for (int c = 0; c < kStageCols; c += 4)
-                            if (c0 + c < t.tn) {
-                                const float4 f = *reinterpret_cast<const float4 *>(row_scale + c0 + c);
-                                v[c] *= f.x; v[c + 1] *= f.y; v[c + 2] *= f.z; v[c + 3] *= f.w;
-                            }
-                    } else {                                  // a rank's columns may start at any even one
-#pragma unroll
-                        for (int c = 0; c < kStageCols; ++c)
-                            if (c0 + c < t.tn) v[c] *= row_scale[c0 + c];
-                    }
-                }
-#pragma unroll
-                for (int c = 0; c < kStageCols; ++c) v[c] = v[c] * channel_scale + bias;
-                if (!p.gated) {
-                    activate<kStageCols>(v, p.act);
-                    if (p.out_type == Elem::BF16) write_columns<__nv_bfloat16, false>(o, v, c0, lane);
-                    else if (p.out_type == Elem::F16) write_columns<__half, false>(o, v, c0, lane);
-                    else write_columns<float, false>(o, v, c0, lane);
-                } else {
-                    // the lower half of the warp finishes the even columns, the upper half the odd ones
-                    float up[kStageCols / 2];
-#pragma unroll
-                    for (int c = 0; c < kStageCols / 2; ++c) {
-                        const float other = __shfl_xor_sync(0xffffffffu, half ? v[2 * c] : v[2 * c + 1], 16);
-                        up[c] = half ? v[2 * c + 1] : other;
-                        v[c] = half ? other : v[2 * c];
-                    }
-                    activate<kStageCols / 2>(v, p.act);
-#pragma unroll
-                    for (int c = 0; c < kStageCols / 2; ++c) v[c] *= up[c];
-                    if (p.out_type == Elem::BF16) write_columns<__nv_bfloat16, true>(o, v, c0, lane);
-                    else if (p.out_type == Elem::F16) write_columns<__half, true>(o, v, c0, lane);
-                    else write_columns<float, true>(o, v, c0, lane);
-                }
-            };
-            if (KIND == kX3) {
-                float sum[kLoaderCols];
-#pragma unroll
-                for (int c = 0; c < kLoaderCols; ++c) sum[c] = 0.0f;
+            // ---- the sums of this CTA's K range ----
+            uint32_t sums = lane_tmem + (uint32_t(turn) & 1u) * uint32_t(t.tn), held = acc_empty0 + 8u * (uint32_t(turn) & 1u);
+            if (KIND != kX3) {
+                ok = wait<PAIR>(acc_full0 + 8u * (uint32_t(turn) & 1u), (uint32_t(turn) >> 1) & 1u);
+                ++turn;
+            } else {
+                // added up in tensor memory behind the two accumulators
+                sums = lane_tmem + 2u * uint32_t(t.tn);
                 for (int k = k_begin; k < k_end && ok; k += kChunkSteps, ++turn) {
                     const uint32_t a = uint32_t(turn) & 1u;
-                    ok = mbar_wait(acc_full0 + 8u * a, (uint32_t(turn) >> 1) & 1u, nullptr);
-                    ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
+                    ok = __all_sync(0xffffffffu, wait<PAIR>(acc_full0 + 8u * a, (uint32_t(turn) >> 1) & 1u) ? 1 : 0) != 0;
                     if (!ok) break;
                     tc_fence_after();
+                    for (int c0 = share * 16; c0 < tile.cols; c0 += kShare * 16) {
+                        float v[16], sum[16];
+                        tmem_ld16(lane_tmem + a * uint32_t(t.tn) + c0, v);
+                        if (k != k_begin) {
+                            tmem_ld16(sums + c0, sum);
 #pragma unroll
-                    for (int c0 = 0; c0 < kLoaderCols; c0 += 16)
-                        if (c0 < tile.cols) {
-                            float v[16];
-                            tmem_ld16(lane_tmem + a * uint32_t(t.tn) + c0, v);
-#pragma unroll
-                            for (int c = 0; c < 16; ++c) sum[c0 + c] += v[c];
+                            for (int c = 0; c < 16; ++c) v[c] += sum[c];
                         }
+                        tmem_st16(sums + c0, v);
+                    }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(acc_empty0 + 8u * a);          // (no pairs)
                 }
-                if (!ok) break;
-                if (t.cluster == 1) {
-#pragma unroll
-                    for (int c = 0; c < kLoaderCols; c += kStageCols) finish(sum + c, c);
-                } else {
-                    ok = round == 0 || wait<true>(recv_free, uint32_t(round - 1) & 1u);
-                    ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
-                    if (!ok) break;
-                    const int per = tile.cols / t.cluster;
-#pragma unroll
-                    for (int c = 0; c < kLoaderCols; ++c)
-                        if (c < tile.cols)
-                            store_cluster(cluster_map(recv + uint32_t((rank * per + c % per) * kTileM + lane_row) * 4u, uint32_t(c / per)), sum[c]);
-                }
-            } else {
-                const uint32_t a = uint32_t(turn) & 1u;
-                ok = wait<PAIR>(acc_full0 + 8u * a, (uint32_t(turn) >> 1) & 1u);
-                if (ok && t.cluster > 1 && round > 0) ok = wait<true>(recv_free, uint32_t(round - 1) & 1u);
-                ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
-                if (!ok) break;
-                tc_fence_after();
-                if (t.cluster == 1) {
-                    for (int c0 = share * kStageCols; c0 < tile.valid; c0 += kShare * kStageCols) {
-                        float v[kStageCols];
-                        if (c0 + kStageCols <= t.tn) tmem_ld32(lane_tmem + a * uint32_t(t.tn) + c0, v);
-                        else tmem_ld16(lane_tmem + a * uint32_t(t.tn) + c0, v);
-                        finish(v, c0);
-                    }
-                } else {
-                    const int per = tile.cols / t.cluster;
-                    for (int c0 = share * 16; c0 < tile.cols; c0 += kShare * 16) {
-                        float v[16];
-                        tmem_ld16(lane_tmem + a * uint32_t(t.tn) + c0, v);
-#pragma unroll
-                        for (int c = 0; c < 16; ++c) {
-                            const int d = (c0 + c) / per;
-                            store_cluster(cluster_map(recv + uint32_t((rank * per + c0 + c - d * per) * kTileM + lane_row) * 4u, uint32_t(d)), v[c]);
-                        }
-                    }
-                }
+            }
+            if (ok && t.cluster > 1 && round > 0) ok = wait<true>(recv_free, uint32_t(round - 1) & 1u);
+            ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
+            if (!ok) break;
+            tc_fence_after();
+            const auto release = [&]() {                              // the accumulator may be written again
+                if (KIND == kX3) return;
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    if (PAIR) mbar_arrive_cluster(cluster_map(acc_empty0 + 8u * a, 0));
-                    else mbar_arrive(acc_empty0 + 8u * a);
+                    if (PAIR) mbar_arrive_cluster(cluster_map(held, 0));
+                    else mbar_arrive(held);
                 }
-                ++turn;
-            }
+            };
+            int from = share * kTurnCols, step = kShare * kTurnCols;
+            const int per = tile.cols / t.cluster;                    // columns that each CTA finishes
             if (t.cluster > 1) {
-                // this CTA's columns: the partial sums of all ranks, added in rank order
-                const int per = tile.cols / t.cluster;
+                for (int c0 = share * 16; c0 < tile.cols; c0 += kShare * 16) {
+                    float v[16];
+                    tmem_ld16(sums + c0, v);
+                    int d = c0 / per, at = c0 - d * per;
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        store_cluster(cluster_map(recv + uint32_t((rank * per + at) * kTileM + lane_row) * 4u, uint32_t(d)), v[c]);
+                        if (++at == per) { at = 0; ++d; }
+                    }
+                }
+                release();
                 __syncwarp();
                 if (lane < t.cluster) mbar_arrive_cluster(cluster_map(recv_full, uint32_t(lane)));
-                ok = wait<true>(recv_full, uint32_t(round) & 1u);
-                ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
+                ok = __all_sync(0xffffffffu, wait<true>(recv_full, uint32_t(round) & 1u) ? 1 : 0) != 0;
                 if (!ok) break;
-                // (pairs of columns: a gated result takes two lanes' columns at once)
+                // pairs of columns: a gated result takes two lanes' columns at once
                 const int mine = kShare == 1 ? per : (per / 2 + 1) / 2 * 2;          // columns of the first warp of a quarter
-                const int from = share * mine, to = share == 0 ? mine : per;
-                o.rows = min(tile.valid, rank * per + to);
-                for (int c0 = from; c0 < to; c0 += kStageCols) {
-                    float v[kStageCols];
+                from = rank * per + share * mine;
+                step = kTurnCols;
+                o.rows = min(tile.valid, rank * per + (share == 0 ? mine : per));
+            }
+            // ---- scales, bias, activation, store: 16 columns at a time (those behind the last are not used) ----
+#pragma unroll 1
+            for (int c0 = from; c0 < o.rows; c0 += step) {
+                float v[kTurnCols];
+                if (t.cluster == 1) {
+                    tmem_ld16(sums + c0, v);
+                } else {
+                    // the partial sums of all ranks, in rank order
+                    const float *part = recv_generic + (c0 - rank * per) * kTileM + lane_row;
+                    const int count = o.rows - c0;
 #pragma unroll
-                    for (int c = 0; c < kStageCols; ++c) {
-                        float f = 0.0f;
-                        int n = 0;
-                        if (c0 + c < to)
-                            for (int q = 0; q < t.cluster; ++q) {
-                                const float part = recv_generic[(q * per + c0 + c) * kTileM + lane_row];
-                                if (KIND == kI8) n += __float_as_int(part);
-                                else f += part;
-                            }
-                        v[c] = KIND == kI8 ? __int_as_float(n) : f;
+                    for (int c = 0; c < kTurnCols; ++c) v[c] = c < count ? part[c * kTileM] : 0.0f;
+#pragma unroll 1
+                    for (int q = 1; q < t.cluster; ++q) {
+                        part += per * kTileM;
+#pragma unroll
+                        for (int c = 0; c < kTurnCols; ++c) {
+                            const float more = c < count ? part[c * kTileM] : 0.0f;
+                            v[c] = KIND == kI8 ? __int_as_float(__float_as_int(v[c]) + __float_as_int(more)) : v[c] + more;
+                        }
                     }
-                    finish(v, rank * per + c0);
                 }
+                if (o.channels == 0) continue;
+                if (KIND == kI8) {
+#pragma unroll
+                    for (int c = 0; c < kTurnCols; ++c) v[c] = float(__float_as_int(v[c]));
+                }
+                if (LOADS == kGather) {                               // a row that is none was loaded as some other one
+                    const uint32_t mask = __funnelshift_r(live[c0 >> 5], live[min(c0 >> 5, 6) + 1], c0);
+                    if ((mask & 0xffffu) != 0xffffu) {
+#pragma unroll
+                        for (int c = 0; c < kTurnCols; ++c)
+                            if (!((mask >> c) & 1u)) v[c] = 0.0f;
+                    }
+                }
+                if (p.row_scale) {
+#pragma unroll
+                    for (int c = 0; c < kTurnCols; ++c)
+                        if (c0 + c < t.tn) v[c] *= row_scale[c0 + c];
+                }
+#pragma unroll
+                for (int c = 0; c < kTurnCols; ++c) v[c] = v[c] * channel_scale + bias;
+                if (!GATED) {
+                    activate<kTurnCols>(v, p.act);
+                } else {
+                    // the lower half of the warp finishes the even columns, the upper half the odd ones
+                    float up[kTurnCols / 2];
+#pragma unroll
+                    for (int c = 0; c < kTurnCols / 2; ++c) {
+                        const float other = __shfl_xor_sync(0xffffffffu, half ? v[2 * c] : v[2 * c + 1], 16);
+                        up[c] = half ? v[2 * c + 1] : other;
+                        v[c] = half ? other : v[2 * c];
+                    }
+                    activate<kTurnCols / 2>(v, p.act);
+#pragma unroll
+                    for (int c = 0; c < kTurnCols / 2; ++c) v[c] *= up[c];
+                }
+                write_columns<GATED>(o, p.out_type, v, c0, lane);
+            }
+            if (t.cluster == 1) {
+                release();
+            } else {
                 __syncwarp();
                 if (lane < t.cluster) mbar_arrive_cluster(cluster_map(recv_free, uint32_t(lane)));
             }
@@ -950,11 +952,11 @@ int choose(const GroupedParams &p, int sm_count, bool tma, MmGeom *t, bool *pair
     }
     t->one_box = p.gated && p.channels % 16 == 0;
     t->box_rows = std::min(*pair ? t->tn / 2 : t->tn, 64);
-    t->tmem_cols = std::max(32, 2 * t->tn);
+    t->tmem_cols = std::max(32, (p.type == Elem::F32 ? 4 : 2) * t->tn);      // two accumulators; float32: and their sum (a power of two)
     const int planes = p.type == Elem::F32 ? 2 : 1;
     const size_t stage = size_t(planes) * (kATileBytes + (*pair ? t->tn / 2 : t->tn) * kRowBytes);
     const size_t recv = t->cluster > 1 ? size_t(t->tn) * kTileM * sizeof(float) : 0;
-    const size_t table = (size_t(p.groups + 1) * sizeof(int) + 15) / 16 * 16;
+    const size_t table = (2 * size_t(p.groups + 1) * sizeof(int) + 15) / 16 * 16;
     const size_t turn = 8 * kTurnBytes;
     const size_t fixed = 1024 + recv + turn + table + kBarBytes + 4096;       // 4096: the kernel's static shared memory
     t->stages = int(std::min<size_t>(kMaxStages, (kSmemLimit - fixed) / stage));
@@ -967,10 +969,10 @@ int choose(const GroupedParams &p, int sm_count, bool tma, MmGeom *t, bool *pair
     return int(std::min<long long>(sm_count / sharing, most)) * sharing;
 }
 
-template <int KIND, int LOADS, bool PAIR>
+template <int KIND, int LOADS, bool PAIR, bool GATED>
 cudaError_t run(const GroupedParams &p, const MmGeom &t, int ctas, const CUtensorMap &map_w, const CUtensorMap &map_x, cudaStream_t stream) {
     const int smem = t.bar_off + kBarBytes + 1024;
-    const auto kernel = expert_mm_kernel<KIND, LOADS, PAIR>;
+    const auto kernel = expert_mm_kernel<KIND, LOADS, PAIR, GATED>;
     cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (err != cudaSuccess) return err;
     cudaLaunchConfig_t config = {};
@@ -1015,16 +1017,23 @@ cudaError_t launch_grouped(const GroupedParams &given, cudaStream_t stream) {
             ctas = choose(p, sm_count, tma, &t, &pair);
         }
     }
-    const auto launch = [&](auto kernel) { return kernel(p, t, ctas, map_w, map_x, stream); };
-    if (p.type == Elem::F32) return launch(run<kX3, kRegs, false>);
+#define IOS_RUN(KIND, LOADS, PAIR)                                                                     \
+    return p.gated ? run<KIND, LOADS, PAIR, true>(p, t, ctas, map_w, map_x, stream)                      \
+                   : run<KIND, LOADS, PAIR, false>(p, t, ctas, map_w, map_x, stream)
+    if (p.type == Elem::F32) IOS_RUN(kX3, kRegs, false);
     if (p.type == Elem::S8) {
-        if (!tma) return launch(run<kI8, kRegs, false>);
-        if (pair) return p.rows ? launch(run<kI8, kGather, true>) : launch(run<kI8, kTma, true>);
-        return p.rows ? launch(run<kI8, kGather, false>) : launch(run<kI8, kTma, false>);
+        if (!tma) IOS_RUN(kI8, kRegs, false);
+        if (pair && p.rows) IOS_RUN(kI8, kGather, true);
+        if (pair) IOS_RUN(kI8, kTma, true);
+        if (p.rows) IOS_RUN(kI8, kGather, false);
+        IOS_RUN(kI8, kTma, false);
     }
-    if (!tma) return launch(run<kF16, kRegs, false>);
-    if (pair) return p.rows ? launch(run<kF16, kGather, true>) : launch(run<kF16, kTma, true>);
-    return p.rows ? launch(run<kF16, kGather, false>) : launch(run<kF16, kTma, false>);
+    if (!tma) IOS_RUN(kF16, kRegs, false);
+    if (pair && p.rows) IOS_RUN(kF16, kGather, true);
+    if (pair) IOS_RUN(kF16, kTma, true);
+    if (p.rows) IOS_RUN(kF16, kGather, false);
+    IOS_RUN(kF16, kTma, false);
+#undef IOS_RUN
 }
 
 cudaError_t expert_mm_status(cudaStream_t stream, int *code) {
