@@ -38,10 +38,12 @@ namespace {
 enum Kind { kF16 = 0, kI8 = 1, kX3 = 2 };       // instruction: 16-bit floats, 8-bit integers, three TF32 products
 enum Loads { kTma = 0, kGather = 1, kRegs = 2 };  // operands by TMA / gathered rows by cp.async warps / all through registers
 
-constexpr int kGatherWarps = 4, kLoaderWarps = 8;
+constexpr int kGatherWarps = 8, kLoaderWarps = 8;
+constexpr int kBoxRows = 64;                    // rows of x per TMA load, in wide tiles
+constexpr int kNarrowCols = 32;                 // tiles up to here gather a step's rows with one warp
 constexpr int kMaxThreads = 512;
-// Two epilogue warps per lane quarter share a tile's columns; one beside the loader warps, which need the registers.
-__host__ __device__ constexpr int epilogue_warps(int loads) { return loads == kRegs ? 4 : 8; }
+// Two epilogue warps per lane quarter share a tile's columns; one beside gathering or loader warps, which need the registers.
+__host__ __device__ constexpr int epilogue_warps(int loads) { return loads != kTma ? 4 : 8; }
 __host__ __device__ constexpr int threads_of(int loads) {
     return 32 * (4 + epilogue_warps(loads) + (loads == kTma ? 0 : loads == kGather ? kGatherWarps : kLoaderWarps));
 }
@@ -239,13 +241,17 @@ __device__ __forceinline__ void umma(uint32_t elected, uint32_t tmem_d, uint32_t
 #undef IOS_UMMA
 // arrives at `bar` (of both CTAs of a pair) once the instructions issued so far have finished
 template <bool PAIR>
-__device__ __forceinline__ void commit(uint32_t bar) {
+__device__ __forceinline__ void commit(uint32_t elected, uint32_t bar) {
     if (PAIR)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                     ::"r"(bar), "h"(uint16_t(3))
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t"
+                     "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%1], %2;\n\t}"
+                     ::"r"(elected), "r"(bar), "h"(uint16_t(3))
                      : "memory");
     else
-        umma_commit(bar);
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t"
+                     "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}"
+                     ::"r"(elected), "r"(bar)
+                     : "memory");
 }
 // mbar_wait for a barrier that other CTAs of the cluster may arrive at
 template <bool CLUSTER>
@@ -461,7 +467,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     // brings some, also where the tile needs none: otherwise the ring of stages could run on without it, and a wait by
     // parity does not notice two rounds.
     const auto row_bytes_of = [&](const Tile &tile, int col0) {
-        const int unit = LOADS == kGather ? 4 : t.box_rows, least = LOADS == kGather ? 4 * kGatherWarps : 1;
+        const int unit = LOADS == kGather ? 4 : t.box_rows, least = LOADS == kGather && t.tn > kNarrowCols ? 4 * kGatherWarps : 1;
         const int rows = max(least, min(PAIR ? tile.cols / 2 : tile.cols, tile.valid - col0));
         return uint32_t((rows + unit - 1) / unit * unit) * kRowBytes;
     };
@@ -500,6 +506,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         }
     } else if (LOADS == kTma && warp == 3) {
         // ---------------- rows ----------------
+        constexpr int kBoxes = (PAIR ? 128 : 256) / kBoxRows;
         const uint32_t elected = elect();
         int s = 0;
         uint32_t phase = 1;
@@ -512,43 +519,43 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
                 if (!ok) break;
                 const uint32_t dst = base + uint32_t(s) * stage_bytes + kATileBytes, bar = full_at + 8u * s;
-                for (int b = 0; b < loads; ++b)
-                    load_2d<PAIR>(elected, dst + uint32_t(b * t.box_rows) * kRowBytes, &map_x, bar, k * k_elems, tile.row0 + col0 + b * t.box_rows);
+#pragma unroll
+                for (int b = 0; b < kBoxes; ++b)                     // (predicated: a branch would cost more than the load)
+                    load_2d<PAIR>(b < loads ? elected : 0u, dst + uint32_t(b * t.box_rows) * kRowBytes, &map_x, bar, k * k_elems, tile.row0 + col0 + b * t.box_rows);
                 if (++s == t.stages) { s = 0; phase ^= 1u; }
             }
         }
         if (!ok && lane == 0) time_out(2);
     } else if (LOADS == kGather && warp >= kLoadWarp0) {
-        // ---------------- gathered rows: every fourth group of four to each of four warps ----------------
-        constexpr int kMost = (PAIR ? 128 : 256) / (4 * kGatherWarps);
-        const uint32_t elected = elect();
+        // ---------------- gathered rows, in groups of four: a group per lane ----------------
+        // Wide tiles: the groups of every step are dealt to all warps.  Narrow tiles, a few groups per step: every warp loads
+        // all groups of its turn's steps.
         const int part = warp - kLoadWarp0;
-        int s = 0;
+        const bool narrow = t.tn <= kNarrowCols;
+        const int group = narrow ? lane : lane * kGatherWarps + part;
+        int s = 0, step = 0;
         uint32_t phase = 1;
         bool ok = true;
         for (int i = tile0; i < total_tiles && ok; i += tile_step) {
             const Tile tile = find_tile(p, t, table, i, cta_channel);
             const int col0 = PAIR ? rank * (tile.cols / 2) : 0;
-            const int loads = int(row_bytes_of(tile, col0)) / (4 * kRowBytes);
-            int4 src[kMost];
+            const bool loads = group < int(row_bytes_of(tile, col0)) / (4 * kRowBytes);
+            int at[4];
 #pragma unroll
-            for (int j = 0; j < kMost; ++j) {
-                int at[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int r = p.rows[tile.row0 + min(col0 + (j * kGatherWarps + part) * 4 + q, tile.valid - 1)];
-                    at[q] = r >= 0 && r < p.x_rows ? r : 0;           // the epilogue makes zeros of a row that is none
-                }
-                src[j] = make_int4(at[0], at[1], at[2], at[3]);
+            for (int q = 0; q < 4; ++q) {
+                const int r = p.rows[tile.row0 + min(col0 + group * 4 + q, tile.valid - 1)];
+                at[q] = r >= 0 && r < p.x_rows ? r : 0;               // the epilogue makes zeros of a row that is none
             }
-            for (int k = k_begin; k < k_end; ++k) {
-                ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
-                if (!ok) break;
-                const uint32_t dst = base + uint32_t(s) * stage_bytes + kATileBytes, bar = full_at + 8u * s;
-#pragma unroll
-                for (int j = 0; j < kMost; ++j)
-                    if (j * kGatherWarps + part < loads)
-                        load_rows4<PAIR>(elected, dst + uint32_t(j * kGatherWarps + part) * 4u * kRowBytes, &map_x, bar, k * k_elems, src[j]);
+            const int4 src = make_int4(at[0], at[1], at[2], at[3]);
+            for (int k = k_begin; k < k_end; ++k, ++step) {
+                if (!narrow || (step & (kGatherWarps - 1)) == part) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
+                    if (!ok) break;
+                    if (loads)
+                        load_rows4<PAIR>(1u, base + uint32_t(s) * stage_bytes + kATileBytes + uint32_t(group) * 4u * kRowBytes, &map_x,
+                                         full_at + 8u * s, k * k_elems, src);
+                    __syncwarp();
+                }
                 if (++s == t.stages) { s = 0; phase ^= 1u; }
             }
         }
@@ -657,12 +664,9 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                         }
                         acc = 1;
                     }
-                    if (elected) {
-                        commit<PAIR>(empty0 + 8u * s);
-                        if (closes) commit<PAIR>(acc_full0 + 8u * a);
-                    }
-                    __syncwarp();
-                    if (closes) ++turn;
+                    commit<PAIR>(elected, empty0 + 8u * s);
+                    commit<PAIR>(closes ? elected : 0u, acc_full0 + 8u * a);
+                    turn += closes ? 1 : 0;
                     if (++s == t.stages) { s = 0; phase ^= 1u; }
                 }
             }
@@ -951,7 +955,7 @@ int choose(const GroupedParams &p, int sm_count, bool tma, MmGeom *t, bool *pair
         t->n_tiles = ceil_div(p.channels, t->tile_channels);
     }
     t->one_box = p.gated && p.channels % 16 == 0;
-    t->box_rows = std::min(*pair ? t->tn / 2 : t->tn, 64);
+    t->box_rows = std::min(*pair ? t->tn / 2 : t->tn, kBoxRows);
     t->tmem_cols = std::max(32, (p.type == Elem::F32 ? 4 : 2) * t->tn);      // two accumulators; float32: and their sum (a power of two)
     const int planes = p.type == Elem::F32 ? 2 : 1;
     const size_t stage = size_t(planes) * (kATileBytes + (*pair ? t->tn / 2 : t->tn) * kRowBytes);
