@@ -254,7 +254,7 @@ IOS_API int ios_device_ops_status(int device, void *cuda_stream);
  * type: IOS_F32 / IOS_F16 / IOS_BF16; experts <= 1024, k <= 32 and k <= experts.  workspace: at least the bytes that
  * ios_route_experts_workspace names (0 for small calls, then NULL is fine), 4-byte aligned, contents irrelevant; it
  * must not be shared by calls that overlap. */
-IOS_API int ios_route_experts_workspace(int tokens, int experts, size_t *bytes);
+IOS_API int ios_route_experts_workspace(int tokens, int experts, int k, size_t *bytes);
 IOS_API int ios_route_experts(const void *logits, int type, int tokens, int experts, long long stride, int k,
                               int renormalize, int *chosen, float *gates, int *offsets, int *rows, int *slots,
                               void *workspace, size_t workspace_bytes, void *cuda_stream);

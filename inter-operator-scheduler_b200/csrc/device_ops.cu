@@ -115,10 +115,10 @@ int run_grouped(const GroupedParams &p, const char *what, void *stream) {
 
 using namespace ios;
 
-extern "C" int ios_route_experts_workspace(int tokens, int experts, size_t *bytes) {
-    if (!bytes || tokens < 0 || experts <= 0 || experts > kMaxExperts)
-        return fail(IOS_ERR_ARGUMENT, "route_experts_workspace: bytes must not be NULL, tokens >= 0, experts in 1..%d", kMaxExperts);
-    *bytes = tokens == 0 ? 0 : route_workspace_bytes(tokens, experts);
+extern "C" int ios_route_experts_workspace(int tokens, int experts, int k, size_t *bytes) {
+    if (!bytes || tokens < 0 || experts <= 0 || experts > kMaxExperts || k <= 0 || k > kMaxChosen)
+        return fail(IOS_ERR_ARGUMENT, "route_experts_workspace: bytes must not be NULL, tokens >= 0, experts in 1..%d, k in 1..%d", kMaxExperts, kMaxChosen);
+    *bytes = tokens == 0 ? 0 : route_workspace_bytes(tokens, experts, k);
     record_error("");
     return IOS_OK;
 }
@@ -134,7 +134,7 @@ extern "C" int ios_route_experts(const void *logits, int type, int tokens, int e
     if ((long long)tokens * k > INT_MAX) return fail(IOS_ERR_LIMIT, "route_experts: more than 2^31 - 1 pairs");
     if (!offsets || (tokens > 0 && (!logits || !chosen || !gates || !rows || !slots)))
         return fail(IOS_ERR_ARGUMENT, "route_experts: logits and the outputs must not be NULL");
-    const size_t need = tokens == 0 ? 0 : route_workspace_bytes(tokens, experts);
+    const size_t need = tokens == 0 ? 0 : route_workspace_bytes(tokens, experts, k);
     if (workspace_bytes < need || (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 3))))
         return fail(IOS_ERR_ARGUMENT, "route_experts: needs %zu bytes of 4-byte aligned workspace", need);
     DeviceScope scope;
@@ -228,6 +228,7 @@ extern "C" int ios_quantize_rows(const void *x, int type, long long x_rows, long
     if (!float_type(type)) return fail(IOS_ERR_ARGUMENT, "quantize_rows: x must be float32, float16 or bfloat16");
     if (inner <= 0 || x_rows < 0 || total_rows < 0 || x_stride < 0 || q_stride < inner)
         return fail(IOS_ERR_ARGUMENT, "quantize_rows: inner > 0, row counts >= 0, x_stride >= 0, q_stride >= inner are needed");
+    if (total_rows > INT_MAX) return fail(IOS_ERR_LIMIT, "quantize_rows: more than 2^31 - 1 rows");
     if (!rows && x_rows < total_rows) return fail(IOS_ERR_ARGUMENT, "quantize_rows: x has %lld rows, q %lld", x_rows, total_rows);
     if (total_rows == 0) {
         record_error("");
@@ -260,6 +261,7 @@ extern "C" int ios_combine_experts(const void *y, int type, long long y_rows, lo
         return fail(IOS_ERR_ARGUMENT, "combine_experts: y and out must be float32, float16 or bfloat16");
     if (k <= 0 || channels <= 0 || tokens < 0 || y_rows < 0 || y_stride < 0 || out_stride < channels)
         return fail(IOS_ERR_ARGUMENT, "combine_experts: k, channels > 0, tokens, y_rows, y_stride >= 0, out_stride >= channels are needed");
+    if (tokens > INT_MAX || channels > 1 << 23) return fail(IOS_ERR_LIMIT, "combine_experts: at most 2^31 - 1 tokens of 2^23 channels");
     if (tokens == 0) {
         record_error("");
         return IOS_OK;

@@ -30,6 +30,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 namespace ios {
@@ -55,7 +56,7 @@ constexpr int kChunkSteps = 4;                  // float32: K steps per partial 
 constexpr int kMaxStages = 12;
 constexpr int kMaxGroupTiles = INT_MAX / kMaxExperts - 1;    // tiles of a group: their sum over all groups fits an int
 constexpr int kBarBytes = 2 * kMaxStages * 8 + 48;    // mbarriers: two per stage, six more
-constexpr size_t kSmemLimit = 227 * 1024;
+constexpr size_t kSmemLimit = 227 * 1024, kStaticBytes = 4096;    // ... of which the kernel's static arrays may take
 
 __device__ int g_expert_error;                  // set by a wait that ran out, read by expert_mm_status
 
@@ -446,12 +447,14 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             tmem_relinquish();
         }
     }
-    grid_dependency_entry();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     build_table(p, t, table, threads_of(LOADS));
     tc_fence_before();
     __syncthreads();
     if (PAIR || t.cluster > 1) cluster_sync_all();
     tc_fence_after();
+    // (only now: a successor that were to share this SM must find the tensor memory taken, not take it)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = tmem_slot;
     const int total_tiles = table.first[p.groups];
     const int rank = PAIR || t.cluster > 1 ? int(cluster_cta_rank()) : 0;
@@ -962,7 +965,7 @@ int choose(const GroupedParams &p, int sm_count, bool tma, MmGeom *t, bool *pair
     const size_t recv = t->cluster > 1 ? size_t(t->tn) * kTileM * sizeof(float) : 0;
     const size_t table = (2 * size_t(p.groups + 1) * sizeof(int) + 15) / 16 * 16;
     const size_t turn = 8 * kTurnBytes;
-    const size_t fixed = 1024 + recv + turn + table + kBarBytes + 4096;       // 4096: the kernel's static shared memory
+    const size_t fixed = 1024 + recv + turn + table + kBarBytes + kStaticBytes;
     t->stages = int(std::min<size_t>(kMaxStages, (kSmemLimit - fixed) / stage));
     t->recv_off = int(t->stages * stage);
     t->turn_off = int(t->recv_off + recv);
@@ -975,22 +978,44 @@ int choose(const GroupedParams &p, int sm_count, bool tma, MmGeom *t, bool *pair
 
 template <int KIND, int LOADS, bool PAIR, bool GATED>
 cudaError_t run(const GroupedParams &p, const MmGeom &t, int ctas, const CUtensorMap &map_w, const CUtensorMap &map_x, cudaStream_t stream) {
-    const int smem = t.bar_off + kBarBytes + 1024;
     const auto kernel = expert_mm_kernel<KIND, LOADS, PAIR, GATED>;
-    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<uint64_t> prepared{0};                // devices (of the first 64) that know the kernel's shared memory
+    int device = 0;
+    cudaError_t err = cudaGetDevice(&device);
     if (err != cudaSuccess) return err;
+    const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+    if (!(prepared.load(std::memory_order_relaxed) & bit)) {
+        err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemLimit - kStaticBytes));
+        if (err != cudaSuccess) return err;
+        prepared.fetch_or(bit, std::memory_order_relaxed);
+    }
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(unsigned(ctas));
     config.blockDim = dim3(threads_of(LOADS));
-    config.dynamicSmemBytes = size_t(smem);
+    config.dynamicSmemBytes = size_t(t.bar_off + kBarBytes + 1024);
     config.stream = stream;
-    cudaLaunchAttribute attribute = {};
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = unsigned(PAIR ? 2 : t.cluster);
-    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-    config.attrs = &attribute;
-    config.numAttrs = 1;
+    cudaLaunchAttribute attributes[2] = {};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // the set-up overlaps the end of the kernel before
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = unsigned(PAIR ? 2 : t.cluster);
+    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = 2;
     return cudaLaunchKernelEx(&config, kernel, map_w, map_x, p, t);
+}
+
+// SMs of the current device, asked once per device
+cudaError_t sm_count_of_current(int *count) {
+    static std::atomic<int> known[64];
+    int device = 0;
+    cudaError_t err = cudaGetDevice(&device);
+    if (err != cudaSuccess) return err;
+    *count = device < 64 ? known[device].load(std::memory_order_relaxed) : 0;
+    if (*count > 0) return cudaSuccess;
+    err = cudaDeviceGetAttribute(count, cudaDevAttrMultiProcessorCount, device);
+    if (err == cudaSuccess && device < 64) known[device].store(*count, std::memory_order_relaxed);
+    return err;
 }
 
 }  // namespace
@@ -1000,9 +1025,8 @@ bool grouped_too_large(const GroupedParams &p) {
 }
 
 cudaError_t launch_grouped(const GroupedParams &given, cudaStream_t stream) {
-    int device = 0, sm_count = 0;
-    cudaError_t err = cudaGetDevice(&device);
-    if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, device);
+    int sm_count = 0;
+    cudaError_t err = sm_count_of_current(&sm_count);
     if (err != cudaSuccess) return err;
     GroupedParams p = given;
     const int wide = p.gated ? 2 * p.channels : p.channels;

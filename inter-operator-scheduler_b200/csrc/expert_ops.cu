@@ -2,12 +2,12 @@
 // gate-weighted sum of expert rows.  Their counterparts among the convolution network's operators are in
 // bandwidth_ops.cu; the products are in expert_mm.cu.
 #include "expert_ops.h"
+#include "kernels.h"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
-#include <climits>
 
 namespace ios {
 namespace {
@@ -20,6 +20,72 @@ template <class T> __device__ __forceinline__ T from_float(float v);
 template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// one 16-byte access, or a single element
+__device__ __forceinline__ void load_vector(const float *p, float (&v)[4]) {
+    const float4 f = *reinterpret_cast<const float4 *>(p);
+    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+}
+__device__ __forceinline__ void load_vector(const __half *p, float (&v)[8]) {
+    const uint4 raw = *reinterpret_cast<const uint4 *>(p);
+    const __half2 *h = reinterpret_cast<const __half2 *>(&raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(h[i]);
+        v[2 * i] = f.x; v[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void load_vector(const __nv_bfloat16 *p, float (&v)[8]) {
+    const uint4 raw = *reinterpret_cast<const uint4 *>(p);
+    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __bfloat1622float2(h[i]);
+        v[2 * i] = f.x; v[2 * i + 1] = f.y;
+    }
+}
+template <class T>
+__device__ __forceinline__ void load_vector(const T *p, float (&v)[1]) { v[0] = to_float(*p); }
+template <class T>
+__device__ __forceinline__ void load8(const T *p, float (&v)[8]) { load_vector(p, v); }
+__device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
+    load_vector(p, *reinterpret_cast<float (*)[4]>(&v[0]));
+    load_vector(p + 4, *reinterpret_cast<float (*)[4]>(&v[4]));
+}
+template <class O, int V>
+__device__ __forceinline__ void store_vector(O *p, const float (&v)[V]) {
+    constexpr int kBytes = V * int(sizeof(O)), kPiece = kBytes < 16 ? kBytes : 16, kPer = kPiece / int(sizeof(O));
+    alignas(16) O out[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = from_float<O>(v[i]);
+#pragma unroll
+    for (int i = 0; i < V; i += kPer) {
+        if (kPiece == 16) *reinterpret_cast<uint4 *>(p + i) = *reinterpret_cast<const uint4 *>(out + i);
+        else if (kPiece == 8) *reinterpret_cast<uint2 *>(p + i) = *reinterpret_cast<const uint2 *>(out + i);
+        else p[i] = out[i];
+    }
+}
+
+// Launches with programmatic dependency: the kernels wait for their predecessors by themselves (grid_dependency_entry),
+// so a block's start-up overlaps the end of the kernel before.
+template <class... Params, class... Args>
+cudaError_t launch(void (*kernel)(Params...), dim3 grid, int block, size_t smem, cudaStream_t stream, const Args &...args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(unsigned(block));
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attribute = {};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, Params(args)...);
+}
+template <class... Params, class... Args>
+cudaError_t launch(void (*kernel)(Params...), long long blocks, int block, size_t smem, cudaStream_t stream, const Args &...args) {
+    return launch(kernel, dim3(unsigned(blocks)), block, smem, stream, args...);
+}
 
 // ---- router ------------------------------------------------------------------------------------
 
@@ -37,15 +103,15 @@ __device__ __forceinline__ float key_logit(uint32_t key) {
 // exp(v - top), with +inf logits sharing the weight among themselves instead of producing NaN
 __device__ __forceinline__ float softmax_term(float v, float top) { return v == top ? 1.0f : expf(v - top); }
 
-constexpr int kRouteThreads = 512;
-constexpr int kRouteWarps = kRouteThreads / 32;
+constexpr int kRouteThreads = 1024;       // 32 warps hide one another's reductions; a call of a few tokens takes 256 threads
+constexpr int kRoutePairs = 8192;         // pairs that a block plans in shared memory
 
 // The k best experts of tokens [first, last): one warp per token, logit e in register e / 32 of lane e % 32.
 // Each pick takes two warp reductions (largest key, then its lowest index) and drops the winner.
 template <class T, int PER>
-__device__ __forceinline__ void pick_experts(const RouteParams &p, int first, int last) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int t = first + warp; t < last; t += kRouteWarps) {
+__device__ __forceinline__ void pick_experts(const RouteParams &p, int first, int last, int *chosen) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    for (int t = first + warp; t < last; t += warps) {
         const T *row = static_cast<const T *>(p.logits) + (long long)t * p.stride;
         uint32_t key[PER];
 #pragma unroll
@@ -95,16 +161,19 @@ __device__ __forceinline__ void pick_experts(const RouteParams &p, int first, in
         if (lane < p.k) {
             p.chosen[(long long)t * p.k + lane] = my_expert;
             p.gates[(long long)t * p.k + lane] = my_expert >= 0 ? my_weight / sum : 0.0f;
+            chosen[(t - first) * p.k + lane] = my_expert;
         }
     }
 }
 
-// Exclusive prefix sums of count[0 .. n) (n <= 2 * kRouteThreads) in place; returns the total.  All threads call it.
+// Exclusive prefix sums of count[0 .. n) in place; returns the total.  All threads call it.
 __device__ int exclusive_scan(int *count, int n) {
-    __shared__ int warp_total[kRouteWarps];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e = 2 * threadIdx.x;
-    const int a = e < n ? count[e] : 0, b = e + 1 < n ? count[e + 1] : 0;
-    int run = a + b;
+    __shared__ int warp_total[kRouteThreads / 32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int per = (n + int(blockDim.x) - 1) / int(blockDim.x), begin = min(int(threadIdx.x) * per, n), end = min(begin + per, n);
+    int sum = 0;
+    for (int e = begin; e < end; ++e) sum += count[e];
+    int run = sum;
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, run, s);
@@ -112,16 +181,16 @@ __device__ int exclusive_scan(int *count, int n) {
     }
     if (lane == 31) warp_total[warp] = run;
     __syncthreads();
-    int before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < kRouteWarps; ++w) {
-        if (w < warp) before += warp_total[w];
+    int start = run - sum, total = 0;
+    for (int w = 0; w < warps; ++w) {
+        if (w < warp) start += warp_total[w];
         total += warp_total[w];
     }
-    const int start = before + run - a - b;
-    __syncthreads();
-    if (e < n) count[e] = start;
-    if (e + 1 < n) count[e + 1] = start + a;
+    for (int e = begin; e < end; ++e) {
+        const int c = count[e];
+        count[e] = start;
+        start += c;
+    }
     __syncthreads();
     return total;
 }
@@ -131,22 +200,25 @@ __device__ int exclusive_scan(int *count, int n) {
 // matching equal experts across its lanes, so nothing depends on timing.
 // kSingle: the grid is one block and the plan is finished here; otherwise slots[] holds ranks inside the block and
 // route_place_kernel adds what lies before it.
+// (16384 tokens, 128 experts, k = 8, bfloat16: bound by the latency of the picks' reductions, not by the 4 MB read.)
 template <class T, int PER, bool kSingle>
 __global__ void __launch_bounds__(kRouteThreads) route_pick_kernel(const RouteParams p, int per_block) {
-    extern __shared__ int counts[];                    // [kRouteWarps][experts], then [experts]
+    extern __shared__ int shared[];                    // [warps][experts] counts, [experts] totals, then chosen and rank of the pairs
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int first = blockIdx.x * per_block, last = min(p.tokens, first + per_block);
-    for (int i = threadIdx.x; i < kRouteWarps * p.experts; i += kRouteThreads) counts[i] = 0;
-    pick_experts<T, PER>(p, first, last);
+    const int pairs = (last - first) * p.k;
+    int *counts = shared, *totals = counts + warps * p.experts, *chosen = totals + p.experts, *rank = chosen + per_block * p.k;
+    for (int i = threadIdx.x; i < warps * p.experts; i += blockDim.x) counts[i] = 0;
+    grid_dependency_entry();
+    pick_experts<T, PER>(p, first, last, chosen);
     __syncthreads();
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long pair0 = (long long)first * p.k;
-    const int pairs = (last - first) * p.k;
-    const int run = (pairs + kRouteWarps * 32 - 1) / (kRouteWarps * 32) * 32;          // pairs per warp
+    const int run = (pairs + warps * 32 - 1) / (warps * 32) * 32;                      // pairs per warp
     const int begin = min(pairs, warp * run), end = min(pairs, begin + run);
     int *mine = counts + warp * p.experts;
     for (int i = begin + lane; i - lane < end; i += 32) {
-        const int e = i < end ? p.chosen[pair0 + i] : -1;
+        const int e = i < end ? chosen[i] : -1;
         const uint32_t same = __match_any_sync(0xffffffffu, e);
         const int before = __popc(same & ((1u << lane) - 1u));
         int base = 0;
@@ -154,14 +226,13 @@ __global__ void __launch_bounds__(kRouteThreads) route_pick_kernel(const RoutePa
         __syncwarp();
         if (e >= 0 && before == 0) mine[e] = base + __popc(same);
         __syncwarp();
-        if (i < end) p.slots[pair0 + i] = e >= 0 ? base + before : -1;
+        if (i < end) rank[i] = base + before;
     }
     __syncthreads();
     // counts per warp -> what lies before each warp; totals of the block behind them
-    int *totals = counts + kRouteWarps * p.experts;
-    for (int e = threadIdx.x; e < p.experts; e += kRouteThreads) {
+    for (int e = threadIdx.x; e < p.experts; e += blockDim.x) {
         int sum = 0;
-        for (int w = 0; w < kRouteWarps; ++w) {
+        for (int w = 0; w < warps; ++w) {
             const int c = counts[w * p.experts + e];
             counts[w * p.experts + e] = sum;
             sum += c;
@@ -173,77 +244,85 @@ __global__ void __launch_bounds__(kRouteThreads) route_pick_kernel(const RoutePa
     int used = 0;
     if (kSingle) {
         used = exclusive_scan(totals, p.experts);
-        for (int e = threadIdx.x; e < p.experts; e += kRouteThreads) p.offsets[e] = totals[e];
+        for (int e = threadIdx.x; e < p.experts; e += blockDim.x) p.offsets[e] = totals[e];
         if (threadIdx.x == 0) p.offsets[p.experts] = used;
     }
     for (int i = begin + lane; i < end; i += 32) {
-        const int e = p.chosen[pair0 + i];
-        if (e < 0) continue;
-        const int slot = p.slots[pair0 + i] + mine[e] + (kSingle ? totals[e] : 0);
+        const int e = chosen[i];
+        const int slot = e < 0 ? -1 : rank[i] + mine[e] + (kSingle ? totals[e] : 0);
         p.slots[pair0 + i] = slot;
-        if (kSingle) p.rows[slot] = first + i / p.k;
+        if (kSingle && e >= 0) p.rows[slot] = first + i / p.k;
     }
     if (kSingle)
-        for (int i = used + int(threadIdx.x); i < pairs; i += kRouteThreads) p.rows[i] = -1;
+        for (int i = used + int(threadIdx.x); i < pairs; i += blockDim.x) p.rows[i] = -1;
 }
 
 // Second pass of a plan over many blocks: block b adds, per expert, the expert's start and the pairs of blocks < b.
+// Every block sums the counts of all blocks; the threads share that by expert and by range of blocks.
 __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteParams p, int per_block, int blocks) {
-    extern __shared__ int counts[];                    // [experts] starts, then [experts] pairs in earlier blocks
-    int *start = counts, *earlier = counts + p.experts;
-    for (int e = threadIdx.x; e < p.experts; e += kRouteThreads) {
+    extern __shared__ int shared[];                    // [experts] starts, [experts] pairs in earlier blocks
+    int *start = shared, *earlier = shared + p.experts;
+    for (int e = threadIdx.x; e < 2 * p.experts; e += blockDim.x) shared[e] = 0;
+    grid_dependency_entry();
+    __syncthreads();
+    const int ranges = max(1, int(blockDim.x) / p.experts);        // threads per expert
+    const int e = int(threadIdx.x) % p.experts, range = int(threadIdx.x) / p.experts;
+    if (range < ranges) {
+        const int b0 = blocks * range / ranges, b1 = blocks * (range + 1) / ranges;
         int sum = 0, before = 0;
-        for (int b = 0; b < blocks; ++b) {
-            if (b == int(blockIdx.x)) before = sum;
-            sum += p.block_counts[(long long)b * p.experts + e];
+#pragma unroll 8
+        for (int b = b0; b < b1; ++b) {
+            const int c = p.block_counts[(long long)b * p.experts + e];
+            sum += c;
+            if (b < int(blockIdx.x)) before += c;
         }
-        start[e] = sum;
-        earlier[e] = before;
+        atomicAdd(&start[e], sum);                      // whole numbers: the order does not matter
+        atomicAdd(&earlier[e], before);
     }
     __syncthreads();
     const int used = exclusive_scan(start, p.experts);
     if (blockIdx.x == 0) {
-        for (int e = threadIdx.x; e < p.experts; e += kRouteThreads) p.offsets[e] = start[e];
+        for (int i = threadIdx.x; i < p.experts; i += blockDim.x) p.offsets[i] = start[i];
         if (threadIdx.x == 0) p.offsets[p.experts] = used;
     }
     const int first = blockIdx.x * per_block, last = min(p.tokens, first + per_block);
     const long long pair0 = (long long)first * p.k;
     const int pairs = (last - first) * p.k;
-    for (int i = threadIdx.x; i < pairs; i += kRouteThreads) {
-        const int e = p.chosen[pair0 + i];
-        if (e < 0) continue;
-        const int slot = p.slots[pair0 + i] + start[e] + earlier[e];
+    for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+        const int expert = p.chosen[pair0 + i];
+        if (expert < 0) continue;
+        const int slot = p.slots[pair0 + i] + start[expert] + earlier[expert];
         p.slots[pair0 + i] = slot;
         p.rows[slot] = first + i / p.k;
     }
     const long long all = (long long)p.tokens * p.k;
-    for (long long i = used + (long long)blockIdx.x * kRouteThreads + threadIdx.x; i < all; i += (long long)blocks * kRouteThreads)
+    for (long long i = used + (long long)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (long long)blocks * blockDim.x)
         p.rows[i] = -1;
 }
 
-// Tokens one block plans: a small call is one block and one launch; beyond that at most 128 blocks, because every
-// block of the second pass reads the counts of all of them.
-constexpr int kRouteSingleTokens = 256;
-int route_per_block(int tokens) { return tokens <= kRouteSingleTokens ? tokens : std::max(32, (tokens + 127) / 128); }
-int route_blocks(int tokens) { return (tokens + route_per_block(tokens) - 1) / route_per_block(tokens); }
+// Tokens one block plans: a small call is one block and one launch; beyond that about 128 blocks, because every block of
+// the second pass reads the counts of all of them.
+constexpr int kRouteSingleTokens = 128;
+int route_per_block(int tokens, int k) {
+    if (tokens <= kRouteSingleTokens) return tokens;
+    return std::min(std::max(32, (tokens + 127) / 128), kRoutePairs / k);
+}
+int route_blocks(int tokens, int k) { return (tokens + route_per_block(tokens, k) - 1) / route_per_block(tokens, k); }
 
 template <class T, int PER>
 cudaError_t route_run(const RouteParams &p, cudaStream_t stream) {
-    const int per_block = route_per_block(p.tokens), blocks = route_blocks(p.tokens);
-    const size_t smem = size_t(kRouteWarps + 1) * p.experts * sizeof(int);
-    const void *fn = blocks == 1 ? reinterpret_cast<const void *>(route_pick_kernel<T, PER, true>)
-                                 : reinterpret_cast<const void *>(route_pick_kernel<T, PER, false>);
+    const int per_block = route_per_block(p.tokens, p.k), blocks = route_blocks(p.tokens, p.k);
+    const int threads = p.tokens <= 8 ? 256 : kRouteThreads;
+    const size_t smem = (size_t(threads / 32 + 1) * p.experts + 2 * size_t(per_block) * p.k) * sizeof(int);
+    const auto pick = blocks == 1 ? route_pick_kernel<T, PER, true> : route_pick_kernel<T, PER, false>;
     if (smem > 48 * 1024) {
-        cudaError_t err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        cudaError_t err = cudaFuncSetAttribute(pick, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
         if (err != cudaSuccess) return err;
     }
-    if (blocks == 1) {
-        route_pick_kernel<T, PER, true><<<1, kRouteThreads, smem, stream>>>(p, per_block);
-        return cudaGetLastError();
-    }
-    route_pick_kernel<T, PER, false><<<blocks, kRouteThreads, smem, stream>>>(p, per_block);
-    route_place_kernel<<<blocks, kRouteThreads, 2 * p.experts * sizeof(int), stream>>>(p, per_block, blocks);
-    return cudaGetLastError();
+    cudaError_t err = launch(pick, blocks, threads, smem, stream, p, per_block);
+    if (err == cudaSuccess && blocks > 1)
+        err = launch(route_place_kernel, blocks, kRouteThreads, 2 * size_t(p.experts) * sizeof(int), stream, p, per_block, blocks);
+    return err;
 }
 
 template <class T>
@@ -257,6 +336,8 @@ cudaError_t route_typed(const RouteParams &p, cudaStream_t stream) {
 }
 
 // ---- row quantiser -----------------------------------------------------------------------------
+
+constexpr float kLift = 18446744073709551616.0f;      // 2^64: rows of tiny values are lifted by it, so that 127 / largest stays finite
 
 // The whole number nearest to 127 x / largest (halves to even), from the float product x * inverse and, where that
 // falls next to a half, from the exact comparison of 127 |x| with (n + 1/2) largest: both are at most 33 bits long,
@@ -276,67 +357,181 @@ __device__ __forceinline__ int quantize_one(float x, float inverse, float larges
     return x < 0 ? -q : q;
 }
 
-// One row per block.  The row is read twice: the second pass finds it in L1.
-template <class T>
-__global__ void __launch_bounds__(256) quantize_kernel(const QuantizeParams p) {
-    __shared__ float warp_max[8];
-    for (long long r = blockIdx.x; r < p.total; r += gridDim.x) {
-        long long src = p.rows ? p.rows[r] : r;
-        const bool live = src >= 0 && src < p.x_rows;
-        const T *x = static_cast<const T *>(p.x) + (live ? src : 0) * p.x_stride;
-        float largest = 0.0f;
-        if (live)
-            for (int c = threadIdx.x; c < p.inner; c += blockDim.x) {
-                const float v = fabsf(to_float(x[c]));
-                if (v <= 3.402823466e38f) largest = fmaxf(largest, v);
-            }
+// Rows whose vectors of eight elements stay in the registers of a group of G threads, V per thread: read once.  Where the
+// quotient is clear of a half it is rounded directly; a thread with anything else among its eight takes the exact form.
+template <class T, int G, int V>
+__global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_rows_kernel(const QuantizeParams p) {
+    constexpr int kBlock = G < 256 ? 256 : G;
+    __shared__ float warp_max[kBlock / 32];
+    const int member = threadIdx.x % G;
+    const long long r = (long long)blockIdx.x * (kBlock / G) + threadIdx.x / G;
+    grid_dependency_entry();
+    const long long src = r >= p.total ? -1 : p.rows ? p.rows[r] : r;
+    const bool live = src >= 0 && src < p.x_rows;
+    const T *x = static_cast<const T *>(p.x) + (live ? src : 0) * p.x_stride;
+    float v[V][8], largest = 0.0f;
+    bool odd = false;
 #pragma unroll
-        for (int s = 16; s > 0; s >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, s));
+    for (int i = 0; i < V; ++i) {
+        const int c = (i * G + member) * 8;
+        if (live && c < p.inner) {
+            load8(x + c, v[i]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float a = fabsf(v[i][j]);
+                const bool finite = a <= 3.402823466e38f;
+                largest = fmaxf(largest, finite ? a : 0.0f);
+                odd |= !finite;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+        }
+    }
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, s));
+    if (G > 32) {
         if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = largest;
         __syncthreads();
+        const int warp0 = threadIdx.x / G * (G / 32);
 #pragma unroll
-        for (int w = 0; w < 8; ++w) largest = fmaxf(largest, warp_max[w]);
-        __syncthreads();
-        if (threadIdx.x == 0) p.scale[r] = largest / 127.0f;
-        // rows of tiny values are lifted by 2^64, so that 127 / largest stays finite
-        const float lift = largest < 1e-30f ? 18446744073709551616.0f : 1.0f;
-        const float inverse = largest > 0.0f ? 127.0f / (largest * lift) : 0.0f;
-        signed char *q = p.q + r * p.q_stride;
-        for (int c = threadIdx.x; c < p.inner; c += blockDim.x)
-            q[c] = live ? (signed char)quantize_one(to_float(x[c]), inverse, largest, lift) : 0;
+        for (int w = 0; w < G / 32; ++w) largest = fmaxf(largest, warp_max[warp0 + w]);
     }
+    if (r >= p.total) return;
+    if (member == 0) p.scale[r] = largest / 127.0f;
+    const float lift = largest < 1e-30f ? kLift : 1.0f;
+    const float inverse = largest > 0.0f ? 127.0f / (largest * lift) : 0.0f;
+    signed char *q = p.q + r * p.q_stride;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int c = (i * G + member) * 8;
+        if (c >= p.inner) continue;
+        int n[8];
+        bool exact = odd || lift != 1.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float f = v[i][j] * inverse, w = rintf(f);
+            n[j] = int(w);
+            exact |= fabsf(f - w) > 0.499f;
+        }
+        if (exact) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) n[j] = quantize_one(v[i][j], inverse, largest, lift);
+        }
+        uint2 packed;
+        packed.x = uint32_t(n[0] & 255) | uint32_t(n[1] & 255) << 8 | uint32_t(n[2] & 255) << 16 | uint32_t(n[3] & 255) << 24;
+        packed.y = uint32_t(n[4] & 255) | uint32_t(n[5] & 255) << 8 | uint32_t(n[6] & 255) << 16 | uint32_t(n[7] & 255) << 24;
+        *reinterpret_cast<uint2 *>(q + c) = packed;
+    }
+}
+
+// Rows of any length, alignment and stride: a row per block, read twice, element by element.
+template <class T>
+__global__ void __launch_bounds__(256) quantize_any_kernel(const QuantizeParams p) {
+    __shared__ float warp_max[8];
+    const long long r = blockIdx.x;
+    grid_dependency_entry();
+    const long long src = p.rows ? p.rows[r] : r;
+    const bool live = src >= 0 && src < p.x_rows;
+    const T *x = static_cast<const T *>(p.x) + (live ? src : 0) * p.x_stride;
+    float largest = 0.0f;
+    if (live)
+        for (int c = threadIdx.x; c < p.inner; c += 256) {
+            const float v = fabsf(to_float(x[c]));
+            if (v <= 3.402823466e38f) largest = fmaxf(largest, v);
+        }
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, s));
+    if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = largest;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) largest = fmaxf(largest, warp_max[w]);
+    if (threadIdx.x == 0) p.scale[r] = largest / 127.0f;
+    const float lift = largest < 1e-30f ? kLift : 1.0f;
+    const float inverse = largest > 0.0f ? 127.0f / (largest * lift) : 0.0f;
+    signed char *q = p.q + r * p.q_stride;
+    for (int c = threadIdx.x; c < p.inner; c += 256)
+        q[c] = live ? (signed char)quantize_one(to_float(x[c]), inverse, largest, lift) : 0;
+}
+
+template <class T>
+cudaError_t quantize_typed(const QuantizeParams &p, cudaStream_t stream) {
+    const bool vectors = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.x_stride * int(sizeof(T)) % 16 == 0 && p.inner % 8 == 0 &&
+                         reinterpret_cast<uintptr_t>(p.q) % 8 == 0 && p.q_stride % 8 == 0;
+    const int pieces = p.inner / 8;
+    const auto go = [&](auto kernel, int block, long long rows) {
+        return launch(kernel, (p.total + rows - 1) / rows, block, 0, stream, p);
+    };
+    // a warp per row up to 1024 elements, four warps up to 4096, sixteen up to 16384
+    if (!vectors || pieces > 512 * 4) return go(quantize_any_kernel<T>, 256, 1);
+    if (pieces <= 32) return go(quantize_rows_kernel<T, 32, 1>, 256, 8);
+    if (pieces <= 64) return go(quantize_rows_kernel<T, 32, 2>, 256, 8);
+    if (pieces <= 128) return go(quantize_rows_kernel<T, 32, 4>, 256, 8);
+    if (pieces <= 256) return go(quantize_rows_kernel<T, 128, 2>, 256, 2);
+    if (pieces <= 512) return go(quantize_rows_kernel<T, 128, 4>, 256, 2);
+    if (pieces <= 1024) return go(quantize_rows_kernel<T, 512, 2>, 512, 1);
+    return go(quantize_rows_kernel<T, 512, 4>, 512, 1);
 }
 
 // ---- weighted sum of expert rows ----------------------------------------------------------------
 
-template <class T, class O>
-__global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
-    for (long long t = blockIdx.x; t < p.tokens; t += gridDim.x) {
-        const float *gates = p.gates + t * p.k;
-        const int *slots = p.slots + t * p.k;
-        O *out = static_cast<O *>(p.out) + t * p.out_stride;
-        for (int c = threadIdx.x; c < p.channels; c += blockDim.x) {
-            float sum = 0.0f;
-            for (int j = 0; j < p.k; ++j) {
-                const int s = slots[j];
-                if (s >= 0 && s < p.y_rows) sum += gates[j] * to_float(static_cast<const T *>(p.y)[(long long)s * p.y_stride + c]);
-            }
-            out[c] = from_float<O>(sum);
+// V consecutive channels of a token per thread, 16 bytes of the rows at a time (or one element: V = 1); eight rows are
+// asked for before the first is added.
+template <class T, class O, int V>
+__global__ void __launch_bounds__(256) combine_kernel(const CombineParams p, int across) {
+    const int lane = threadIdx.x % across;
+    const long long t = (long long)blockIdx.x * (256 / across) + threadIdx.x / across;
+    const int c = (int(blockIdx.y) * across + lane) * V;
+    grid_dependency_entry();
+    if (t >= p.tokens || c >= p.channels) return;
+    const float *gates = p.gates + t * p.k;
+    const int *slots = p.slots + t * p.k;
+    float sum[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] = 0.0f;
+    // (every load is made, from row 0 where a slot names none: under a branch they would wait for one another)
+    for (int j0 = 0; j0 < p.k && p.y_rows > 0; j0 += 8) {
+        float part[8][V], gate[8];
+        bool live[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int s = j0 + j < p.k ? slots[j0 + j] : -1;
+            live[j] = s >= 0 && s < p.y_rows;
+            gate[j] = live[j] ? gates[j0 + j] : 0.0f;
+            load_vector(static_cast<const T *>(p.y) + (live[j] ? (long long)s * p.y_stride : 0) + c, part[j]);
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum[i] += live[j] ? gate[j] * part[j][i] : 0.0f;
     }
+    store_vector(static_cast<O *>(p.out) + t * p.out_stride + c, sum);
+}
+
+template <class T, class O>
+cudaError_t combine_run(const CombineParams &p, cudaStream_t stream) {
+    constexpr int kWide = 16 / int(sizeof(T));
+    const bool vectors = reinterpret_cast<uintptr_t>(p.y) % 16 == 0 && p.y_stride % kWide == 0 && p.channels % kWide == 0 &&
+                         reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_stride * int(sizeof(O)) % 16 == 0;
+    const int pieces = vectors ? p.channels / kWide : p.channels;
+    int across = 8;                                    // threads of a block along the channels
+    while (across < 256 && across < pieces) across *= 2;
+    const dim3 grid(unsigned((p.tokens + 256 / across - 1) / (256 / across)), unsigned((pieces + across - 1) / across));
+    return vectors ? launch(combine_kernel<T, O, kWide>, grid, 256, 0, stream, p, across)
+                   : launch(combine_kernel<T, O, 1>, grid, 256, 0, stream, p, across);
 }
 
 template <class T>
-void combine_typed(const CombineParams &p, unsigned blocks, cudaStream_t stream) {
-    if (p.out_type == Elem::F32) combine_kernel<T, float><<<blocks, 256, 0, stream>>>(p);
-    else if (p.out_type == Elem::F16) combine_kernel<T, __half><<<blocks, 256, 0, stream>>>(p);
-    else combine_kernel<T, __nv_bfloat16><<<blocks, 256, 0, stream>>>(p);
+cudaError_t combine_typed(const CombineParams &p, cudaStream_t stream) {
+    if (p.out_type == Elem::F32) return combine_run<T, float>(p, stream);
+    if (p.out_type == Elem::F16) return combine_run<T, __half>(p, stream);
+    return combine_run<T, __nv_bfloat16>(p, stream);
 }
 
 }  // namespace
 
-size_t route_workspace_bytes(int tokens, int experts) {
-    const int blocks = route_blocks(tokens);
+size_t route_workspace_bytes(int tokens, int experts, int k) {
+    const int blocks = route_blocks(tokens, k);
     return blocks == 1 ? 0 : size_t(blocks) * experts * sizeof(int);
 }
 
@@ -347,19 +542,15 @@ cudaError_t launch_route(const RouteParams &p, cudaStream_t stream) {
 }
 
 cudaError_t launch_quantize(const QuantizeParams &p, cudaStream_t stream) {
-    const unsigned blocks = unsigned(std::min<long long>(p.total, INT_MAX));
-    if (p.type == Elem::F32) quantize_kernel<float><<<blocks, 256, 0, stream>>>(p);
-    else if (p.type == Elem::F16) quantize_kernel<__half><<<blocks, 256, 0, stream>>>(p);
-    else quantize_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(p);
-    return cudaGetLastError();
+    if (p.type == Elem::F32) return quantize_typed<float>(p, stream);
+    if (p.type == Elem::F16) return quantize_typed<__half>(p, stream);
+    return quantize_typed<__nv_bfloat16>(p, stream);
 }
 
 cudaError_t launch_combine(const CombineParams &p, cudaStream_t stream) {
-    const unsigned blocks = unsigned(std::min<long long>(p.tokens, INT_MAX));
-    if (p.type == Elem::F32) combine_typed<float>(p, blocks, stream);
-    else if (p.type == Elem::F16) combine_typed<__half>(p, blocks, stream);
-    else combine_typed<__nv_bfloat16>(p, blocks, stream);
-    return cudaGetLastError();
+    if (p.type == Elem::F32) return combine_typed<float>(p, stream);
+    if (p.type == Elem::F16) return combine_typed<__half>(p, stream);
+    return combine_typed<__nv_bfloat16>(p, stream);
 }
 
 }  // namespace ios

@@ -29,7 +29,7 @@ struct RouteParams {
     int *slots;             // [tokens][k]
     int *block_counts;      // workspace, [blocks][experts]; unused when one block does everything
 };
-size_t route_workspace_bytes(int tokens, int experts);
+size_t route_workspace_bytes(int tokens, int experts, int k);
 cudaError_t launch_route(const RouteParams &p, cudaStream_t stream);
 
 struct QuantizeParams {

@@ -16,6 +16,7 @@ See ``include/ios_runtime.h`` for the formulas.  (The reference has no counterpa
 convolution networks.)
 """
 import ctypes
+import functools
 from collections import namedtuple
 
 _ACTS = {'identity': 0, 'relu': 1, 'sigmoid': 2, 'tanh': 3, 'silu': 4}
@@ -27,7 +28,7 @@ _INT, _LONG, _PTR, _SIZE = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p, cty
 
 def declare(handle):
     """Argument types of this module's entry points; called by the library loader."""
-    handle.ios_route_experts_workspace.argtypes = [_INT, _INT, ctypes.POINTER(_SIZE)]
+    handle.ios_route_experts_workspace.argtypes = [_INT, _INT, _INT, ctypes.POINTER(_SIZE)]
     handle.ios_route_experts.argtypes = [_PTR, _INT, _INT, _INT, _LONG, _INT, _INT] + [_PTR] * 6 + [_SIZE, _PTR]
     handle.ios_grouped_matmul.argtypes = [_PTR, _INT, _LONG, _LONG, _PTR, _INT, _INT, _INT, _LONG, _LONG, _PTR, _PTR, _INT,
                                           _PTR, _PTR, _PTR, _INT, _INT, _PTR, _INT, _LONG, _PTR]
@@ -38,77 +39,109 @@ def declare(handle):
     handle.ios_combine_experts.argtypes = [_PTR, _INT, _LONG, _LONG, _PTR, _PTR, _LONG, _INT, _INT, _PTR, _INT, _LONG, _PTR]
 
 
-class _Torch:
-    """torch and its types, looked up on the first call (the rest of the package does not need torch)."""
-    module = None
-    codes = {}
+torch = None          # looked up on the first call: the rest of the package does not need it
+_codes = {}           # torch type -> element type of the C interface
+_lib = None
+_raw_stream = None
+_FLOATS, _ALL, _INT8 = (0, 1, 2), (0, 1, 2, 3), (3,)
 
-    @classmethod
-    def get(cls):
-        if cls.module is None:
-            import torch
-            cls.codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}
-            cls.module = torch
-        return cls.module
+
+def _load():
+    global torch, _lib, _raw_stream
+    import torch as module
+    from . import ios_runtime
+    _codes.update({module.float32: 0, module.float16: 1, module.bfloat16: 2, module.int8: 3})
+    # the stream's handle without a Stream object around it, where torch offers that: these calls are short
+    _raw_stream = getattr(module._C, '_cuda_getCurrentRawStream', None) or (lambda index: module.cuda.current_stream(index).cuda_stream)
+    _lib = ios_runtime._library()
+    torch = module
 
 
 def _matrix(tensor, name, dims, codes):
     """Checks a tensor whose last axis is dense and returns the code of its type."""
-    torch = _Torch.get()
+    if torch is None:
+        _load()
     if not isinstance(tensor, torch.Tensor):
         raise ValueError(f'{name} must be a torch.Tensor')
+    code = _codes.get(tensor.dtype)
+    if code not in codes:
+        raise ValueError(f'{name} has type {tensor.dtype}, which this operator does not take')
     if tensor.dim() != dims:
         raise ValueError(f'{name} must have {dims} axes, not {tensor.dim()}')
-    code = _Torch.codes.get(tensor.dtype)
-    if code is None or code not in codes:
-        raise ValueError(f'{name} has type {tensor.dtype}, which this operator does not take')
     if not tensor.is_cuda:
         raise ValueError(f'{name} must be on a GPU')
     if tensor.requires_grad and torch.is_grad_enabled():
         raise ValueError(f'{name} asks for a gradient: this operator has none, call it under torch.no_grad()')
-    if tensor.shape[-1] > 1 and tensor.stride(-1) != 1:
+    if tensor.stride(-1) != 1 and tensor.shape[-1] > 1:
         raise ValueError(f'the last axis of {name} must be dense (its stride is {tensor.stride(-1)})')
     return code
 
 
-def _dense(tensor, name, shape, dtype, device):
+def _dense(tensor, name, shape, dtype, index):
     """Checks an optional dense tensor of known shape; returns its address."""
     if tensor is None:
         return None
-    if not isinstance(tensor, _Torch.get().Tensor) or tensor.dtype != dtype or tuple(tensor.shape) != shape:
-        raise ValueError(f'{name} must be a {dtype} tensor of shape {shape}')
-    if tensor.device != device:
-        raise ValueError(f'{name} is on {tensor.device}, the operands are on {device}')
+    if not isinstance(tensor, torch.Tensor) or tensor.dtype != dtype or tensor.shape != shape:
+        raise ValueError(f'{name} must be a {dtype} tensor of shape {tuple(shape)}')
+    if tensor.get_device() != index:
+        raise ValueError(f'{name} is on {tensor.device}, the operands are on cuda:{index}')
     if not tensor.is_contiguous():
         raise ValueError(f'{name} must be contiguous')
-    if tensor.requires_grad and _Torch.module.is_grad_enabled():
+    if tensor.requires_grad and torch.is_grad_enabled():
         raise ValueError(f'{name} asks for a gradient: this operator has none, call it under torch.no_grad()')
     return tensor.data_ptr()
 
 
-def _same_device(tensor, name, device):
-    if tensor.device != device:
-        raise ValueError(f'{name} is on {tensor.device}, the operands are on {device}')
+def _needed(tensor, name, shape, dtype, index):
+    if tensor is None:
+        raise ValueError(f'{name} must not be None')
+    return _dense(tensor, name, shape, dtype, index)
 
 
-def _output(out, shape, dtype, device):
-    """The output tensor: a new one, or the caller's after a check."""
+def _same_device(tensor, name, index):
+    if tensor.get_device() != index:
+        raise ValueError(f'{name} is on {tensor.device}, the operands are on cuda:{index}')
+
+
+def _length(rows, name='rows'):
+    if not isinstance(rows, torch.Tensor) or rows.dim() != 1:
+        raise ValueError(f'{name} must be a tensor of one axis')
+    return rows.shape[0]
+
+
+def _output(out, out_dtype, default, like, shape):
+    """(tensor, code of its type, row stride): a new one of `out_dtype`, else `default`, or the caller's after a check."""
     if out is None:
-        return _Torch.module.empty(shape, dtype=dtype, device=device)
-    _matrix(out, 'out', len(shape), (0, 1, 2))
-    if tuple(out.shape) != shape or (dtype is not None and out.dtype != dtype):
-        raise ValueError(f'out must be a {dtype} tensor of shape {shape}')
-    _same_device(out, 'out', device)
-    return out
+        dtype = default if out_dtype is None else out_dtype
+        code = _codes.get(dtype)
+        if code not in _FLOATS:
+            raise ValueError(f'the result cannot have type {dtype}')
+        return like.new_empty(shape, dtype=dtype), code, shape[1]
+    code = _matrix(out, 'out', 2, _FLOATS)
+    if out.shape != shape or (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError(f'out must be a {out.dtype if out_dtype is None else out_dtype} tensor of shape {shape}')
+    _same_device(out, 'out', like.get_device())
+    return out, code, max(out.stride(0), shape[1]) if shape[0] == 1 else out.stride(0)
 
 
-def _stream(device):
-    return _Torch.module.cuda.current_stream(device).cuda_stream
+def _act(act):
+    code = _ACTS.get(act)
+    if code is None:
+        raise ValueError(f'act must be one of {", ".join(_ACTS)}')
+    return code
 
 
-def _call(entry, *args):
-    from . import ios_runtime
-    ios_runtime._check(getattr(ios_runtime._library(), entry)(*args))
+def _check(status):
+    if status != 0:
+        from . import ios_runtime
+        ios_runtime._check(status)
+
+
+@functools.lru_cache(maxsize=None)
+def _route_workspace(tokens, experts, k):
+    need = _SIZE(0)
+    _check(_lib.ios_route_experts_workspace(tokens, experts, k, ctypes.byref(need)))
+    return need.value
 
 
 def route_experts(logits, k, renormalize=True):
@@ -120,24 +153,23 @@ def route_experts(logits, k, renormalize=True):
     never chosen; a token with fewer than ``k`` others gets experts and slots of -1 and gates of 0 in their place.
     ``renormalize``: the gates of a token sum to one; otherwise they are its softmax over all experts.
     """
-    code = _matrix(logits, 'logits', 2, (0, 1, 2))
-    torch = _Torch.module
+    code = _matrix(logits, 'logits', 2, _FLOATS)
     tokens, experts = logits.shape
     k = int(k)
     if not 1 <= k <= experts:
         raise ValueError(f'k must be in 1..{experts}, not {k}')
-    device = logits.device
-    need = _SIZE(0)
-    _call('ios_route_experts_workspace', tokens, experts, ctypes.byref(need))
-    pairs = tokens * k
-    # one allocation: [experts | slots | rows | offsets], then the workspace
-    whole = torch.empty(3 * pairs + experts + 1 + (need.value + 3) // 4, dtype=torch.int32, device=device)
-    chosen, slots, rows, offsets, work = whole.split([pairs, pairs, pairs, experts + 1, whole.numel() - 3 * pairs - experts - 1])
-    gates = torch.empty((tokens, k), dtype=torch.float32, device=device)
-    _call('ios_route_experts', logits.data_ptr(), code, tokens, experts, logits.stride(0), k, 1 if renormalize else 0,
-          chosen.data_ptr(), gates.data_ptr(), offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(),
-          work.data_ptr() if need.value else None, need.value, _stream(device))
-    return Routing(chosen.view(tokens, k), gates, offsets, rows, slots.view(tokens, k))
+    pairs, need = tokens * k, _route_workspace(tokens, experts, k)
+    # one allocation for everything: experts, slots, gates, rows, offsets, workspace
+    whole = logits.new_empty(4 * pairs + experts + 1 + (need + 3) // 4, dtype=torch.int32)
+    chosen, slots, gates, rows, offsets, work = whole.split_with_sizes(
+        (pairs, pairs, pairs, pairs, experts + 1, (need + 3) // 4))
+    gates = gates.view(torch.float32)
+    base = whole.data_ptr()
+    _check(_lib.ios_route_experts(
+        logits.data_ptr(), code, tokens, experts, logits.stride(0), k, 1 if renormalize else 0, base, base + 8 * pairs,
+        base + 16 * pairs, base + 12 * pairs, base + 4 * pairs, work.data_ptr() if need else None, need,
+        _raw_stream(logits.get_device())))
+    return Routing(chosen.view(tokens, k), gates.view(tokens, k), offsets, rows, slots.view(tokens, k))
 
 
 def grouped_matmul(x, weight, offsets, rows=None, bias=None, act='identity', gated=False, row_scale=None,
@@ -150,42 +182,30 @@ def grouped_matmul(x, weight, offsets, rows=None, bias=None, act='identity', gat
     rows per group and the result is ``act(first half) * second half``.  The result has as many rows as ``rows`` (else
     ``x``); those behind ``offsets[-1]`` are not written.  ``out_dtype``: the type of ``x`` unless given (int8: bfloat16).
     """
-    code = _matrix(x, 'x', 2, (0, 1, 2, 3))
-    torch = _Torch.module
-    if _matrix(weight, 'weight', 3, (0, 1, 2, 3)) != code:
+    code = _matrix(x, 'x', 2, _ALL)
+    if _matrix(weight, 'weight', 3, _ALL) != code:
         raise ValueError(f'x is {x.dtype}, weight {weight.dtype}: they must have one type')
-    device = x.device
-    _same_device(weight, 'weight', device)
-    groups, channels, inner = weight.shape
-    if x.shape[1] != inner:
-        raise ValueError(f'x has rows of {x.shape[1]} elements, weight of {inner}')
-    per_group = channels
+    index = x.get_device()
+    _same_device(weight, 'weight', index)
+    x_rows, inner = x.shape
+    groups, per_group, weight_inner = weight.shape
+    if weight_inner != inner:
+        raise ValueError(f'x has rows of {inner} elements, weight of {weight_inner}')
+    channels = per_group
     if gated:
-        if channels % 2:
-            raise ValueError(f'a gated product needs an even number of weight rows, not {channels}')
-        channels //= 2
-    if act not in _ACTS:
-        raise ValueError(f'act must be one of {", ".join(_ACTS)}')
-    offsets_at = _dense(offsets, 'offsets', (groups + 1,), torch.int32, device)
-    if offsets_at is None:
-        raise ValueError('offsets must not be None')
-    total = x.shape[0]
-    if rows is not None:
-        if not isinstance(rows, torch.Tensor) or rows.dim() != 1:
-            raise ValueError('rows must be a tensor of one axis')
-        total = rows.shape[0]
-    rows_at = _dense(rows, 'rows', (total,), torch.int32, device)
-    if out_dtype is None:
-        out_dtype = out.dtype if out is not None else (torch.bfloat16 if code == 3 else x.dtype)
-    if _Torch.codes.get(out_dtype) not in (0, 1, 2):
-        raise ValueError(f'the result cannot have type {out_dtype}')
-    out = _output(out, (total, channels), out_dtype, device)
-    _call('ios_grouped_matmul', x.data_ptr(), code, x.shape[0], x.stride(0), weight.data_ptr(), groups, channels, inner,
-          weight.stride(1), weight.stride(0), offsets_at, rows_at, total,
-          _dense(row_scale, 'row_scale', (x.shape[0],), torch.float32, device),
-          _dense(channel_scale, 'channel_scale', (groups, per_group), torch.float32, device),
-          _dense(bias, 'bias', (groups, per_group), torch.float32, device),
-          _ACTS[act], 1 if gated else 0, out.data_ptr(), _Torch.codes[out_dtype], out.stride(0), _stream(device))
+        if per_group % 2:
+            raise ValueError(f'a gated product needs an even number of weight rows, not {per_group}')
+        channels = per_group // 2
+    total = x_rows if rows is None else _length(rows)
+    f32, i32 = torch.float32, torch.int32
+    out, out_code, out_stride = _output(out, out_dtype, torch.bfloat16 if code == 3 else x.dtype, x, (total, channels))
+    _check(_lib.ios_grouped_matmul(
+        x.data_ptr(), code, x_rows, x.stride(0), weight.data_ptr(), groups, channels, inner, weight.stride(1), weight.stride(0),
+        _needed(offsets, 'offsets', (groups + 1,), i32, index), _dense(rows, 'rows', (total,), i32, index), total,
+        _dense(row_scale, 'row_scale', (x_rows,), f32, index),
+        _dense(channel_scale, 'channel_scale', (groups, per_group), f32, index),
+        _dense(bias, 'bias', (groups, per_group), f32, index), _act(act), 1 if gated else 0, out.data_ptr(), out_code, out_stride,
+        _raw_stream(index)))
     return out
 
 
@@ -194,26 +214,20 @@ def matmul_int8(a, b, row_scale=None, channel_scale=None, bias=None, act='identi
     ``act(a @ b.T * row_scale[:, None] * channel_scale + bias)`` for int8 ``a`` [rows, inner] and ``b`` [channels, inner], the
     sums exact; scales and bias float32.  The result is bfloat16 unless ``out_dtype`` says otherwise.
     """
-    _matrix(a, 'a', 2, (3,))
-    _matrix(b, 'b', 2, (3,))
-    torch, device = _Torch.module, a.device
-    _same_device(b, 'b', device)
+    _matrix(a, 'a', 2, _INT8)
+    _matrix(b, 'b', 2, _INT8)
+    index = a.get_device()
+    _same_device(b, 'b', index)
     rows, inner = a.shape
-    channels = b.shape[0]
-    if b.shape[1] != inner:
-        raise ValueError(f'a has rows of {inner} elements, b of {b.shape[1]}')
-    if act not in _ACTS:
-        raise ValueError(f'act must be one of {", ".join(_ACTS)}')
-    if out_dtype is None:
-        out_dtype = out.dtype if out is not None else torch.bfloat16
-    if _Torch.codes.get(out_dtype) not in (0, 1, 2):
-        raise ValueError(f'the result cannot have type {out_dtype}')
-    out = _output(out, (rows, channels), out_dtype, device)
-    _call('ios_matmul_int8', a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), rows, channels, inner,
-          _dense(row_scale, 'row_scale', (rows,), torch.float32, device),
-          _dense(channel_scale, 'channel_scale', (channels,), torch.float32, device),
-          _dense(bias, 'bias', (channels,), torch.float32, device),
-          _ACTS[act], out.data_ptr(), _Torch.codes[out_dtype], out.stride(0), _stream(device))
+    channels, b_inner = b.shape
+    if b_inner != inner:
+        raise ValueError(f'a has rows of {inner} elements, b of {b_inner}')
+    f32 = torch.float32
+    out, out_code, out_stride = _output(out, out_dtype, torch.bfloat16, a, (rows, channels))
+    _check(_lib.ios_matmul_int8(
+        a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), rows, channels, inner, _dense(row_scale, 'row_scale', (rows,), f32, index),
+        _dense(channel_scale, 'channel_scale', (channels,), f32, index), _dense(bias, 'bias', (channels,), f32, index), _act(act),
+        out.data_ptr(), out_code, out_stride, _raw_stream(index)))
     return out
 
 
@@ -223,18 +237,14 @@ def quantize_rows(x, rows=None):
     each: ``(q, scale)`` with ``q * scale[:, None]`` nearest to the row and the largest magnitude of a row at 127.  NaN
     becomes 0, an infinity +-127.  On a weight matrix it gives the scale per channel that ``matmul_int8`` takes.
     """
-    code = _matrix(x, 'x', 2, (0, 1, 2))
-    torch, device = _Torch.module, x.device
-    total = x.shape[0]
-    if rows is not None:
-        if not isinstance(rows, torch.Tensor) or rows.dim() != 1:
-            raise ValueError('rows must be a tensor of one axis')
-        total = rows.shape[0]
-    rows_at = _dense(rows, 'rows', (total,), torch.int32, device)
-    q = torch.empty((total, x.shape[1]), dtype=torch.int8, device=device)
-    scale = torch.empty((total,), dtype=torch.float32, device=device)
-    _call('ios_quantize_rows', x.data_ptr(), code, x.shape[0], x.stride(0), x.shape[1], rows_at, total, q.data_ptr(),
-          x.shape[1], scale.data_ptr(), _stream(device))
+    code = _matrix(x, 'x', 2, _FLOATS)
+    index = x.get_device()
+    x_rows, inner = x.shape
+    total = x_rows if rows is None else _length(rows)
+    q, scale = x.new_empty((total, inner), dtype=torch.int8), x.new_empty((total,), dtype=torch.float32)
+    _check(_lib.ios_quantize_rows(
+        x.data_ptr(), code, x_rows, x.stride(0), inner, _dense(rows, 'rows', (total,), torch.int32, index), total, q.data_ptr(), inner,
+        scale.data_ptr(), _raw_stream(index)))
     return q, scale
 
 
@@ -243,27 +253,23 @@ def combine_experts(y, gates, slots, out_dtype=None, out=None):
     The gate-weighted sum of every token's expert rows: ``out[t] = sum_j gates[t, j] * y[slots[t, j]]`` in float32, in the
     order of ``j``.  A slot outside the rows of ``y`` (-1) adds nothing.  The result has the type of ``y`` unless given.
     """
-    code = _matrix(y, 'y', 2, (0, 1, 2))
-    torch, device = _Torch.module, y.device
+    code = _matrix(y, 'y', 2, _FLOATS)
     if not isinstance(slots, torch.Tensor) or slots.dim() != 2:
         raise ValueError('slots must be a tensor of two axes')
-    tokens, k = slots.shape
-    slots_at = _dense(slots, 'slots', (tokens, k), torch.int32, device)
-    gates_at = _dense(gates, 'gates', (tokens, k), torch.float32, device)
-    if gates_at is None:
-        raise ValueError('gates must not be None')
-    if out_dtype is None:
-        out_dtype = out.dtype if out is not None else y.dtype
-    if _Torch.codes.get(out_dtype) not in (0, 1, 2):
-        raise ValueError(f'the result cannot have type {out_dtype}')
-    out = _output(out, (tokens, y.shape[1]), out_dtype, device)
-    _call('ios_combine_experts', y.data_ptr(), code, y.shape[0], y.stride(0), gates_at, slots_at, tokens, k, y.shape[1],
-          out.data_ptr(), _Torch.codes[out_dtype], out.stride(0), _stream(device))
+    index = y.get_device()
+    y_rows, channels = y.shape
+    shape = tokens, k = slots.shape
+    out, out_code, out_stride = _output(out, out_dtype, y.dtype, y, (tokens, channels))
+    _check(_lib.ios_combine_experts(
+        y.data_ptr(), code, y_rows, y.stride(0), _needed(gates, 'gates', shape, torch.float32, index),
+        _dense(slots, 'slots', shape, torch.int32, index), tokens, k, channels, out.data_ptr(), out_code, out_stride,
+        _raw_stream(index)))
     return out
 
 
 def device_ops_status(device=None):
     """Waits for torch's current stream of ``device`` and raises if a bounded wait inside a product ran out since the last call."""
-    torch = _Torch.get()
+    if torch is None:
+        _load()
     index = torch.cuda.current_device() if device is None else torch.device(device).index or 0
-    _call('ios_device_ops_status', index, _stream(index))
+    _check(_lib.ios_device_ops_status(index, _raw_stream(index)))

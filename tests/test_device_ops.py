@@ -38,11 +38,11 @@ def test_route_refuses(lib, change, status):
 
 def test_route_workspace(lib):
     size = ctypes.c_size_t(7)
-    assert lib.ios_route_experts_workspace(1, 64, ctypes.byref(size)) == 0 and size.value == 0
-    assert lib.ios_route_experts_workspace(100000, 1024, ctypes.byref(size)) == 0
+    assert lib.ios_route_experts_workspace(1, 64, 8, ctypes.byref(size)) == 0 and size.value == 0
+    assert lib.ios_route_experts_workspace(100000, 1024, 8, ctypes.byref(size)) == 0
     assert 0 < size.value <= 128 * 1024 * 4
-    assert lib.ios_route_experts_workspace(1, 0, ctypes.byref(size)) == ARGUMENT
-    assert lib.ios_route_experts_workspace(1, 8, None) == ARGUMENT
+    assert lib.ios_route_experts_workspace(1, 0, 8, ctypes.byref(size)) == ARGUMENT
+    assert lib.ios_route_experts_workspace(1, 8, 2, None) == ARGUMENT
 
 
 def grouped(lib, **change):

@@ -67,7 +67,7 @@ def check_route(logits, k, renormalize):
 
 
 @pytest.mark.parametrize('tokens,experts,k,dtype', [
-    (1, 1, 1, F32), (1, 64, 8, BF16), (3, 5, 5, F16), (7, 33, 2, F32), (40, 1000, 32, BF16), (255, 16, 4, F16),
+    (1, 1, 1, F32), (1, 64, 8, BF16), (3, 5, 5, F16), (9, 33, 2, F32), (128, 40, 8, BF16), (129, 40, 8, F16), (40, 1000, 32, BF16), (255, 16, 4, F16),
     (256, 129, 6, F32), (257, 8, 2, BF16), (1000, 60, 4, F32), (5003, 257, 3, F16), (600, 1024, 32, F32)])
 @pytest.mark.parametrize('renormalize', [True, False])
 def test_route(tokens, experts, k, dtype, renormalize):
