@@ -21,37 +21,11 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// one 16-byte access, or a single element
-__device__ __forceinline__ void load_vector(const float *p, float (&v)[4]) {
-    const float4 f = *reinterpret_cast<const float4 *>(p);
-    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-}
-__device__ __forceinline__ void load_vector(const __half *p, float (&v)[8]) {
-    const uint4 raw = *reinterpret_cast<const uint4 *>(p);
-    const __half2 *h = reinterpret_cast<const __half2 *>(&raw);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(h[i]);
-        v[2 * i] = f.x; v[2 * i + 1] = f.y;
-    }
-}
-__device__ __forceinline__ void load_vector(const __nv_bfloat16 *p, float (&v)[8]) {
-    const uint4 raw = *reinterpret_cast<const uint4 *>(p);
-    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&raw);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __bfloat1622float2(h[i]);
-        v[2 * i] = f.x; v[2 * i + 1] = f.y;
-    }
-}
-template <class T>
-__device__ __forceinline__ void load_vector(const T *p, float (&v)[1]) { v[0] = to_float(*p); }
-template <class T>
-__device__ __forceinline__ void load8(const T *p, float (&v)[8]) { load_vector(p, v); }
-__device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
-    load_vector(p, *reinterpret_cast<float (*)[4]>(&v[0]));
-    load_vector(p + 4, *reinterpret_cast<float (*)[4]>(&v[4]));
-}
+// V elements that are moved by one access
+template <class T, int V>
+struct alignas(V * sizeof(T)) Vector {
+    T v[V];
+};
 template <class O, int V>
 __device__ __forceinline__ void store_vector(O *p, const float (&v)[V]) {
     constexpr int kBytes = V * int(sizeof(O)), kPiece = kBytes < 16 ? kBytes : 16, kPer = kPiece / int(sizeof(O));
@@ -357,47 +331,103 @@ __device__ __forceinline__ int quantize_one(float x, float inverse, float larges
     return x < 0 ? -q : q;
 }
 
-// Rows whose vectors of eight elements stay in the registers of a group of G threads, V per thread: read once.  Where the
-// quotient is clear of a half it is rounded directly; a thread with anything else among its eight takes the exact form.
+// Eight elements as they lie in memory, and their magnitudes as whole numbers: in each of the three types the order of the
+// bits without the sign is the order of the magnitudes, infinities and NaN on top.
+template <class T> struct Eight;
+template <> struct Eight<float> {
+    uint32_t w[8];
+    static constexpr uint32_t kInfinite = 0x7F800000u;
+    __device__ __forceinline__ void load(const float *p) {
+        const uint4 a = *reinterpret_cast<const uint4 *>(p), b = *reinterpret_cast<const uint4 *>(p + 4);
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ float at(int i) const { return __uint_as_float(w[i]); }
+    __device__ __forceinline__ void raise(uint32_t &most) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = max(most, w[i] & 0x7FFFFFFFu);
+    }
+    static __device__ __forceinline__ uint32_t key(uint32_t most) { return most; }
+    static __device__ __forceinline__ float magnitude(uint32_t key) { return __uint_as_float(key); }
+};
+struct EightHalves {
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const void *p) {
+        const uint4 a = *static_cast<const uint4 *>(p);
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+    }
+    __device__ __forceinline__ void clear() { w[0] = w[1] = w[2] = w[3] = 0; }
+    __device__ __forceinline__ void raise(uint32_t &most) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most = __vmaxu2(most, w[i] & 0x7FFF7FFFu);
+    }
+    static __device__ __forceinline__ uint32_t key(uint32_t most) { return max(most & 0xFFFFu, most >> 16); }
+};
+template <> struct Eight<__half> : EightHalves {
+    static constexpr uint32_t kInfinite = 0x7C00u;
+    __device__ __forceinline__ float at(int i) const { return __half2float(__ushort_as_half(uint16_t(w[i >> 1] >> (16 * (i & 1))))); }
+    static __device__ __forceinline__ float magnitude(uint32_t key) { return __half2float(__ushort_as_half(uint16_t(key))); }
+};
+template <> struct Eight<__nv_bfloat16> : EightHalves {
+    static constexpr uint32_t kInfinite = 0x7F80u;
+    __device__ __forceinline__ float at(int i) const { return __uint_as_float((i & 1) ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16); }
+    static __device__ __forceinline__ float magnitude(uint32_t key) { return __uint_as_float(key << 16); }
+};
+
+// Rows whose vectors of eight elements stay in the registers of a group of G threads, V per thread: read once.  Adding
+// 1.5 * 2^23 leaves the quotient's nearest whole number in the low bits of the sum; a thread that finds one of its eight
+// next to a half, and every thread of a row that holds an infinity or NaN, takes the exact form instead.
+// (8192 rows of 4096 bfloat16: 100 MB, bound by memory.)
 template <class T, int G, int V>
 __global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_rows_kernel(const QuantizeParams p) {
     constexpr int kBlock = G < 256 ? 256 : G;
-    __shared__ float warp_max[kBlock / 32];
-    const int member = threadIdx.x % G;
+    constexpr float kMagic = 12582912.0f;
+    __shared__ uint32_t warp_key[kBlock / 32];
+    const int member = threadIdx.x % G, warp0 = threadIdx.x / G * (G / 32);
     const long long r = (long long)blockIdx.x * (kBlock / G) + threadIdx.x / G;
     grid_dependency_entry();
     const long long src = r >= p.total ? -1 : p.rows ? p.rows[r] : r;
     const bool live = src >= 0 && src < p.x_rows;
     const T *x = static_cast<const T *>(p.x) + (live ? src : 0) * p.x_stride;
-    float v[V][8], largest = 0.0f;
-    bool odd = false;
+    Eight<T> v[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const int c = (i * G + member) * 8;
-        if (live && c < p.inner) {
-            load8(x + c, v[i]);
+        if (live && c < p.inner) v[i].load(x + c);
+        else v[i].clear();
+    }
+    const auto most_of_row = [&](uint32_t key) {
+        key = __reduce_max_sync(0xffffffffu, key);
+        if (G > 32) {
+            if ((threadIdx.x & 31) == 0) warp_key[threadIdx.x >> 5] = key;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < G / 32; ++w) key = max(key, warp_key[warp0 + w]);
+        }
+        return key;
+    };
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i].raise(most);
+    uint32_t key = most_of_row(Eight<T>::key(most));
+    const bool odd = key >= Eight<T>::kInfinite;
+    if (G > 32 ? __syncthreads_or(odd) : odd) {              // the largest finite magnitude of such a row
+        float largest = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float a = fabsf(v[i][j]);
-                const bool finite = a <= 3.402823466e38f;
-                largest = fmaxf(largest, finite ? a : 0.0f);
-                odd |= !finite;
+                const float a = fabsf(v[i].at(j));
+                if (a <= 3.402823466e38f) largest = fmaxf(largest, a);
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
-        }
-    }
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, s));
-    if (G > 32) {
-        if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = largest;
-        __syncthreads();
-        const int warp0 = threadIdx.x / G * (G / 32);
-#pragma unroll
-        for (int w = 0; w < G / 32; ++w) largest = fmaxf(largest, warp_max[warp0 + w]);
+        const uint32_t finite = most_of_row(__float_as_uint(largest));
+        if (odd) key = finite;
     }
     if (r >= p.total) return;
+    const float largest = odd ? __uint_as_float(key) : Eight<T>::magnitude(key);
     if (member == 0) p.scale[r] = largest / 127.0f;
     const float lift = largest < 1e-30f ? kLift : 1.0f;
     const float inverse = largest > 0.0f ? 127.0f / (largest * lift) : 0.0f;
@@ -406,21 +436,21 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_rows_kernel(const 
     for (int i = 0; i < V; ++i) {
         const int c = (i * G + member) * 8;
         if (c >= p.inner) continue;
-        int n[8];
-        bool exact = odd || lift != 1.0f;
+        uint32_t n[8];
+        float off = odd || lift != 1.0f ? 1.0f : 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float f = v[i][j] * inverse, w = rintf(f);
-            n[j] = int(w);
-            exact |= fabsf(f - w) > 0.499f;
+            const float sum = fmaf(v[i].at(j), inverse, kMagic);
+            n[j] = __float_as_uint(sum);
+            off = fmaxf(off, fabsf(fmaf(v[i].at(j), inverse, kMagic - sum)));
         }
-        if (exact) {
+        if (off > 0.49998f) {                     // (the quotient is off by less than 127 * 2^-23)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) n[j] = quantize_one(v[i][j], inverse, largest, lift);
+            for (int j = 0; j < 8; ++j) n[j] = uint32_t(quantize_one(v[i].at(j), inverse, largest, lift));
         }
         uint2 packed;
-        packed.x = uint32_t(n[0] & 255) | uint32_t(n[1] & 255) << 8 | uint32_t(n[2] & 255) << 16 | uint32_t(n[3] & 255) << 24;
-        packed.y = uint32_t(n[4] & 255) | uint32_t(n[5] & 255) << 8 | uint32_t(n[6] & 255) << 16 | uint32_t(n[7] & 255) << 24;
+        packed.x = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
+        packed.y = __byte_perm(__byte_perm(n[4], n[5], 0x0040), __byte_perm(n[6], n[7], 0x0040), 0x5410);
         *reinterpret_cast<uint2 *>(q + c) = packed;
     }
 }
@@ -491,19 +521,22 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p, int
     for (int i = 0; i < V; ++i) sum[i] = 0.0f;
     // (every load is made, from row 0 where a slot names none: under a branch they would wait for one another)
     for (int j0 = 0; j0 < p.k && p.y_rows > 0; j0 += 8) {
-        float part[8][V], gate[8];
+        Vector<T, V> part[8];
+        float gate[8];
         bool live[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int s = j0 + j < p.k ? slots[j0 + j] : -1;
             live[j] = s >= 0 && s < p.y_rows;
             gate[j] = live[j] ? gates[j0 + j] : 0.0f;
-            load_vector(static_cast<const T *>(p.y) + (live[j] ? (long long)s * p.y_stride : 0) + c, part[j]);
+            part[j] = *reinterpret_cast<const Vector<T, V> *>(static_cast<const T *>(p.y) + (live[j] ? (long long)s * p.y_stride : 0) + c);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
+            if (live[j]) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) sum[i] += live[j] ? gate[j] * part[j][i] : 0.0f;
+                for (int i = 0; i < V; ++i) sum[i] += gate[j] * to_float(part[j].v[i]);
+            }
     }
     store_vector(static_cast<O *>(p.out) + t * p.out_stride + c, sum);
 }
