@@ -76,6 +76,10 @@ struct MmGeom {
     int recv_off, turn_off, table_off, bar_off;   // byte offsets in shared memory
 };
 
+// The same value in every lane, and known to the compiler as such: what depends on it may live in uniform registers, where
+// the tensor core's and the TMA unit's operands have to be.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 struct Tile {
     int group, row0, valid, cols, channel0;
 };
@@ -138,7 +142,7 @@ __device__ void build_table(const GroupedParams &p, const MmGeom &t, const Table
 }
 
 // Tiles of a group: up to 8 column tiles side by side, then the next channels, so that neighbours in the list share
-// weights and rows in L2.
+// weights and rows in L2.  Whole warps call it.
 __device__ __forceinline__ Tile find_tile(const GroupedParams &p, const MmGeom &t, const Table &table, int index, int cta_channel) {
     int lo = 0, hi = p.groups;                    // table.first[lo] <= index < table.first[hi]
     while (hi - lo > 1) {
@@ -154,12 +158,12 @@ __device__ __forceinline__ Tile find_tile(const GroupedParams &p, const MmGeom &
     const int wide = min(8, col_tiles - band * 8);
     const int inside = at - band * 8 * t.n_tiles;
     Tile tile;
-    tile.group = lo;
+    tile.group = uniform(lo);
     const int col0 = (band * 8 + inside % wide) * cols;
-    tile.row0 = begin + col0;
-    tile.valid = min(cols, count - col0);
+    tile.row0 = uniform(begin + col0);
+    tile.valid = uniform(min(cols, count - col0));
     tile.cols = (tile.valid + t.grain - 1) & -t.grain;
-    tile.channel0 = inside / wide * t.tile_channels + cta_channel;
+    tile.channel0 = uniform(inside / wide * t.tile_channels + cta_channel);
     return tile;
 }
 
@@ -412,7 +416,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     __shared__ uint32_t tmem_slot;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *generic = smem_raw + (base - smem_u32(smem_raw));
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const uint32_t b_bytes = uint32_t(PAIR ? t.tn / 2 : t.tn) * kRowBytes;
     const uint32_t stage_bytes = kPlanes * (kATileBytes + b_bytes);
     const uint32_t full0 = base + t.bar_off, empty0 = full0 + 8u * t.stages;
@@ -455,9 +459,9 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     tc_fence_after();
     // (only now: a successor that were to share this SM must find the tensor memory taken, not take it)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const uint32_t tmem = tmem_slot;
-    const int total_tiles = table.first[p.groups];
-    const int rank = PAIR || t.cluster > 1 ? int(cluster_cta_rank()) : 0;
+    const uint32_t tmem = uint32_t(uniform(int(tmem_slot)));
+    const int total_tiles = uniform(table.first[p.groups]);
+    const int rank = PAIR || t.cluster > 1 ? uniform(int(cluster_cta_rank())) : 0;
     const int sharing = PAIR ? 2 : t.cluster;                    // CTAs of a tile
     const int tile0 = int(blockIdx.x) / sharing, tile_step = int(gridDim.x) / sharing;
     const int k_begin = PAIR ? 0 : t.k_steps * rank / t.cluster, k_end = PAIR ? t.k_steps : t.k_steps * (rank + 1) / t.cluster;
@@ -509,7 +513,6 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         }
     } else if (LOADS == kTma && warp == 3) {
         // ---------------- rows ----------------
-        constexpr int kBoxes = (PAIR ? 128 : 256) / kBoxRows;
         const uint32_t elected = elect();
         int s = 0;
         uint32_t phase = 1;
@@ -522,9 +525,8 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
                 if (!ok) break;
                 const uint32_t dst = base + uint32_t(s) * stage_bytes + kATileBytes, bar = full_at + 8u * s;
-#pragma unroll
-                for (int b = 0; b < kBoxes; ++b)                     // (predicated: a branch would cost more than the load)
-                    load_2d<PAIR>(b < loads ? elected : 0u, dst + uint32_t(b * t.box_rows) * kRowBytes, &map_x, bar, k * k_elems, tile.row0 + col0 + b * t.box_rows);
+                for (int b = 0; b < loads; ++b)
+                    load_2d<PAIR>(elected, dst + uint32_t(b * t.box_rows) * kRowBytes, &map_x, bar, k * k_elems, tile.row0 + col0 + b * t.box_rows);
                 if (++s == t.stages) { s = 0; phase ^= 1u; }
             }
         }
