@@ -39,10 +39,11 @@ namespace {
 enum Kind { kF16 = 0, kI8 = 1, kX3 = 2 };       // instruction: 16-bit floats, 8-bit integers, three TF32 products
 enum Loads { kTma = 0, kGather = 1, kRegs = 2 };  // operands by TMA / gathered rows by cp.async warps / all through registers
 
-constexpr int kGatherWarps = 8, kLoaderWarps = 8;
+constexpr int kGatherWarps = 8, kLoaderWarps = 16;
+constexpr int kLoaderRows = 128 / kLoaderWarps; // rows of each operand that a loader warp moves
 constexpr int kBoxRows = 64;                    // rows of x per TMA load, in wide tiles
 constexpr int kNarrowCols = 32;                 // tiles up to here gather a step's rows with one warp
-constexpr int kMaxThreads = 512;
+constexpr int kMaxThreads = 768;
 // Two epilogue warps per lane quarter share a tile's columns; one beside gathering or loader warps, which need the registers.
 __host__ __device__ constexpr int epilogue_warps(int loads) { return loads != kTma ? 4 : 8; }
 __host__ __device__ constexpr int threads_of(int loads) {
@@ -56,7 +57,7 @@ constexpr int kChunkSteps = 4;                  // float32: K steps per partial 
 constexpr int kMaxStages = 12;
 constexpr int kMaxGroupTiles = INT_MAX / kMaxExperts - 1;    // tiles of a group: their sum over all groups fits an int
 constexpr int kBarBytes = 2 * kMaxStages * 8 + 48;    // mbarriers: two per stage, six more
-constexpr size_t kSmemLimit = 227 * 1024, kStaticBytes = 4096;    // ... of which the kernel's static arrays may take
+constexpr size_t kSmemLimit = 227 * 1024, kStaticBytes = 4608;    // ... of which the kernel's static arrays may take
 
 __device__ int g_expert_error;                  // set by a wait that ran out, read by expert_mm_status
 
@@ -289,42 +290,27 @@ __device__ __noinline__ void time_out(int code) {
     while (global_ns() - t0 < 1000000) __nanosleep(1000);
 }
 
-// ---- loader warps: 16 bytes of a row, zeros behind its end, for any alignment ----------------------
-__device__ __noinline__ uint4 load_chunk_edge(const uint8_t *row, long long byte0, long long row_bytes, int esize) {
-    uint4 out = make_uint4(0, 0, 0, 0);
-    uint32_t *words = reinterpret_cast<uint32_t *>(&out);
-    for (int b = 0; b < 16; b += esize) {
-        if (byte0 + b >= row_bytes) break;
-        uint32_t v;
-        if (esize == 1) v = row[byte0 + b];
-        else if (esize == 2) v = *reinterpret_cast<const uint16_t *>(row + byte0 + b);
-        else v = *reinterpret_cast<const uint32_t *>(row + byte0 + b);
-        words[b >> 2] |= v << (8 * (b & 3));
+// ---- loader warps: aligned words of rows that start anywhere --------------------------------------
+// The word at byte `off` of a row, where it may lie partly or wholly outside: elements outside are zeros and are not read.
+__device__ __noinline__ uint32_t load_edge(const uint8_t *row, long long off, long long row_bytes, int esize) {
+    uint32_t out = 0;
+    if (off >= 0 && off + 4 <= row_bytes) return __ldg(reinterpret_cast<const uint32_t *>(row + off));
+    if (esize == 4) return 0u;
+    for (int b = 0; b < 4; b += esize) {
+        if (off + b < 0 || off + b >= row_bytes) continue;
+        const uint32_t v = esize == 1 ? uint32_t(row[off + b]) : uint32_t(*reinterpret_cast<const uint16_t *>(row + off + b));
+        out |= v << (8 * b);
     }
     return out;
 }
-__device__ __forceinline__ uint4 load_chunk(const uint8_t *row, long long byte0, long long row_bytes, int esize) {
-    const uint8_t *at = row + byte0;
-    const uint32_t skew = uint32_t(reinterpret_cast<uintptr_t>(at)) & 15u;
-    if (skew == 0 && byte0 + 16 <= row_bytes) return __ldg(reinterpret_cast<const uint4 *>(at));
-    if (byte0 >= row_bytes) return make_uint4(0, 0, 0, 0);
-    // aligned words around the chunk, shifted into place; all of them inside the row
-    if (byte0 >= 4 && byte0 + 20 <= row_bytes) {
-        const uint32_t *w = reinterpret_cast<const uint32_t *>(at - (skew & 3u));
-        const uint32_t shift = 8 * (skew & 3u);
-        const uint32_t a = __ldg(w), b = __ldg(w + 1), c = __ldg(w + 2), d = __ldg(w + 3), e = __ldg(w + 4);
-        return make_uint4(__funnelshift_r(a, b, shift), __funnelshift_r(b, c, shift), __funnelshift_r(c, d, shift),
-                          __funnelshift_r(d, e, shift));
-    }
-    return load_chunk_edge(row, byte0, row_bytes, esize);
-}
 
-// x = hi + lo + (less than 2^-22 |x|), both TF32.  An infinity or NaN is all in hi.
-__device__ __forceinline__ void split_tf32(float x, float *hi, float *lo) {
-    float h = round_tf32(x);
-    if (!(fabsf(h) <= 3.402823466e38f)) h = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u);
+// x = hi + lo + (at most 2^-22 |x|) for the tensor core, which drops the low 13 bits of an operand: hi is rounded to the
+// bits it keeps, lo is what is missing plus half a step of its own.  (Whole-number arithmetic: cvt.rna.tf32 runs at an eighth of
+// its rate.)  Values that would round to infinity are cut instead; an infinity's lo is NaN.
+__device__ __forceinline__ void split_tf32(uint32_t x, uint32_t *hi, uint32_t *lo) {
+    const uint32_t h = ((x & 0x7FFFFFFFu) >= 0x7F7FF000u ? x : x + 0x1000u) & 0xFFFFE000u;
     *hi = h;
-    *lo = fabsf(h) <= 3.402823466e38f ? round_tf32(x - h) : 0.0f;
+    *lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(h)) + 0x1000u;
 }
 
 __device__ __noinline__ float act_far(float v, int act) {
@@ -567,56 +553,101 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         if (!ok && lane == 0) time_out(3);
     } else if (LOADS == kRegs && warp >= kLoadWarp0) {
         // ---------------- loader warps ----------------
-        // thread i of 256 moves 16-byte column i % 8 of rows i / 8, i / 8 + 32, ...: four of the weights, up to four of x
-        const int tid = int(threadIdx.x) - 32 * kLoadWarp0, c16 = tid & 7, r0 = tid >> 3;
+        // Each warp moves 8 rows of the weights and 8 of x: lane l the word at 4 l of a row's 128 bytes.  A row that starts off
+        // a word boundary takes the 33 words around them, shifted into place between neighbouring lanes; the last words of the
+        // 16 rows are loaded together, lane r that of row r.  The next step is asked for before this one is stored.  Where the
+        // rows start stands in shared memory, so that nothing but loads is left to do for a row (16 instructions and a branch
+        // per row took 130 cycles).  Rows that are not there repeat some row that is: their results are not stored, or made
+        // zeros by the epilogue.
+        __shared__ unsigned long long src_s[kLoaderWarps][2 * kLoaderRows];
+        constexpr int kR = kLoaderRows;
+        const int part = warp - kLoadWarp0;
+        const unsigned long long *src = src_s[part];
         const long long row_bytes = (long long)p.inner * t.esize;
         int s = 0;
         uint32_t phase = 1;
         bool ok = true;
         for (int i = tile0; i < total_tiles && ok; i += tile_step) {
             const Tile tile = find_tile(p, t, table, i, cta_channel);
-            const int wide = GATED ? 2 * p.channels : p.channels;
-            const uint8_t *src[8];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int r = weight_row<GATED>(p, tile, r0 + 32 * j);
-                const uint8_t *w = static_cast<const uint8_t *>(p.w) + ((long long)tile.group * p.w_group_stride + (long long)r * p.w_stride) * t.esize;
-                src[j] = r < wide ? w : nullptr;
-                const int c = r0 + 32 * j;
-                src[4 + j] = nullptr;
-                if (c < tile.valid) {
-                    const int at = p.rows ? p.rows[tile.row0 + c] : tile.row0 + c;
-                    if (at >= 0 && at < p.x_rows) src[4 + j] = static_cast<const uint8_t *>(p.x) + (long long)at * p.x_stride * t.esize;
+            const bool with_x = part * kR < tile.cols;
+            unsigned long long own;                          // lane r: where row r of the warp's 16 starts
+            {
+                const int r = min(weight_row<GATED>(p, tile, part * kR + (lane & (kR - 1))), (GATED ? 2 * p.channels : p.channels) - 1);
+                own = reinterpret_cast<unsigned long long>(p.w) + (tile.group * p.w_group_stride + r * p.w_stride) * t.esize;
+                if (lane >= kR && p.x_rows > 0) {
+                    const int c = tile.row0 + min(part * kR + (lane & (kR - 1)), tile.valid - 1), at = p.rows ? p.rows[c] : c;
+                    own = reinterpret_cast<unsigned long long>(p.x) + (at >= 0 && at < p.x_rows ? at : 0) * p.x_stride * t.esize;
                 }
             }
-            uint4 now[8], next[8];
-            auto fetch = [&](uint4 *v, int k) {
-                const long long byte0 = (long long)k * kRowBytes + c16 * 16;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = src[j] ? load_chunk(src[j], byte0, row_bytes, t.esize) : make_uint4(0, 0, 0, 0);
+            __syncwarp();
+            if (lane < 2 * kR) src_s[part][lane] = own;
+            __syncwarp();
+            const uint32_t own_skew = uint32_t(own) & 3u;
+            const bool skewed = __any_sync(0xffffffffu, own_skew != 0);
+            // Steps whose words are whole words of their rows (or, without skew, of the zeros behind them).
+            const auto plain = [&](int k) {
+                return (!skewed && (row_bytes & 3) == 0) || ((k > 0 || !skewed) && (k + 1LL) * kRowBytes + 4 <= row_bytes);
             };
-            fetch(now, k_begin);
-            for (int k = k_begin; k < k_end; ++k) {
-                if (k + 1 < k_end) fetch(next, k + 1);
-                ok = mbar_wait(empty0 + 8u * s, phase, nullptr);
-                ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
-                if (!ok) break;
-                uint8_t *stage = generic + size_t(s) * stage_bytes;
+            const auto fetch = [&](uint32_t *v, uint32_t &last, int k) {
+                const long long byte0 = (long long)k * kRowBytes;
+                const bool inside = byte0 + 4 * lane + 4 <= row_bytes;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int r = r0 + 32 * (j & 3);
-                    if (j >= 4 && r >= tile.cols) continue;
-                    uint8_t *dst = stage + (j < 4 ? 0 : kPlanes * kATileBytes) + sw128_offset(r, c16);
+                for (int r = 0; r < kR; ++r)
+                    v[r] = inside ? __ldg(reinterpret_cast<const uint32_t *>((src[r] & ~3ull) + byte0 + 4 * lane)) : 0u;
+                if (with_x) {
+#pragma unroll
+                    for (int r = kR; r < 2 * kR; ++r)
+                        v[r] = inside ? __ldg(reinterpret_cast<const uint32_t *>((src[r] & ~3ull) + byte0 + 4 * lane)) : 0u;
+                }
+                if (skewed) last = own_skew ? __ldg(reinterpret_cast<const uint32_t *>((own & ~3ull) + byte0 + kRowBytes)) : 0u;
+            };
+            uint32_t now[2 * kR], next[2 * kR], now_last = 0, next_last = 0;
+#pragma unroll
+            for (int r = 0; r < 2 * kR; ++r) now[r] = next[r] = 0;
+            if (plain(k_begin)) fetch(now, now_last, k_begin);
+            for (int k = k_begin; k < k_end; ++k) {
+                if (k + 1 < k_end && plain(k + 1)) fetch(next, next_last, k + 1);
+                ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
+                if (!ok) break;
+                uint8_t *stage = generic + size_t(s) * stage_bytes + part * kR * kRowBytes + (lane & 3) * 4;
+                const auto store = [&](int r, uint32_t word) {
+                    uint8_t *dst = stage + (r < kR ? 0 : kPlanes * kATileBytes) + sw128_offset(r & (kR - 1), lane >> 2);
                     if (KIND != kX3) {
-                        *reinterpret_cast<uint4 *>(dst) = now[j];
+                        *reinterpret_cast<uint32_t *>(dst) = word;
                     } else {
-                        float4 hi, lo;
-                        split_tf32(__uint_as_float(now[j].x), &hi.x, &lo.x);
-                        split_tf32(__uint_as_float(now[j].y), &hi.y, &lo.y);
-                        split_tf32(__uint_as_float(now[j].z), &hi.z, &lo.z);
-                        split_tf32(__uint_as_float(now[j].w), &hi.w, &lo.w);
-                        *reinterpret_cast<float4 *>(dst) = hi;
-                        *reinterpret_cast<float4 *>(dst + (j < 4 ? uint32_t(kATileBytes) : b_bytes)) = lo;
+                        uint32_t hi, lo;
+                        split_tf32(word, &hi, &lo);
+                        *reinterpret_cast<uint32_t *>(dst) = hi;
+                        *reinterpret_cast<uint32_t *>(dst + (r < kR ? uint32_t(kATileBytes) : b_bytes)) = lo;
+                    }
+                };
+                const auto shifted = [&](int r, uint32_t word, uint32_t last) {
+                    const uint32_t beside = __shfl_down_sync(0xffffffffu, word, 1);
+                    return __funnelshift_r(word, lane == 31 ? last : beside, 8 * (uint32_t(src[r]) & 3u));
+                };
+                if (!plain(k)) {
+                    const long long byte0 = (long long)k * kRowBytes;
+#pragma unroll 1
+                    for (int r = 0; r < (with_x ? 2 * kR : kR); ++r) {
+                        const uint8_t *row = reinterpret_cast<const uint8_t *>(src[r]);
+                        const int skew = int(src[r] & 3ull);
+                        const uint32_t word = load_edge(row, byte0 + 4 * lane - skew, row_bytes, t.esize);
+                        const uint32_t last = lane == 31 && skew ? load_edge(row, byte0 + kRowBytes - skew, row_bytes, t.esize) : 0u;
+                        store(r, shifted(r, word, last));
+                    }
+                } else if (!skewed) {
+#pragma unroll
+                    for (int r = 0; r < kR; ++r) store(r, now[r]);
+                    if (with_x) {
+#pragma unroll
+                        for (int r = kR; r < 2 * kR; ++r) store(r, now[r]);
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < kR; ++r) store(r, shifted(r, now[r], __shfl_sync(0xffffffffu, now_last, r)));
+                    if (with_x) {
+#pragma unroll
+                        for (int r = kR; r < 2 * kR; ++r) store(r, shifted(r, now[r], __shfl_sync(0xffffffffu, now_last, r)));
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -624,7 +655,8 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 if (lane == 0) mbar_arrive(full0 + 8u * s);
                 if (++s == t.stages) { s = 0; phase ^= 1u; }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) now[j] = next[j];
+                for (int r = 0; r < 2 * kR; ++r) now[r] = next[r];
+                now_last = next_last;
             }
         }
         if (!ok && lane == 0) time_out(6);
@@ -707,7 +739,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             o.vectors = ((reinterpret_cast<uintptr_t>(o.first) | uintptr_t(o.row_bytes)) & 15) == 0 && o.channels == kWidth;
             const float *row_scale = row_scale_s[round & 1];
             const uint32_t *live = live_s[round & 1];
-            if (p.row_scale || LOADS == kGather) {
+            if (p.row_scale || (LOADS != kTma && p.rows)) {
                 for (int c = tid; c < max(t.tn, 32); c += 32 * kEpilogueWarps) {              // whole warps
                     const int src = c >= tile.valid ? 0 : p.rows ? p.rows[tile.row0 + c] : tile.row0 + c;
                     const bool known = src >= 0 && src < p.x_rows;
@@ -810,7 +842,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 #pragma unroll
                     for (int c = 0; c < kTurnCols; ++c) v[c] = float(__float_as_int(v[c]));
                 }
-                if (LOADS == kGather) {                               // a row that is none was loaded as some other one
+                if (LOADS != kTma && p.rows) {                        // a row that is none was loaded as some other one
                     const uint32_t mask = __funnelshift_r(live[c0 >> 5], live[min(c0 >> 5, 6) + 1], c0);
                     if ((mask & 0xffffu) != 0xffffu) {
 #pragma unroll
