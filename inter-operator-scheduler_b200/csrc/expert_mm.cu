@@ -37,17 +37,20 @@ namespace ios {
 namespace {
 
 enum Kind { kF16 = 0, kI8 = 1, kX3 = 2 };       // instruction: 16-bit floats, 8-bit integers, three TF32 products
-enum Loads { kTma = 0, kGather = 1, kRegs = 2 };  // operands by TMA / gathered rows by cp.async warps / all through registers
+enum Loads { kTma = 0, kGather = 1, kRegs = 2 };  // operands by TMA / rows gathered by TMA, four at a time / all through registers
 
 constexpr int kGatherWarps = 8, kLoaderWarps = 16;
 constexpr int kLoaderRows = 128 / kLoaderWarps; // rows of each operand that a loader warp moves
 constexpr int kBoxRows = 64;                    // rows of x per TMA load, in wide tiles
 constexpr int kNarrowCols = 32;                 // tiles up to here gather a step's rows with one warp
 constexpr int kMaxThreads = 768;
-// Two epilogue warps per lane quarter share a tile's columns; one beside gathering or loader warps, which need the registers.
-__host__ __device__ constexpr int epilogue_warps(int loads) { return loads != kTma ? 4 : 8; }
-__host__ __device__ constexpr int threads_of(int loads) {
-    return 32 * (4 + epilogue_warps(loads) + (loads == kTma ? 0 : loads == kGather ? kGatherWarps : kLoaderWarps));
+constexpr int kSplitWarps = 8;                  // float32 by TMA: warps that split the operands where they have landed
+// Two epilogue warps per lane quarter share a tile's columns; one beside gathering, loading or splitting warps, which need
+// the registers.
+__host__ __device__ constexpr int epilogue_warps(int kind, int loads) { return loads == kTma && kind != kX3 ? 8 : 4; }
+__host__ __device__ constexpr int threads_of(int kind, int loads) {
+    return 32 * (4 + epilogue_warps(kind, loads) + (loads == kTma ? 0 : loads == kGather ? kGatherWarps : kLoaderWarps) +
+                 (kind == kX3 && loads != kRegs ? kSplitWarps : 0));
 }
 constexpr int kLoaderCols = 128;                // widest tile of the loader warps (their registers hold a step)
 constexpr int kTurnCols = 16;                   // columns an epilogue warp turns round at a time: few, because a small
@@ -56,7 +59,7 @@ constexpr int kTurnBytes = kTurnCols * 32 * 4;  // ... in this much shared memor
 constexpr int kChunkSteps = 4;                  // float32: K steps per partial sum
 constexpr int kMaxStages = 12;
 constexpr int kMaxGroupTiles = INT_MAX / kMaxExperts - 1;    // tiles of a group: their sum over all groups fits an int
-constexpr int kBarBytes = 2 * kMaxStages * 8 + 48;    // mbarriers: two per stage, six more
+constexpr int kBarBytes = 3 * kMaxStages * 8 + 48;    // mbarriers: three per stage, six more
 constexpr size_t kSmemLimit = 227 * 1024, kStaticBytes = 4608;    // ... of which the kernel's static arrays may take
 
 __device__ int g_expert_error;                  // set by a wait that ran out, read by expert_mm_status
@@ -391,11 +394,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float *v) {
 }
 
 template <int KIND, int LOADS, bool PAIR, bool GATED>
-__global__ void __launch_bounds__(threads_of(LOADS), 1)
+__global__ void __launch_bounds__(threads_of(KIND, LOADS), 1)
 expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const GroupedParams p,
                  const MmGeom t) {
     constexpr int kPlanes = KIND == kX3 ? 2 : 1;
-    constexpr int kEpilogueWarps = epilogue_warps(LOADS), kLoadWarp0 = 4 + kEpilogueWarps;
+    constexpr int kEpilogueWarps = epilogue_warps(KIND, LOADS), kLoadWarp0 = 4 + kEpilogueWarps;
+    constexpr bool kSplit = KIND == kX3 && LOADS != kRegs;
+    constexpr int kSplitWarp0 = kLoadWarp0 + (LOADS == kGather ? kGatherWarps : 0);
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(16) float row_scale_s[2][256];
     __shared__ uint32_t live_s[2][8];                            // one bit per column: its row exists
@@ -407,7 +412,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     const uint32_t stage_bytes = kPlanes * (kATileBytes + b_bytes);
     const uint32_t full0 = base + t.bar_off, empty0 = full0 + 8u * t.stages;
     const uint32_t acc_full0 = empty0 + 8u * t.stages, acc_empty0 = acc_full0 + 16u;
-    const uint32_t recv_full = acc_empty0 + 16u, recv_free = recv_full + 8u;
+    const uint32_t recv_full = acc_empty0 + 16u, recv_free = recv_full + 8u, ready0 = recv_free + 8u;
     const Table table = {reinterpret_cast<int *>(generic + t.table_off), reinterpret_cast<int *>(generic + t.table_off) + p.groups + 1};
 
     if (LOADS != kRegs && threadIdx.x == 32) {
@@ -418,6 +423,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         for (int s = 0; s < t.stages; ++s) {
             mbar_init(full0 + 8u * s, LOADS == kRegs ? kLoaderWarps : 1);
             mbar_init(empty0 + 8u * s, 1);
+            mbar_init(ready0 + 8u * s, kSplitWarps);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(acc_full0 + 8u * a, 1);
@@ -438,7 +444,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         }
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    build_table(p, t, table, threads_of(LOADS));
+    build_table(p, t, table, threads_of(KIND, LOADS));
     tc_fence_before();
     __syncthreads();
     if (PAIR || t.cluster > 1) cluster_sync_all();
@@ -510,19 +516,21 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             for (int k = k_begin; k < k_end; ++k) {
                 ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
                 if (!ok) break;
-                const uint32_t dst = base + uint32_t(s) * stage_bytes + kATileBytes, bar = full_at + 8u * s;
+                const uint32_t dst = base + uint32_t(s) * stage_bytes + kPlanes * kATileBytes, bar = full_at + 8u * s;
                 for (int b = 0; b < loads; ++b)
                     load_2d<PAIR>(elected, dst + uint32_t(b * t.box_rows) * kRowBytes, &map_x, bar, k * k_elems, tile.row0 + col0 + b * t.box_rows);
                 if (++s == t.stages) { s = 0; phase ^= 1u; }
             }
         }
         if (!ok && lane == 0) time_out(2);
-    } else if (LOADS == kGather && warp >= kLoadWarp0) {
+    } else if (LOADS == kGather && warp >= kLoadWarp0 && warp < kLoadWarp0 + kGatherWarps) {
         // ---------------- gathered rows, in groups of four: a group per lane ----------------
         // Wide tiles: the groups of every step are dealt to all warps.  Narrow tiles, a few groups per step: every warp loads
-        // all groups of its turn's steps.
+        // all groups of its turn's steps -- and there are no more turns than stages, or a warp's wait by parity could take the
+        // stage's last round but one for its last.
         const int part = warp - kLoadWarp0;
         const bool narrow = t.tn <= kNarrowCols;
+        const int turns = t.stages >= kGatherWarps ? kGatherWarps : kGatherWarps / 2;
         const int group = narrow ? lane : lane * kGatherWarps + part;
         int s = 0, step = 0;
         uint32_t phase = 1;
@@ -539,11 +547,11 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             }
             const int4 src = make_int4(at[0], at[1], at[2], at[3]);
             for (int k = k_begin; k < k_end; ++k, ++step) {
-                if (!narrow || (step & (kGatherWarps - 1)) == part) {
+                if (!narrow || (step & (turns - 1)) == part) {
                     ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
                     if (!ok) break;
                     if (loads)
-                        load_rows4<PAIR>(1u, base + uint32_t(s) * stage_bytes + kATileBytes + uint32_t(group) * 4u * kRowBytes, &map_x,
+                        load_rows4<PAIR>(1u, base + uint32_t(s) * stage_bytes + kPlanes * kATileBytes + uint32_t(group) * 4u * kRowBytes, &map_x,
                                          full_at + 8u * s, k * k_elems, src);
                     __syncwarp();
                 }
@@ -660,6 +668,40 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             }
         }
         if (!ok && lane == 0) time_out(6);
+    } else if (kSplit && warp >= kSplitWarp0) {
+        // ---------------- landed float32 operands into two TF32 numbers each, the larger in place ----------------
+        const int tid = int(threadIdx.x) - 32 * kSplitWarp0;
+        int s = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int i = tile0; i < total_tiles && ok; i += tile_step) {
+            const Tile tile = find_tile(p, t, table, i, cta_channel);
+            for (int k = k_begin; k < k_end; ++k) {
+                ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
+                if (!ok) break;
+                uint8_t *stage = generic + size_t(s) * stage_bytes;
+                const auto split = [&](uint8_t *at, uint32_t apart) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(at);
+                    uint4 hi, lo;
+                    split_tf32(x.x, &hi.x, &lo.x);
+                    split_tf32(x.y, &hi.y, &lo.y);
+                    split_tf32(x.z, &hi.z, &lo.z);
+                    split_tf32(x.w, &hi.w, &lo.w);
+                    *reinterpret_cast<uint4 *>(at) = hi;
+                    *reinterpret_cast<uint4 *>(at + apart) = lo;
+                };
+                constexpr int kThreads = 32 * kSplitWarps;
+#pragma unroll
+                for (int q = 0; q < kATileBytes / 16 / kThreads; ++q) split(stage + (q * kThreads + tid) * 16, kATileBytes);
+#pragma unroll 4
+                for (int v = tid; v < tile.cols * (kRowBytes / 16); v += kThreads) split(stage + 2 * kATileBytes + v * 16, b_bytes);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(ready0 + 8u * s);
+                if (++s == t.stages) { s = 0; phase ^= 1u; }
+            }
+        }
+        if (!ok && lane == 0) time_out(7);
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
         if (!PAIR || rank == 0) {
@@ -684,7 +726,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                         ok = wait<PAIR>(acc_empty0 + 8u * a, ((uint32_t(turn) >> 1) & 1u) ^ 1u);
                         acc = 0;
                     }
-                    if (ok) ok = wait<PAIR>(full0 + 8u * s, phase);
+                    if (ok) ok = wait<PAIR>((kSplit ? ready0 : full0) + 8u * s, phase);
                     ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
                     if (!ok) break;
                     tc_fence_after();
@@ -956,7 +998,7 @@ int ceil_div(long long a, long long b) { return int((a + b - 1) / b); }
 bool tma_able(const GroupedParams &p) {
     const int esize = elem_size(p.type);
     const long long wide = p.gated ? 2 * p.channels : p.channels, group_bytes = p.w_group_stride * esize;
-    return p.type != Elem::F32 && p.x_rows > 0 && tma_rows(p.x, p.x_stride, p.inner, esize) && tma_rows(p.w, p.w_stride, p.inner, esize) &&
+    return p.x_rows > 0 && tma_rows(p.x, p.x_stride, p.inner, esize) && tma_rows(p.w, p.w_stride, p.inner, esize) &&
            (p.groups == 1 || (group_bytes % 16 == 0 && p.w_group_stride >= wide * p.w_stride && group_bytes < (1LL << 40)));
 }
 
@@ -977,7 +1019,7 @@ int choose(const GroupedParams &p, int sm_count, bool tma, MmGeom *t, bool *pair
     t->n_tiles = ceil_div(p.channels, t->tile_channels);
     t->k_steps = ceil_div((long long)p.inner * esize, kRowBytes);
     const int busy = std::min(p.groups, p.total);
-    t->tn = columns_for(p, tma ? 256 : kLoaderCols);
+    t->tn = columns_for(p, tma && p.type != Elem::F32 ? 256 : kLoaderCols);
     auto tiles = [&]() { return (long long)t->n_tiles * std::max<long long>(busy, ceil_div(p.total, t->tn)); };
     if (tiles() < sm_count && t->tn > 128) t->tn = 128;
     // K split: as long as it fills SMs that would idle and leaves every CTA two K steps
@@ -1001,6 +1043,8 @@ int choose(const GroupedParams &p, int sm_count, bool tma, MmGeom *t, bool *pair
     const size_t turn = 8 * kTurnBytes;
     const size_t fixed = 1024 + recv + turn + table + kBarBytes + kStaticBytes;
     t->stages = int(std::min<size_t>(kMaxStages, (kSmemLimit - fixed) / stage));
+    static_assert((kSmemLimit - 1024 - kNarrowCols * kTileM * 4 - 8 * kTurnBytes - 2 * (kMaxExperts + 4) * 4 - kBarBytes - kStaticBytes) /
+                  (2 * (kATileBytes + kNarrowCols * kRowBytes)) >= kGatherWarps / 2, "narrow tiles gather in that many turns");
     t->recv_off = int(t->stages * stage);
     t->turn_off = int(t->recv_off + recv);
     t->table_off = int(t->turn_off + turn);
@@ -1025,7 +1069,7 @@ cudaError_t run(const GroupedParams &p, const MmGeom &t, int ctas, const CUtenso
     }
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(unsigned(ctas));
-    config.blockDim = dim3(threads_of(LOADS));
+    config.blockDim = dim3(threads_of(KIND, LOADS));
     config.dynamicSmemBytes = size_t(t.bar_off + kBarBytes + 1024);
     config.stream = stream;
     cudaLaunchAttribute attributes[2] = {};
@@ -1082,7 +1126,11 @@ cudaError_t launch_grouped(const GroupedParams &given, cudaStream_t stream) {
 #define IOS_RUN(KIND, LOADS, PAIR)                                                                     \
     return p.gated ? run<KIND, LOADS, PAIR, true>(p, t, ctas, map_w, map_x, stream)                      \
                    : run<KIND, LOADS, PAIR, false>(p, t, ctas, map_w, map_x, stream)
-    if (p.type == Elem::F32) IOS_RUN(kX3, kRegs, false);
+    if (p.type == Elem::F32) {
+        if (!tma) IOS_RUN(kX3, kRegs, false);
+        if (p.rows) IOS_RUN(kX3, kGather, false);
+        IOS_RUN(kX3, kTma, false);
+    }
     if (p.type == Elem::S8) {
         if (!tma) IOS_RUN(kI8, kRegs, false);
         if (pair && p.rows) IOS_RUN(kI8, kGather, true);

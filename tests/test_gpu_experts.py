@@ -216,7 +216,7 @@ def test_grouped_product(dtype, total, groups, inner, channels):
 
 
 @ALL_TYPES
-@pytest.mark.parametrize('total,groups,inner,channels', [(5, 8, 256, 96), (130, 6, 200, 100), (1100, 4, 576, 272), (900, 3, 129, 40)])
+@pytest.mark.parametrize('total,groups,inner,channels', [(5, 8, 256, 96), (8, 8, 2048, 512), (30, 3, 1000, 64), (130, 6, 200, 100), (1100, 4, 576, 272), (900, 3, 129, 40)])
 def test_grouped_product_gathered_gated(dtype, total, groups, inner, channels):
     run_grouped(total, groups, inner, channels, dtype, gather=True, gated=True, act='silu', bias=True)
 
