@@ -15,8 +15,8 @@
 //   warps (tile::gather4 moves 512 bytes per instruction and took 68 cycles for each: 1480 us where this takes @GATHER@ us, 4096
 //   tokens x 8 of 64 experts, gated, 2048 -> 1280).  Anything else goes through registers of eight loader warps.
 // * float32: every operand is split into two TF32 numbers on its way into shared memory (loader warps); three products
-//   a_hi b_hi + a_hi b_lo + a_lo b_hi.  The tensor core truncates where it adds, so the sum over more than 128 elements is
-//   formed in registers, rounded to nearest, from partial sums over 128.
+//   a_hi b_hi + a_hi b_lo + a_lo b_hi.  The tensor core truncates where it adds, so the sum over more than 64 elements is
+//   formed in registers, rounded to nearest, from partial sums over 64.
 // * gated: 16 rows of the gate half and the 16 rows of the same channels of the other half alternate in the tile, so that
 //   a lane and the lane 16 further on hold the two factors of one result.
 //
@@ -56,7 +56,7 @@ constexpr int kLoaderCols = 128;                // widest tile of the loader war
 constexpr int kTurnCols = 16;                   // columns an epilogue warp turns round at a time: few, because a small
                                                 // product runs this code once, and cold code costs more than it does
 constexpr int kTurnBytes = kTurnCols * 32 * 4;  // ... in this much shared memory
-constexpr int kChunkSteps = 4;                  // float32: K steps per partial sum
+constexpr int kChunkSteps = 2;                  // float32: K steps per partial sum
 constexpr int kMaxStages = 12;
 constexpr int kMaxGroupTiles = INT_MAX / kMaxExperts - 1;    // tiles of a group: their sum over all groups fits an int
 constexpr int kBarBytes = 3 * kMaxStages * 8 + 48;    // mbarriers: three per stage, six more
@@ -369,6 +369,35 @@ template <bool GATED>
 __device__ __forceinline__ void write_columns(const Out &o, Elem type, const float *v, int c0, int lane) {
     constexpr int kWidth = GATED ? 16 : 32;                           // channels of the warp
     const int at = GATED ? (lane >> 4) * 16 + (lane & 15) : lane;
+    if (!GATED && type != Elem::F32 && o.vectors) {
+        // two columns to a word, [column pair][channel]; lane l takes eight channels of pair l / 4 apart again
+        uint32_t *turn = reinterpret_cast<uint32_t *>(o.turn);
+        if (type == Elem::BF16) {
+#pragma unroll
+            for (int c = 0; c < kTurnCols; c += 2) {
+                const __nv_bfloat162 two = __floats2bfloat162_rn(v[c], v[c + 1]);
+                turn[c * 16 + lane] = *reinterpret_cast<const uint32_t *>(&two);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < kTurnCols; c += 2) {
+                const __half2 two = __floats2half2_rn(v[c], v[c + 1]);
+                turn[c * 16 + lane] = *reinterpret_cast<const uint32_t *>(&two);
+            }
+        }
+        __syncwarp();
+        const uint4 a = reinterpret_cast<const uint4 *>(turn)[lane * 2], b = reinterpret_cast<const uint4 *>(turn)[lane * 2 + 1];
+        const int row = c0 + (lane >> 2) * 2;
+        uint8_t *to = o.first + row * o.row_bytes + (lane & 3) * 16;
+        if (row < o.rows)
+            *reinterpret_cast<uint4 *>(to) = make_uint4(__byte_perm(a.x, a.y, 0x5410), __byte_perm(a.z, a.w, 0x5410),
+                                                        __byte_perm(b.x, b.y, 0x5410), __byte_perm(b.z, b.w, 0x5410));
+        if (row + 1 < o.rows)
+            *reinterpret_cast<uint4 *>(to + o.row_bytes) = make_uint4(__byte_perm(a.x, a.y, 0x7632), __byte_perm(a.z, a.w, 0x7632),
+                                                                      __byte_perm(b.x, b.y, 0x7632), __byte_perm(b.z, b.w, 0x7632));
+        __syncwarp();
+        return;
+    }
     if (type == Elem::F32) {
 #pragma unroll
         for (int c = 0; c < (GATED ? kTurnCols / 2 : kTurnCols); ++c) reinterpret_cast<float *>(o.turn)[c * 32 + at] = v[c];
@@ -385,6 +414,20 @@ __device__ __forceinline__ void write_columns(const Out &o, Elem type, const flo
     __syncwarp();
 }
 
+// 16 columns on their way into registers, which may be looked at after tmem_arrived
+__device__ __forceinline__ void tmem_ask16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_arrived(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :: "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float *v) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
@@ -858,11 +901,17 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 o.rows = min(tile.valid, rank * per + (share == 0 ? mine : per));
             }
             // ---- scales, bias, activation, store: 16 columns at a time (those behind the last are not used) ----
+            uint32_t ahead[kTurnCols];
+            if (t.cluster == 1 && from < o.rows) tmem_ask16(sums + from, ahead);
 #pragma unroll 1
             for (int c0 = from; c0 < o.rows; c0 += step) {
                 float v[kTurnCols];
                 if (t.cluster == 1) {
-                    tmem_ld16(sums + c0, v);
+                    tmem_arrived(ahead);
+#pragma unroll
+                    for (int c = 0; c < kTurnCols; ++c) v[c] = __uint_as_float(ahead[c]);
+                    if (c0 + step < o.rows) tmem_ask16(sums + c0 + step, ahead);
+                    else release();
                 } else {
                     // the partial sums of all ranks, in rank order
                     const float *part = recv_generic + (c0 - rank * per) * kTileM + lane_row;
@@ -893,9 +942,16 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                     }
                 }
                 if (p.row_scale) {
+                    if (t.cluster == 1) {
 #pragma unroll
-                    for (int c = 0; c < kTurnCols; ++c)
-                        if (c0 + c < t.tn) v[c] *= row_scale[c0 + c];
+                        for (int c = 0; c < kTurnCols; c += 4) {
+                            const float4 f = *reinterpret_cast<const float4 *>(row_scale + c0 + c);
+                            v[c] *= f.x; v[c + 1] *= f.y; v[c + 2] *= f.z; v[c + 3] *= f.w;
+                        }
+                    } else {                                          // a rank's columns start at any even one
+#pragma unroll
+                        for (int c = 0; c < kTurnCols; ++c) v[c] *= row_scale[c0 + c];
+                    }
                 }
 #pragma unroll
                 for (int c = 0; c < kTurnCols; ++c) v[c] = v[c] * channel_scale + bias;
@@ -917,7 +973,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 write_columns<GATED>(o, p.out_type, v, c0, lane);
             }
             if (t.cluster == 1) {
-                release();
+                if (from >= o.rows) release();
             } else {
                 __syncwarp();
                 if (lane < t.cluster) mbar_arrive_cluster(cluster_map(recv_free, uint32_t(lane)));

@@ -161,15 +161,16 @@ def route_experts(logits, k, renormalize=True):
     pairs, need = tokens * k, _route_workspace(tokens, experts, k)
     # one allocation for everything: experts, slots, gates, rows, offsets, workspace
     whole = logits.new_empty(4 * pairs + experts + 1 + (need + 3) // 4, dtype=torch.int32)
-    chosen, slots, gates, rows, offsets, work = whole.split_with_sizes(
-        (pairs, pairs, pairs, pairs, experts + 1, (need + 3) // 4))
-    gates = gates.view(torch.float32)
+    square, apart = (tokens, k), (k, 1)
+    chosen, slots = whole.as_strided(square, apart, 0), whole.as_strided(square, apart, pairs)
+    gates = whole.as_strided(square, apart, 2 * pairs).view(torch.float32)
+    rows, offsets = whole.as_strided((pairs,), (1,), 3 * pairs), whole.as_strided((experts + 1,), (1,), 4 * pairs)
     base = whole.data_ptr()
     _check(_lib.ios_route_experts(
         logits.data_ptr(), code, tokens, experts, logits.stride(0), k, 1 if renormalize else 0, base, base + 8 * pairs,
-        base + 16 * pairs, base + 12 * pairs, base + 4 * pairs, work.data_ptr() if need else None, need,
+        base + 16 * pairs, base + 12 * pairs, base + 4 * pairs, base + 4 * (4 * pairs + experts + 1) if need else None, need,
         _raw_stream(logits.get_device())))
-    return Routing(chosen.view(tokens, k), gates.view(tokens, k), offsets, rows, slots.view(tokens, k))
+    return Routing(chosen, gates, offsets, rows, slots)
 
 
 def grouped_matmul(x, weight, offsets, rows=None, bias=None, act='identity', gated=False, row_scale=None,
