@@ -73,6 +73,37 @@ __device__ __forceinline__ uint32_t logit_key(float v) {
 __device__ __forceinline__ float key_logit(uint32_t key) {
     return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
 }
+// The same in 16 bits
+__device__ __forceinline__ uint32_t ordered16(uint32_t b, bool able) {
+    if (b == 0x8000u) b = 0;
+    return !able ? 0u : (b & 0x8000u) ? (~b & 0xFFFFu) : (b | 0x8000u);
+}
+__device__ __forceinline__ uint32_t unordered16(uint32_t key) { return (key & 0x8000u) ? (key & 0x7FFFu) : (~key & 0xFFFFu); }
+
+// What the picks compare: for 16-bit logits the key above the complement of the expert's index, so that one reduction finds
+// the largest logit and the lowest index that has it; for float32 the key alone.
+template <class T> struct Rank;
+template <> struct Rank<float> {
+    static constexpr bool kWithIndex = false;
+    static __device__ __forceinline__ uint32_t of(float v, int) { return logit_key(v); }
+    static __device__ __forceinline__ float logit(uint32_t rank) { return key_logit(rank); }
+};
+template <> struct Rank<__half> {
+    static constexpr bool kWithIndex = true;
+    static __device__ __forceinline__ uint32_t of(__half v, int e) {
+        const uint32_t key = ordered16(__half_as_ushort(v), __half2float(v) > -INFINITY);
+        return key ? key << 16 | (0xFFFFu - uint32_t(e)) : 0u;
+    }
+    static __device__ __forceinline__ float logit(uint32_t rank) { return __half2float(__ushort_as_half(uint16_t(unordered16(rank >> 16)))); }
+};
+template <> struct Rank<__nv_bfloat16> {
+    static constexpr bool kWithIndex = true;
+    static __device__ __forceinline__ uint32_t of(__nv_bfloat16 v, int e) {
+        const uint32_t key = ordered16(__bfloat16_as_ushort(v), __bfloat162float(v) > -INFINITY);
+        return key ? key << 16 | (0xFFFFu - uint32_t(e)) : 0u;
+    }
+    static __device__ __forceinline__ float logit(uint32_t rank) { return __uint_as_float(unordered16(rank >> 16) << 16); }
+};
 
 // exp(v - top), with +inf logits sharing the weight among themselves instead of producing NaN
 __device__ __forceinline__ float softmax_term(float v, float top) { return v == top ? 1.0f : expf(v - top); }
@@ -80,61 +111,72 @@ __device__ __forceinline__ float softmax_term(float v, float top) { return v == 
 constexpr int kRouteThreads = 1024;       // 32 warps hide one another's reductions; a call of a few tokens takes 256 threads
 constexpr int kRoutePairs = 8192;         // pairs that a block plans in shared memory
 
-// The k best experts of tokens [first, last): one warp per token, logit e in register e / 32 of lane e % 32.
-// Each pick takes two warp reductions (largest key, then its lowest index) and drops the winner.
+// The k best experts of tokens [first, last): one warp per token, logit e in register e / 32 of lane e % 32; the next
+// token's logits are on their way meanwhile.  Each pick takes one or two warp reductions and drops the winner.
 template <class T, int PER>
 __device__ __forceinline__ void pick_experts(const RouteParams &p, int first, int last, int *chosen) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    for (int t = first + warp; t < last; t += warps) {
+    T ahead[PER];
+    const auto ask = [&](int t) {
         const T *row = static_cast<const T *>(p.logits) + (long long)t * p.stride;
-        uint32_t key[PER];
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int e = i * 32 + lane;
-            key[i] = e < p.experts ? logit_key(to_float(row[e])) : 0u;
-        }
-        uint32_t mine = 0;
-        int mine_at = 0;
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-            if (key[i] > mine) { mine = key[i]; mine_at = i; }
+            if (i * 32 + lane < p.experts) ahead[i] = row[i * 32 + lane];
+    };
+    if (first + warp < last) ask(first + warp);
+    for (int t = first + warp; t < last; t += warps) {
+        uint32_t rank[PER], mine = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            rank[i] = i * 32 + lane < p.experts ? Rank<T>::of(ahead[i], i * 32 + lane) : 0u;
+            mine = max(mine, rank[i]);
+        }
+        if (t + warps < last) ask(t + warps);
         const uint32_t top = __reduce_max_sync(0xffffffffu, mine);
-        const float top_logit = key_logit(top);
+        const float top_logit = Rank<T>::logit(top);
         float sum = 0.0f;
         if (!p.renormalize && top != 0) {
 #pragma unroll
             for (int i = 0; i < PER; ++i)
-                if (key[i]) sum += softmax_term(key_logit(key[i]), top_logit);
+                if (rank[i]) sum += softmax_term(Rank<T>::logit(rank[i]), top_logit);
 #pragma unroll
             for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
         }
         int my_expert = -1;          // lane j keeps pick j
-        float my_weight = 0.0f;
+        uint32_t my_rank = 0;
         for (int j = 0; j < p.k; ++j) {
-            const uint32_t best = __reduce_max_sync(0xffffffffu, mine);
+            const uint32_t best = j == 0 ? top : __reduce_max_sync(0xffffffffu, mine);
             if (best == 0) break;                                                // no expert left: the rest stays -1
-            const uint32_t at = __reduce_min_sync(0xffffffffu, mine == best ? uint32_t(mine_at * 32 + lane) : 0xffffffffu);
+            uint32_t at;
+            if (Rank<T>::kWithIndex) {
+                at = 0xFFFFu - (best & 0xFFFFu);
+            } else {
+                uint32_t lowest = 0xffffffffu;
+#pragma unroll
+                for (int i = PER - 1; i >= 0; --i)
+                    if (rank[i] == best) lowest = uint32_t(i * 32 + lane);
+                at = __reduce_min_sync(0xffffffffu, lowest);
+            }
             if (lane == j) {
                 my_expert = int(at);
-                my_weight = softmax_term(key_logit(best), top_logit);
+                my_rank = best;
             }
-            if (lane == int(at & 31u)) {
-                mine = 0;
+            mine = 0;
 #pragma unroll
-                for (int i = 0; i < PER; ++i) {
-                    if (i == int(at >> 5)) key[i] = 0;
-                    if (key[i] > mine) { mine = key[i]; mine_at = i; }
-                }
+            for (int i = 0; i < PER; ++i) {
+                if (i * 32 + lane == int(at)) rank[i] = 0;
+                mine = max(mine, rank[i]);
             }
         }
+        const float weight = my_expert >= 0 ? softmax_term(Rank<T>::logit(my_rank), top_logit) : 0.0f;
         if (p.renormalize) {
-            sum = my_weight;
+            sum = weight;
 #pragma unroll
             for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
         }
         if (lane < p.k) {
             p.chosen[(long long)t * p.k + lane] = my_expert;
-            p.gates[(long long)t * p.k + lane] = my_expert >= 0 ? my_weight / sum : 0.0f;
+            p.gates[(long long)t * p.k + lane] = my_expert >= 0 ? weight / sum : 0.0f;
             chosen[(t - first) * p.k + lane] = my_expert;
         }
     }
