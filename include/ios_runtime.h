@@ -236,7 +236,7 @@ IOS_API int ios_static_scratch_status(void *cuda_stream);
  * cuda_stream (a cudaStream_t of that device, NULL = default stream) and NOT synchronised; nothing is allocated or
  * kept between calls, so calls may overlap and may be captured into graphs.  Outputs must not overlap inputs.
  * Sums, softmax terms and scales are float32 (8-bit products: int32).  Everything runs in a fixed order: the same
- * inputs give the same bits.  Zero rows are no error. */
+ * inputs give the same bits.  Zero rows are no error; more than 2^30 rows or pairs are one (IOS_ERR_LIMIT). */
 enum { IOS_F32 = 0, IOS_F16 = 1, IOS_BF16 = 2, IOS_S8 = 3 };   /* element types */
 
 /* Waits for cuda_stream, then tells whether a bounded wait inside a product on `device` ran out since the last call of
@@ -267,8 +267,10 @@ IOS_API int ios_route_experts(const void *logits, int type, int tokens, int expe
  * IOS_F16, IOS_BF16; IOS_S8: inner < 131072), y[total_rows, channels] is IOS_F32 / IOS_F16 / IOS_BF16.  row_scale[x_rows],
  * channel_scale and bias (groups x channels or 2 * channels, dense) are float32 or NULL.  act: 0 identity, 1 relu,
  * 2 sigmoid, 3 tanh, 4 silu.  offsets[groups + 1] is read on the device and must not decrease; it may stop short of
- * total_rows, rows of y behind the last group are left as they were.  An entry of rows outside [0, x_rows) reads as a row
- * of zeros.  groups <= 1024. */
+ * total_rows, rows of y before the first group and behind the last are left as they were.  An entry of rows outside
+ * [0, x_rows) reads as a row of zeros.  groups <= 1024.  Any strides and alignments are taken; rows of x and w that start on
+ * 16-byte boundaries (and groups of w that do not overlap) are several times faster than others.  IOS_F32: a sum that an
+ * infinity enters may come out as NaN. */
 IOS_API int ios_grouped_matmul(const void *x, int type, long long x_rows, long long x_stride, const void *w, int groups,
                                int channels, int inner, long long w_stride, long long w_group_stride, const int *offsets,
                                const int *rows, int total_rows, const float *row_scale, const float *channel_scale,

@@ -27,6 +27,8 @@ int fail(int status, const char *format, ...) {
     return status;
 }
 
+constexpr int kMaxRows = 1 << 30;       // row numbers and what is added to them stay inside an int
+
 bool float_type(int t) { return t == IOS_F32 || t == IOS_F16 || t == IOS_BF16; }
 
 // Makes the device that owns `out` current until the end of the call.
@@ -86,7 +88,7 @@ int check_grouped(const GroupedParams &p, const char *what) {
     if (p.y_stride < p.channels) return fail(IOS_ERR_ARGUMENT, "%s: rows of y overlap (stride %lld, %d channels)", what, p.y_stride, p.channels);
     if (p.type == Elem::S8 && p.inner >= 131072)
         return fail(IOS_ERR_LIMIT, "%s: 8-bit products of 131072 or more elements can pass the 32 bits of their sum", what);
-    if (grouped_too_large(p)) return fail(IOS_ERR_LIMIT, "%s: %d rows of %d channels are too many for one call", what, p.total, p.channels);
+    if (p.total > kMaxRows || grouped_too_large(p)) return fail(IOS_ERR_LIMIT, "%s: %d rows of %d channels are too many for one call", what, p.total, p.channels);
     if (!p.rows && p.x_rows < p.total) return fail(IOS_ERR_ARGUMENT, "%s: x has %lld rows, y %d", what, p.x_rows, p.total);
     return IOS_OK;
 }
@@ -131,7 +133,7 @@ extern "C" int ios_route_experts(const void *logits, int type, int tokens, int e
         return fail(IOS_ERR_ARGUMENT, "route_experts: tokens >= 0, 1 <= k <= experts and stride >= 0 are needed");
     if (experts > kMaxExperts || k > kMaxChosen)
         return fail(IOS_ERR_LIMIT, "route_experts: at most %d experts and %d of them per token", kMaxExperts, kMaxChosen);
-    if ((long long)tokens * k > INT_MAX) return fail(IOS_ERR_LIMIT, "route_experts: more than 2^31 - 1 pairs");
+    if ((long long)tokens * k > kMaxRows) return fail(IOS_ERR_LIMIT, "route_experts: more than 2^30 pairs");
     if (!offsets || (tokens > 0 && (!logits || !chosen || !gates || !rows || !slots)))
         return fail(IOS_ERR_ARGUMENT, "route_experts: logits and the outputs must not be NULL");
     const size_t need = tokens == 0 ? 0 : route_workspace_bytes(tokens, experts, k);
@@ -228,7 +230,7 @@ extern "C" int ios_quantize_rows(const void *x, int type, long long x_rows, long
     if (!float_type(type)) return fail(IOS_ERR_ARGUMENT, "quantize_rows: x must be float32, float16 or bfloat16");
     if (inner <= 0 || x_rows < 0 || total_rows < 0 || x_stride < 0 || q_stride < inner)
         return fail(IOS_ERR_ARGUMENT, "quantize_rows: inner > 0, row counts >= 0, x_stride >= 0, q_stride >= inner are needed");
-    if (total_rows > INT_MAX) return fail(IOS_ERR_LIMIT, "quantize_rows: more than 2^31 - 1 rows");
+    if (total_rows > kMaxRows) return fail(IOS_ERR_LIMIT, "quantize_rows: more than 2^30 rows");
     if (!rows && x_rows < total_rows) return fail(IOS_ERR_ARGUMENT, "quantize_rows: x has %lld rows, q %lld", x_rows, total_rows);
     if (total_rows == 0) {
         record_error("");
@@ -261,7 +263,7 @@ extern "C" int ios_combine_experts(const void *y, int type, long long y_rows, lo
         return fail(IOS_ERR_ARGUMENT, "combine_experts: y and out must be float32, float16 or bfloat16");
     if (k <= 0 || channels <= 0 || tokens < 0 || y_rows < 0 || y_stride < 0 || out_stride < channels)
         return fail(IOS_ERR_ARGUMENT, "combine_experts: k, channels > 0, tokens, y_rows, y_stride >= 0, out_stride >= channels are needed");
-    if (tokens > INT_MAX || channels > 1 << 23) return fail(IOS_ERR_LIMIT, "combine_experts: at most 2^31 - 1 tokens of 2^23 channels");
+    if (tokens > kMaxRows || channels > 1 << 23) return fail(IOS_ERR_LIMIT, "combine_experts: at most 2^30 tokens of 2^23 channels");
     if (tokens == 0) {
         record_error("");
         return IOS_OK;

@@ -29,7 +29,7 @@ def route(lib, **change):
 @pytest.mark.parametrize('change,status', [
     (dict(type=S8), ARGUMENT), (dict(type=9), ARGUMENT), (dict(tokens=-1), ARGUMENT), (dict(experts=0), ARGUMENT),
     (dict(k=0), ARGUMENT), (dict(k=9), ARGUMENT), (dict(stride=-8), ARGUMENT), (dict(experts=1025), LIMIT),
-    (dict(experts=64, k=33), LIMIT), (dict(tokens=2 ** 30, k=4), LIMIT), (dict(logits=None), ARGUMENT), (dict(slots=None), ARGUMENT),
+    (dict(experts=64, k=33), LIMIT), (dict(tokens=2 ** 29, k=4), LIMIT), (dict(logits=None), ARGUMENT), (dict(slots=None), ARGUMENT),
     (dict(offsets=None), ARGUMENT), (dict(tokens=5000), ARGUMENT), (dict(tokens=5000, workspace=SOME, bytes=64), ARGUMENT)])
 def test_route_refuses(lib, change, status):
     assert route(lib, **change) == status
@@ -59,7 +59,8 @@ def grouped(lib, **change):
     (dict(act=-1), ARGUMENT), (dict(channels=0), ARGUMENT), (dict(inner=0), ARGUMENT), (dict(total=-1), ARGUMENT),
     (dict(groups=0), LIMIT), (dict(groups=1025), LIMIT), (dict(x_stride=-1), ARGUMENT), (dict(y_stride=31), ARGUMENT),
     (dict(type=S8, inner=131072, x_stride=131072), LIMIT), (dict(x_rows=9), ARGUMENT), (dict(x=None), ARGUMENT),
-    (dict(w=None), ARGUMENT), (dict(y=None), ARGUMENT), (dict(channels=2 ** 30, y_stride=2 ** 30), LIMIT)])
+    (dict(w=None), ARGUMENT), (dict(y=None), ARGUMENT), (dict(channels=2 ** 30, y_stride=2 ** 30), LIMIT), (dict(total=2 ** 30 + 1, x_rows=2 ** 31), LIMIT),
+    (dict(total=2 ** 29, x_rows=2 ** 29, channels=2 ** 20, y_stride=2 ** 20), LIMIT)])
 def test_grouped_refuses(lib, change, status):
     assert grouped(lib, **change) == status
     assert b'grouped_matmul' in lib.ios_last_error()
@@ -93,6 +94,8 @@ def test_quantize_and_combine_refuse(lib):
 
     def combine(y=SOME, type=F32, y_rows=4, gates=SOME, slots=SOME, tokens=2, k=2, channels=8, out=SOME, out_type=F32, stride=8):
         return lib.ios_combine_experts(y, type, y_rows, 8, gates, slots, tokens, k, channels, out, out_type, stride, None)
+    assert quantize(total=2 ** 30 + 1, x_rows=2 ** 31) == LIMIT and combine(tokens=2 ** 30 + 1) == LIMIT
+    assert combine(channels=2 ** 24, stride=2 ** 24) == LIMIT
     for change in (dict(y=None), dict(type=S8), dict(out_type=S8), dict(gates=None), dict(slots=None), dict(tokens=-1), dict(k=0),
                    dict(channels=0), dict(out=None), dict(stride=7), dict(y_rows=-1)):
         assert combine(**change) == ARGUMENT, change

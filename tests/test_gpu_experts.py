@@ -8,6 +8,9 @@ truncate where an addition rounds) loses at most 2^-23 of the running magnitude,
 (K / 8 + 32) 2^-23 S.  A float32 operand split into two TF32 numbers is off by 2^-22, and the product of the two small parts
 is dropped: 3 * 2^-22 S more.
 """
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -594,6 +597,31 @@ def test_captured_layer_on_a_side_stream_with_new_inputs():
         assert torch.equal(eager, expect[j])
         for _, _, _, out, _ in graphs:
             assert torch.equal(out, expect[j])
+
+
+def test_the_first_call_of_a_process_may_be_a_captured_one():
+    code = '''
+import sys
+sys.path[:0] = %r
+import torch
+from test_gpu_experts import layer
+from ios.contrib import ios_runtime as rt
+x, logits = torch.randn(20, 64, device="cuda").bfloat16(), torch.randn(20, 4, device="cuda")
+w_in, w_out = torch.randn(4, 96, 64, device="cuda").bfloat16(), torch.randn(4, 64, 48, device="cuda").bfloat16()
+graph = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph):
+    out = layer(x, logits, w_in, w_out, 2)
+graph.replay()
+assert torch.equal(out, layer(x, logits, w_in, w_out, 2))
+rt.device_ops_status()
+''' % [path for path in sys.path if path]
+    done = subprocess.run([sys.executable, '-c', code], capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_no_wait_ran_out():
+    rt.device_ops_status()
 
 
 def test_the_current_device_is_left_alone_and_host_memory_refused():
