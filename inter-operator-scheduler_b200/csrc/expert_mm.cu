@@ -8,21 +8,32 @@
 //   swizzle row per step (64 elements of 16 bits, 128 of 8 bits, 32 of float32).
 // * The group sizes are only known on the device.  Every CTA works out the same list of tiles from the offsets (one
 //   scan) and resident CTAs walk it; a group's rows are dealt evenly to its tiles.
+// * Few rows: bound by the weights, which are read once (4 tokens x 8 of 64 experts, gated, 2048 -> 1280, bfloat16: 273 MB
+//   in 49 us, 5.6 TB/s of the 6.5 that a copy reaches; what is left is four rounds of tiles where 3.5 would do).
+// * Many rows: bound by the tensor cores and the power they draw.  Pairs of CTAs (cta_group::2) share the rows of a tile of
+//   256 channels x 256 rows, which halves the loads of x and doubles the K steps in flight: 32768 rows in four groups, 2048 ->
+//   1280, bfloat16: 1500 TFLOP/s after 1200 with one CTA per tile; 8192 x 4096 x 8192 in 8 bits: 3300 TOP/s.
 // * Products too small to fill the GPU split K over a thread-block cluster: the CTAs deal the tile's columns among
 //   themselves, push their partial sums into the shared memory of the CTA that finishes a column, and that CTA adds them
 //   in rank order.  No workspace, no counters, the same bits every time.
-// * Operands arrive by TMA where their rows start on 16-byte boundaries; rows gathered by index then by cp.async of four
-//   warps (tile::gather4 moves 512 bytes per instruction and took 68 cycles for each: 1480 us where this takes @GATHER@ us, 4096
-//   tokens x 8 of 64 experts, gated, 2048 -> 1280).  Anything else goes through registers of eight loader warps.
-// * float32: every operand is split into two TF32 numbers on its way into shared memory (loader warps); three products
-//   a_hi b_hi + a_hi b_lo + a_lo b_hi.  The tensor core truncates where it adds, so the sum over more than 64 elements is
-//   formed in registers, rounded to nearest, from partial sums over 64.
-// * gated: 16 rows of the gate half and the 16 rows of the same channels of the other half alternate in the tile, so that
-//   a lane and the lane 16 further on hold the two factors of one result.
+// * Operands arrive by TMA where their rows start on 16-byte boundaries.  Rows gathered by index then come four at a time
+//   (tile::gather4).  Such a load keeps a warp for some 130 cycles, so eight warps share them (4096 tokens x 8 of 64 experts, gated:
+//   405 us with four warps, 305 with eight, 348 with sixteen, which leave the epilogue too few registers; 264 from rows that lie
+//   sorted).  Gathering by cp.async took 737 us: its fence between the copies and the tensor core waits for every copy under way.
+// * Anything else goes through registers of sixteen loader warps, word by word, shifted into place: 4096 x 8 rows of 2047
+//   bfloat16 at 135 TFLOP/s.
+// * float32: three products a_hi b_hi + a_hi b_lo + a_lo b_hi of TF32 numbers; the operands are split in shared memory, after
+//   they have landed (or by the loader warps): 16384 rows, 2048 -> 1024, at 130 TFLOP/s, bound by the splitting.  The tensor
+//   core truncates where it adds, which costs 1e-6 of a sum over 128 elements; so sums over 64 elements are added up in
+//   tensor memory, rounded to nearest: 4e-7 to 5e-7 of the result at any length.
+// * gated: 16 rows of the gate half and the 16 rows of the same channels of the other half alternate in the tile (one box of
+//   a five-dimensional view), so that a lane and the lane 16 further on hold the two factors of one result.
+// * Loads and tensor-core instructions are issued from warp-uniform code by a predicated lane.  Issued from a branch that one
+//   lane takes, each cost some 100 cycles, and 8192 x 4096 x 8192 in 8 bits took 300 us instead of 165.
 //
 // Warp roles: 0 = weight loads, 1 = MMA issuer, 2 = tensor memory, 3 = row loads, 4..11 (4..7) = epilogue, then
-// gathering or loader warps.  Every wait is bounded; on a time-out the device's error word is set, loads in flight are
-// waited for, tensor memory is freed and the kernel returns.
+// gathering, loader or splitting warps.  Every wait is bounded; on a time-out the device's error word is set, loads in flight
+// are waited for, tensor memory is freed and the kernel returns.
 #include "expert_ops.h"
 #include "kernels.h"
 #include "tc_device.h"
@@ -1077,18 +1088,22 @@ int choose(const GroupedParams &p, int sm_count, bool tma, MmGeom *t, bool *pair
     const int busy = std::min(p.groups, p.total);
     t->tn = columns_for(p, tma && p.type != Elem::F32 ? 256 : kLoaderCols);
     auto tiles = [&]() { return (long long)t->n_tiles * std::max<long long>(busy, ceil_div(p.total, t->tn)); };
-    if (tiles() < sm_count && t->tn > 128) t->tn = 128;
-    // K split: as long as it fills SMs that would idle and leaves every CTA two K steps
+    // ... or half of that where twice the tiles still run at once (200 rows, 4096 -> 2048 in 8 bits: 20.5 us instead of 24.6)
+    if (tiles() * 2 <= sm_count && t->tn > 128) t->tn = 128;
+    // K split: as long as it fills SMs that would idle and leaves every CTA two K steps (one row, 4096 -> 1024 in 8 bits, eight
+    // CTAs to a tile: 14.4 us instead of 16.4; where only two fit, 4096 -> 8192, 18.5 either way)
     t->cluster = 1;
     while (t->cluster < 8 && t->tn <= 128 && tiles() * t->cluster * 2 <= sm_count && t->k_steps >= 4 * t->cluster) t->cluster *= 2;
-    // Pairs of CTAs share the rows of a tile of 256 channels: half of the loads of x per SM, and with them twice the K
-    // steps in flight.  Worth it once the tiles are wide and keep every pair busy.
-    *pair = tma && t->tn == 256 && (long long)ceil_div(p.channels, 2 * t->tile_channels) * ceil_div(p.total, t->tn) >= sm_count / 2;
+    // Pairs of CTAs share the rows of a tile of 256 channels: half of the loads of x per SM, and with them more K steps in
+    // flight (32768 rows in four groups, 2048 -> 1280, bfloat16: 113 us instead of 129; 1024 rows, 4096 -> 8192 in 8 bits: 43 instead
+    // of 45; level where there are few tiles)
+    *pair = tma && t->tn == 256;
     t->grain = *pair ? 32 : 16;
     if (*pair) {
         t->tile_channels *= 2;
         t->n_tiles = ceil_div(p.channels, t->tile_channels);
     }
+    // (eight boxes of 16 rows instead: 272 us for 266, 4096 tokens x 8 of 64 experts)
     t->one_box = p.gated && p.channels % 16 == 0;
     t->box_rows = std::min(*pair ? t->tn / 2 : t->tn, kBoxRows);
     t->tmem_cols = std::max(32, (p.type == Elem::F32 ? 4 : 2) * t->tn);      // two accumulators; float32: and their sum (a power of two)
