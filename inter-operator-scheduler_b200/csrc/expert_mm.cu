@@ -67,6 +67,7 @@ constexpr int kLoaderCols = 128;                // widest tile of the loader war
 constexpr int kTurnCols = 16;                   // columns an epilogue warp turns round at a time: few, because a small
                                                 // product runs this code once, and cold code costs more than it does
 constexpr int kTurnBytes = kTurnCols * 32 * 4;  // ... in this much shared memory
+constexpr int kListed = 96;                     // tiles of a CTA that are found when it starts
 constexpr int kChunkSteps = 2;                  // float32: K steps per partial sum
 constexpr int kMaxStages = 12;
 constexpr int kMaxGroupTiles = INT_MAX / kMaxExperts - 1;    // tiles of a group: their sum over all groups fits an int
@@ -108,7 +109,8 @@ __device__ __forceinline__ int even_cols(int count, const MmGeom &t) {
 // The list of tiles: bound[g] = first row of group g, first[g] = tiles before group g.  Offsets come from the device:
 // whatever they hold, a group stays inside [0, total].  All threads call it; a barrier has to follow.
 struct Table {
-    int *bound, *first;       // groups + 1 each, in shared memory
+    int4 *listed;             // the CTA's first kListed tiles: (row0, channel0, group, valid)
+    int *bound, *first;       // groups + 1 each; all in shared memory
 };
 __device__ __forceinline__ int tiles_of(int count, const MmGeom &t) {
     if (count <= 0) return 0;
@@ -157,9 +159,9 @@ __device__ void build_table(const GroupedParams &p, const MmGeom &t, const Table
 }
 
 // Tiles of a group: up to 8 column tiles side by side, then the next channels, so that neighbours in the list share
-// weights and rows in L2.  Whole warps call it.
-__device__ __forceinline__ Tile find_tile(const GroupedParams &p, const MmGeom &t, const Table &table, int index, int cta_channel) {
-    int lo = 0, hi = p.groups;                    // table.first[lo] <= index < table.first[hi]
+// weights and rows in L2.
+__device__ int4 find_tile(const MmGeom &t, const Table &table, int groups, int index, int cta_channel) {
+    int lo = 0, hi = groups;                      // table.first[lo] <= index < table.first[hi]
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (table.first[mid] <= index) lo = mid;
@@ -172,13 +174,19 @@ __device__ __forceinline__ Tile find_tile(const GroupedParams &p, const MmGeom &
     const int band = at / (8 * t.n_tiles);
     const int wide = min(8, col_tiles - band * 8);
     const int inside = at - band * 8 * t.n_tiles;
-    Tile tile;
-    tile.group = uniform(lo);
     const int col0 = (band * 8 + inside % wide) * cols;
-    tile.row0 = uniform(begin + col0);
-    tile.valid = uniform(min(cols, count - col0));
+    return make_int4(begin + col0, inside / wide * t.tile_channels + cta_channel, lo, min(cols, count - col0));
+}
+// The CTA's n-th tile, number `index` of all.  Every role asks for it, whole warps at a time; finding a tile takes 1400
+// cycles, so the first are found by a thread each when the kernel starts.
+__device__ __forceinline__ Tile tile_of(const GroupedParams &p, const MmGeom &t, const Table &table, int n, int index, int cta_channel) {
+    const int4 found = n < kListed ? table.listed[n] : find_tile(t, table, p.groups, index, cta_channel);
+    Tile tile;
+    tile.row0 = uniform(found.x);
+    tile.channel0 = uniform(found.y);
+    tile.group = uniform(found.z);
+    tile.valid = uniform(found.w);
     tile.cols = (tile.valid + t.grain - 1) & -t.grain;
-    tile.channel0 = uniform(inside / wide * t.tile_channels + cta_channel);
     return tile;
 }
 
@@ -467,7 +475,8 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     const uint32_t full0 = base + t.bar_off, empty0 = full0 + 8u * t.stages;
     const uint32_t acc_full0 = empty0 + 8u * t.stages, acc_empty0 = acc_full0 + 16u;
     const uint32_t recv_full = acc_empty0 + 16u, recv_free = recv_full + 8u, ready0 = recv_free + 8u;
-    const Table table = {reinterpret_cast<int *>(generic + t.table_off), reinterpret_cast<int *>(generic + t.table_off) + p.groups + 1};
+    int *const bounds = reinterpret_cast<int *>(generic + t.table_off + kListed * sizeof(int4));
+    const Table table = {reinterpret_cast<int4 *>(generic + t.table_off), bounds, bounds + p.groups + 1};
 
     if (LOADS != kRegs && threadIdx.x == 32) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
@@ -499,6 +508,15 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     build_table(p, t, table, threads_of(KIND, LOADS));
+    __syncthreads();
+    const int rank = PAIR || t.cluster > 1 ? uniform(int(cluster_cta_rank())) : 0;
+    const int sharing = PAIR ? 2 : t.cluster;                    // CTAs of a tile
+    const int tile0 = int(blockIdx.x) / sharing, tile_step = int(gridDim.x) / sharing;
+    const int k_begin = PAIR ? 0 : t.k_steps * rank / t.cluster, k_end = PAIR ? t.k_steps : t.k_steps * (rank + 1) / t.cluster;
+    const int cta_channel = PAIR ? rank * (t.tile_channels / 2) : 0;
+    const int total_tiles = uniform(table.first[p.groups]);
+    if (threadIdx.x < kListed && int(threadIdx.x) * tile_step < total_tiles - tile0)
+        table.listed[threadIdx.x] = find_tile(t, table, p.groups, tile0 + int(threadIdx.x) * tile_step, cta_channel);
     tc_fence_before();
     __syncthreads();
     if (PAIR || t.cluster > 1) cluster_sync_all();
@@ -506,12 +524,6 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     // (only now: a successor that were to share this SM must find the tensor memory taken, not take it)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = uint32_t(uniform(int(tmem_slot)));
-    const int total_tiles = uniform(table.first[p.groups]);
-    const int rank = PAIR || t.cluster > 1 ? uniform(int(cluster_cta_rank())) : 0;
-    const int sharing = PAIR ? 2 : t.cluster;                    // CTAs of a tile
-    const int tile0 = int(blockIdx.x) / sharing, tile_step = int(gridDim.x) / sharing;
-    const int k_begin = PAIR ? 0 : t.k_steps * rank / t.cluster, k_end = PAIR ? t.k_steps : t.k_steps * (rank + 1) / t.cluster;
-    const int cta_channel = PAIR ? rank * (t.tile_channels / 2) : 0;
     // a pair's loads are counted in the CTA of rank 0, whose MMA issuer works for both
     const uint32_t full_at = PAIR ? cluster_map(full0, 0) : full0;
     const int k_elems = kRowBytes / t.esize;
@@ -531,8 +543,8 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         uint32_t phase = 1;
         int armed = 0;
         bool ok = true;
-        for (int i = tile0; i < total_tiles && ok; i += tile_step) {
-            const Tile tile = find_tile(p, t, table, i, cta_channel);
+        for (int i = tile0, n = 0; i < total_tiles && ok; i += tile_step, ++n) {
+            const Tile tile = tile_of(p, t, table, n, i, cta_channel);
             const uint32_t bytes = (PAIR ? 2 : 1) * kATileBytes + row_bytes_of(tile, 0) + (PAIR ? row_bytes_of(tile, tile.cols / 2) : 0);
             for (int k = k_begin; k < k_end; ++k) {
                 ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
@@ -554,7 +566,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         }
         if (!ok) {
             if (lane == 0) time_out(1);
-            for (int j = armed - 1, n = 0; j >= 0 && n < t.stages && (!PAIR || rank == 0); --j, ++n)
+            for (int j = armed - 1, left = t.stages; j >= 0 && left > 0 && (!PAIR || rank == 0); --j, --left)
                 mbar_wait(full0 + 8u * (j % t.stages), uint32_t((j / t.stages) & 1), nullptr);
         }
     } else if (LOADS == kTma && warp == 3) {
@@ -563,8 +575,8 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         int s = 0;
         uint32_t phase = 1;
         bool ok = true;
-        for (int i = tile0; i < total_tiles && ok; i += tile_step) {
-            const Tile tile = find_tile(p, t, table, i, cta_channel);
+        for (int i = tile0, n = 0; i < total_tiles && ok; i += tile_step, ++n) {
+            const Tile tile = tile_of(p, t, table, n, i, cta_channel);
             const int col0 = PAIR ? rank * (tile.cols / 2) : 0;              // a pair's CTAs hold half of the columns each
             const int loads = int(row_bytes_of(tile, col0)) / (t.box_rows * kRowBytes);
             for (int k = k_begin; k < k_end; ++k) {
@@ -589,8 +601,8 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         int s = 0, step = 0;
         uint32_t phase = 1;
         bool ok = true;
-        for (int i = tile0; i < total_tiles && ok; i += tile_step) {
-            const Tile tile = find_tile(p, t, table, i, cta_channel);
+        for (int i = tile0, n = 0; i < total_tiles && ok; i += tile_step, ++n) {
+            const Tile tile = tile_of(p, t, table, n, i, cta_channel);
             const int col0 = PAIR ? rank * (tile.cols / 2) : 0;
             const bool loads = group < int(row_bytes_of(tile, col0)) / (4 * kRowBytes);
             int at[4];
@@ -629,8 +641,8 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         int s = 0;
         uint32_t phase = 1;
         bool ok = true;
-        for (int i = tile0; i < total_tiles && ok; i += tile_step) {
-            const Tile tile = find_tile(p, t, table, i, cta_channel);
+        for (int i = tile0, n = 0; i < total_tiles && ok; i += tile_step, ++n) {
+            const Tile tile = tile_of(p, t, table, n, i, cta_channel);
             const bool with_x = part * kR < tile.cols;
             unsigned long long own;                          // lane r: where row r of the warp's 16 starts
             {
@@ -728,8 +740,8 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         int s = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (int i = tile0; i < total_tiles && ok; i += tile_step) {
-            const Tile tile = find_tile(p, t, table, i, cta_channel);
+        for (int i = tile0, n = 0; i < total_tiles && ok; i += tile_step, ++n) {
+            const Tile tile = tile_of(p, t, table, n, i, cta_channel);
             for (int k = k_begin; k < k_end; ++k) {
                 ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
                 if (!ok) break;
@@ -765,42 +777,39 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             int turn = 0;                                       // accumulator hand-overs so far
             bool ok = true;
             const uint32_t a_low0 = desc_low(base), stage_low = stage_bytes >> 4, b_low0 = kPlanes * kATileBytes >> 4;
-            for (int i = tile0; i < total_tiles && ok; i += tile_step) {
-                const Tile tile = find_tile(p, t, table, i, cta_channel);
+            for (int i = tile0, n = 0; i < total_tiles && ok; i += tile_step, ++n) {
+                const Tile tile = tile_of(p, t, table, n, i, cta_channel);
                 // sums in float32 / int32 (bit 4 / 5), operand formats, both K-major, N and M
                 const uint32_t idesc = (KIND == kI8 ? 2u << 4 : 1u << 4) | (t.format << 7) | (t.format << 10) |
                                        (uint32_t(tile.cols >> 3) << 17) | (uint32_t((PAIR ? 2 : 1) * kTileM >> 4) << 24);
-                uint32_t acc = 0;
-                for (int k = k_begin; k < k_end; ++k) {
-                    const bool opens = KIND == kX3 ? (k - k_begin) % kChunkSteps == 0 : k == k_begin;
-                    const bool closes = k + 1 == k_end || (KIND == kX3 && (k - k_begin) % kChunkSteps == kChunkSteps - 1);
-                    const uint32_t a = uint32_t(turn) & 1u;
-                    const uint32_t d = tmem + a * uint32_t(t.tn);
-                    if (opens) {
-                        ok = wait<PAIR>(acc_empty0 + 8u * a, ((uint32_t(turn) >> 1) & 1u) ^ 1u);
-                        acc = 0;
-                    }
-                    if (ok) ok = wait<PAIR>((kSplit ? ready0 : full0) + 8u * s, phase);
-                    ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t a_low = a_low0 + uint32_t(s) * stage_low, b_low = a_low + b_low0;
+                for (int k = k_begin; k < k_end;) {
+                    const int stop = KIND == kX3 ? min(k + kChunkSteps, k_end) : k_end;
+                    const uint32_t a = uint32_t(turn) & 1u, d = tmem + a * uint32_t(t.tn);
+                    ok = __all_sync(0xffffffffu, wait<PAIR>(acc_empty0 + 8u * a, ((uint32_t(turn) >> 1) & 1u) ^ 1u) ? 1 : 0) != 0;
+                    uint32_t acc = 0;
+                    for (; ok && k < stop; ++k) {
+                        ok = __all_sync(0xffffffffu, wait<PAIR>((kSplit ? ready0 : full0) + 8u * s, phase) ? 1 : 0) != 0;
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t a_low = a_low0 + uint32_t(s) * stage_low, b_low = a_low + b_low0;
 #pragma unroll
-                    for (uint32_t q = 0; q < 8; q += 2) {
-                        if (KIND != kX3) {
-                            umma<KIND, PAIR>(elected, d, a_low + q, b_low + q, idesc, acc);
-                        } else {
-                            const uint32_t a_rest = a_low + (kATileBytes >> 4), b_rest = b_low + (b_bytes >> 4);
-                            umma<KIND, PAIR>(elected, d, a_rest + q, b_low + q, idesc, acc);
-                            umma<KIND, PAIR>(elected, d, a_low + q, b_rest + q, idesc, 1u);
-                            umma<KIND, PAIR>(elected, d, a_low + q, b_low + q, idesc, 1u);
+                        for (uint32_t q = 0; q < 8; q += 2) {
+                            if (KIND != kX3) {
+                                umma<KIND, PAIR>(elected, d, a_low + q, b_low + q, idesc, acc);
+                            } else {
+                                const uint32_t a_rest = a_low + (kATileBytes >> 4), b_rest = b_low + (b_bytes >> 4);
+                                umma<KIND, PAIR>(elected, d, a_rest + q, b_low + q, idesc, acc);
+                                umma<KIND, PAIR>(elected, d, a_low + q, b_rest + q, idesc, 1u);
+                                umma<KIND, PAIR>(elected, d, a_low + q, b_low + q, idesc, 1u);
+                            }
+                            acc = 1;
                         }
-                        acc = 1;
+                        commit<PAIR>(elected, empty0 + 8u * s);
+                        if (++s == t.stages) { s = 0; phase ^= 1u; }
                     }
-                    commit<PAIR>(elected, empty0 + 8u * s);
-                    commit<PAIR>(closes ? elected : 0u, acc_full0 + 8u * a);
-                    turn += closes ? 1 : 0;
-                    if (++s == t.stages) { s = 0; phase ^= 1u; }
+                    if (!ok) break;
+                    commit<PAIR>(elected, acc_full0 + 8u * a);
+                    ++turn;
                 }
             }
             if (!ok && lane == 0) time_out(4);
@@ -822,8 +831,8 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         int turn = 0, round = 0;
         bool ok = true;
 #pragma unroll 1
-        for (int i = tile0; i < total_tiles && ok; i += tile_step, ++round) {
-            const Tile tile = find_tile(p, t, table, i, cta_channel);
+        for (int i = tile0, n = 0; i < total_tiles && ok; i += tile_step, ++n, ++round) {
+            const Tile tile = tile_of(p, t, table, n, i, cta_channel);
             const int warp_channel = tile.channel0 + quad * kWidth;
             const int channel = warp_channel + lane % kWidth;
             const long long per_channel = (long long)tile.group * (GATED ? 2 : 1) * p.channels + (long long)half * p.channels + channel;
@@ -1110,11 +1119,11 @@ int choose(const GroupedParams &p, int sm_count, bool tma, MmGeom *t, bool *pair
     const int planes = p.type == Elem::F32 ? 2 : 1;
     const size_t stage = size_t(planes) * (kATileBytes + (*pair ? t->tn / 2 : t->tn) * kRowBytes);
     const size_t recv = t->cluster > 1 ? size_t(t->tn) * kTileM * sizeof(float) : 0;
-    const size_t table = (2 * size_t(p.groups + 1) * sizeof(int) + 15) / 16 * 16;
+    const size_t table = kListed * sizeof(int4) + (2 * size_t(p.groups + 1) * sizeof(int) + 15) / 16 * 16;
     const size_t turn = 8 * kTurnBytes;
     const size_t fixed = 1024 + recv + turn + table + kBarBytes + kStaticBytes;
     t->stages = int(std::min<size_t>(kMaxStages, (kSmemLimit - fixed) / stage));
-    static_assert((kSmemLimit - 1024 - kNarrowCols * kTileM * 4 - 8 * kTurnBytes - 2 * (kMaxExperts + 4) * 4 - kBarBytes - kStaticBytes) /
+    static_assert((kSmemLimit - 1024 - kNarrowCols * kTileM * 4 - 8 * kTurnBytes - kListed * 16 - 2 * (kMaxExperts + 4) * 4 - kBarBytes - kStaticBytes) /
                   (2 * (kATileBytes + kNarrowCols * kRowBytes)) >= kGatherWarps / 2, "narrow tiles gather in that many turns");
     t->recv_off = int(t->stages * stage);
     t->turn_off = int(t->recv_off + recv);

@@ -257,6 +257,12 @@ def test_grouped_product_of_many_groups():
     run_grouped(4000, 1024, 64, 48, BF16, skew=0.3)
 
 
+def test_grouped_product_of_many_tiles():
+    """More tiles than a CTA finds when it starts: narrow ones, and those of pairs."""
+    run_grouped(2000, 1024, 16, 2100, BF16, skew=0.2)
+    run_grouped(50000, 2, 8, 5000, BF16, gated=True, skew=0.5)
+
+
 @ALL_TYPES
 def test_grouped_product_strides_and_odd_addresses(dtype):
     """Views into larger buffers: rows apart from one another, first elements at odd addresses, weights of one group shared."""
