@@ -357,18 +357,28 @@ cudaError_t route_typed(const RouteParams &p, cudaStream_t stream) {
 constexpr float kLift = 18446744073709551616.0f;      // 2^64: rows of tiny values are lifted by it, so that 127 / largest stays finite
 
 // The whole number nearest to 127 x / largest (halves to even), from the float product x * inverse and, where that
-// falls next to a half, from the exact comparison of 127 |x| with (n + 1/2) largest: both are at most 33 bits long,
-// so their difference in double precision is exact.  NaN gives 0, an infinity +-127.
+// falls next to a half, from the exact comparison of 127 |x| with (n + 1/2) largest.  For 16-bit x both sides have at most 19
+// bits and their difference is exact in float32; for float32 they have 33 and it is exact in double precision.  (Exact halves
+// are common: in bfloat16 one element in a thousand is half of its row's largest, which gives 63.5.)  NaN gives 0, an
+// infinity +-127.
+template <class T>
 __device__ __forceinline__ int quantize_one(float x, float inverse, float largest, float lift) {
     if (!(fabsf(x) <= 3.402823466e38f)) return isnan(x) ? 0 : (x > 0 ? 127 : -127);
     const float t = fabsf(x * lift) * inverse;
     const float n = floorf(t);
-    int q;
+    int q = int(rintf(t));
     if (fabsf(t - n - 0.5f) < 1e-3f) {
-        const double d = 127.0 * double(fabsf(x)) - (double(n) + 0.5) * double(largest);
-        q = int(n) + (d > 0.0 || (d == 0.0 && (int(n) & 1)) ? 1 : 0);
-    } else {
-        q = int(rintf(t));
+        bool above, equal;
+        if (sizeof(T) == 2) {
+            const float d = fmaf(-(2.0f * n + 1.0f), largest * lift, 254.0f * fabsf(x * lift));
+            above = d > 0.0f;
+            equal = d == 0.0f;
+        } else {
+            const double d = 127.0 * double(fabsf(x)) - (double(n) + 0.5) * double(largest);
+            above = d > 0.0;
+            equal = d == 0.0;
+        }
+        q = int(n) + (above || (equal && (int(n) & 1)) ? 1 : 0);
     }
     q = min(q, 127);
     return x < 0 ? -q : q;
@@ -421,9 +431,9 @@ template <> struct Eight<__nv_bfloat16> : EightHalves {
 };
 
 // Rows whose vectors of eight elements stay in the registers of a group of G threads, V per thread: read once.  Adding
-// 1.5 * 2^23 leaves the quotient's nearest whole number in the low bits of the sum; a thread that finds one of its eight
-// next to a half, and every thread of a row that holds an infinity or NaN, takes the exact form instead.
-// (4096 rows of 4096 bfloat16, 50 MB: 16 us, about half of it the memory's; the rest is eight instructions per element.)
+// 1.5 * 2^23 leaves the quotient's nearest whole number in the low bits of the sum; elements next to a half, and all of a row
+// that holds an infinity or NaN, take the exact form instead.  (8192 rows of 4096 bfloat16, 100 MB: 28 us, 3.6 TB/s; float32, 168 MB:
+// 5.1 TB/s -- bound by 14 instructions per element.  Blocks that stay and fetch the next row ahead took 38 us: fewer of them fit.)
 template <class T, int G, int V>
 __global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_rows_kernel(const QuantizeParams p) {
     constexpr int kBlock = G < 256 ? 256 : G;
@@ -475,21 +485,25 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_rows_kernel(const 
     const float lift = largest < 1e-30f ? kLift : 1.0f;
     const float inverse = largest > 0.0f ? 127.0f / (largest * lift) : 0.0f;
     signed char *q = p.q + r * p.q_stride;
+    // (the quotient is off by less than 127 * 2^-23; rows that need the exact form throughout get it: NaN compares as near, too)
+    const float near = odd || lift != 1.0f ? -1.0f : 0.49998f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const int c = (i * G + member) * 8;
         if (c >= p.inner) continue;
         uint32_t n[8];
-        float off = odd || lift != 1.0f ? 1.0f : 0.0f;
+        float off[8], most_off = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const float sum = fmaf(v[i].at(j), inverse, kMagic);
             n[j] = __float_as_uint(sum);
-            off = fmaxf(off, fabsf(fmaf(v[i].at(j), inverse, kMagic - sum)));
+            off[j] = fabsf(fmaf(v[i].at(j), inverse, kMagic - sum));
+            most_off = fmaxf(most_off, off[j]);
         }
-        if (off > 0.49998f) {                     // (the quotient is off by less than 127 * 2^-23)
+        if (!(most_off <= near)) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) n[j] = uint32_t(quantize_one(v[i].at(j), inverse, largest, lift));
+            for (int j = 0; j < 8; ++j)
+                if (!(off[j] <= near)) n[j] = uint32_t(quantize_one<T>(v[i].at(j), inverse, largest, lift));
         }
         uint2 packed;
         packed.x = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
@@ -524,7 +538,7 @@ __global__ void __launch_bounds__(256) quantize_any_kernel(const QuantizeParams 
     const float inverse = largest > 0.0f ? 127.0f / (largest * lift) : 0.0f;
     signed char *q = p.q + r * p.q_stride;
     for (int c = threadIdx.x; c < p.inner; c += 256)
-        q[c] = live ? (signed char)quantize_one(to_float(x[c]), inverse, largest, lift) : 0;
+        q[c] = live ? (signed char)quantize_one<T>(to_float(x[c]), inverse, largest, lift) : 0;
 }
 
 template <class T>
