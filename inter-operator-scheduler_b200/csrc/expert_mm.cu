@@ -24,8 +24,8 @@
 //   bfloat16 at 135 TFLOP/s.
 // * float32: three products a_hi b_hi + a_hi b_lo + a_lo b_hi of TF32 numbers; the operands are split in shared memory, after
 //   they have landed (or by the loader warps): 16384 rows, 2048 -> 1024, at 130 TFLOP/s, bound by the splitting.  The tensor
-//   core truncates where it adds, which costs 1e-6 of a sum over 128 elements; so sums over 64 elements are added up in
-//   tensor memory, rounded to nearest: 4e-7 to 5e-7 of the result at any length.
+//   core truncates where it adds, which costs 1e-6 of a sum over 128 elements; so the sums of every K step, 32 elements, are
+//   added up in tensor memory, rounded to nearest: 3e-7 of the result at any length, and no slower.
 // * gated: 16 rows of the gate half and the 16 rows of the same channels of the other half alternate in the tile (one box of
 //   a five-dimensional view), so that a lane and the lane 16 further on hold the two factors of one result.
 // * Loads and tensor-core instructions are issued from warp-uniform code by a predicated lane.  Issued from a branch that one
@@ -68,7 +68,7 @@ constexpr int kTurnCols = 16;                   // columns an epilogue warp turn
                                                 // product runs this code once, and cold code costs more than it does
 constexpr int kTurnBytes = kTurnCols * 32 * 4;  // ... in this much shared memory
 constexpr int kListed = 96;                     // tiles of a CTA that are found when it starts
-constexpr int kChunkSteps = 2;                  // float32: K steps per partial sum
+constexpr int kChunkSteps = 1;                  // float32: K steps per partial sum
 constexpr int kMaxStages = 12;
 constexpr int kMaxGroupTiles = INT_MAX / kMaxExperts - 1;    // tiles of a group: their sum over all groups fits an int
 constexpr int kBarBytes = 3 * kMaxStages * 8 + 48;    // mbarriers: three per stage, six more
@@ -336,17 +336,18 @@ __device__ __forceinline__ void split_tf32(uint32_t x, uint32_t *hi, uint32_t *l
 }
 
 __device__ __noinline__ float act_far(float v, int act) {
-    if (act == 2) return 1.0f / (1.0f + __expf(-v));
+    if (act == 4) return v / (1.0f + expf(-v));
+    if (act == 2) return 1.0f / (1.0f + expf(-v));
     return tanhf(v);
 }
-// the activation of N values; one branch for all of them
+// the activation of N values; one branch for all of them.  Results that are rounded to 16 bits take the fast exponential.
 template <int N>
-__device__ __forceinline__ void activate(float *v, int act) {
+__device__ __forceinline__ void activate(float *v, int act, bool fast) {
     if (act == 0) return;
     if (act == 1) {
 #pragma unroll
         for (int c = 0; c < N; ++c) v[c] = fmaxf(v[c], 0.0f);
-    } else if (act == 4) {
+    } else if (act == 4 && fast) {
 #pragma unroll
         for (int c = 0; c < N; ++c) v[c] = __fdividef(v[c], 1.0f + __expf(-v[c]));
     } else {
@@ -976,7 +977,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 #pragma unroll
                 for (int c = 0; c < kTurnCols; ++c) v[c] = v[c] * channel_scale + bias;
                 if (!GATED) {
-                    activate<kTurnCols>(v, p.act);
+                    activate<kTurnCols>(v, p.act, p.out_type != Elem::F32);
                 } else {
                     // the lower half of the warp finishes the even columns, the upper half the odd ones
                     float up[kTurnCols / 2];
@@ -986,7 +987,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                         up[c] = half ? v[2 * c + 1] : other;
                         v[c] = half ? other : v[2 * c];
                     }
-                    activate<kTurnCols / 2>(v, p.act);
+                    activate<kTurnCols / 2>(v, p.act, p.out_type != Elem::F32);
 #pragma unroll
                     for (int c = 0; c < kTurnCols / 2; ++c) v[c] *= up[c];
                 }
