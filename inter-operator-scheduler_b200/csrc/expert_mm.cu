@@ -9,7 +9,7 @@
 // * The group sizes are only known on the device.  Every CTA works out the same list of tiles from the offsets (one
 //   scan) and resident CTAs walk it; a group's rows are dealt evenly to its tiles.
 // * Few rows: bound by the weights, which are read once (4 tokens x 8 of 64 experts, gated, 2048 -> 1280, bfloat16: 273 MB
-//   in 49 us, 5.6 TB/s of the 6.5 that a copy reaches; what is left is four rounds of tiles where 3.5 would do).
+//   in 46 us, 5.9 TB/s of the 6.5 that a copy reaches; what is left is four rounds of tiles where 3.5 would do).
 // * Many rows: bound by the tensor cores and the power they draw.  Pairs of CTAs (cta_group::2) share the rows of a tile of
 //   256 channels x 256 rows, which halves the loads of x and doubles the K steps in flight: 32768 rows in four groups, 2048 ->
 //   1280, bfloat16: 1500 TFLOP/s after 1200 with one CTA per tile; 8192 x 4096 x 8192 in 8 bits: 3300 TOP/s.
@@ -18,14 +18,15 @@
 //   in rank order.  No workspace, no counters, the same bits every time.
 // * Operands arrive by TMA where their rows start on 16-byte boundaries.  Rows gathered by index then come four at a time
 //   (tile::gather4).  Such a load keeps a warp for some 130 cycles, so eight warps share them (4096 tokens x 8 of 64 experts, gated:
-//   405 us with four warps, 305 with eight, 348 with sixteen, which leave the epilogue too few registers; 264 from rows that lie
-//   sorted).  Gathering by cp.async took 737 us: its fence between the copies and the tensor core waits for every copy under way.
+//   405 us with four warps, 305 with eight, 348 with sixteen, which leave the epilogue too few registers; now 287, and 264 from
+//   rows that lie sorted).  Gathering by cp.async took 737 us: its fence between the copies and the tensor core waits for every copy under way.
 // * Anything else goes through registers of sixteen loader warps, word by word, shifted into place: 4096 x 8 rows of 2047
 //   bfloat16 at 135 TFLOP/s.
 // * float32: three products a_hi b_hi + a_hi b_lo + a_lo b_hi of TF32 numbers; the operands are split in shared memory, after
-//   they have landed (or by the loader warps): 16384 rows, 2048 -> 1024, at 130 TFLOP/s, bound by the splitting.  The tensor
-//   core truncates where it adds, which costs 1e-6 of a sum over 128 elements; so the sums of every K step, 32 elements, are
-//   added up in tensor memory, rounded to nearest: 3e-7 of the result at any length, and no slower.
+//   they have landed (or by the loader warps): 16384 rows, 2048 -> 1024, at 130 TFLOP/s, bound by three stages being loaded,
+//   split and multiplied in turn.  The tensor core truncates where it adds, which costs 1e-6 of a sum over 128 elements; so the
+//   sums of every K step, 32 elements, are added up in tensor memory, rounded to nearest: 3e-7 of the result at any length,
+//   and no slower.
 // * gated: 16 rows of the gate half and the 16 rows of the same channels of the other half alternate in the tile (one box of
 //   a five-dimensional view), so that a lane and the lane 16 further on hold the two factors of one result.
 // * Loads and tensor-core instructions are issued from warp-uniform code by a predicated lane.  Issued from a branch that one

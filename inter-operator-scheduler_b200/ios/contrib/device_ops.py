@@ -137,7 +137,7 @@ def _check(status):
         ios_runtime._check(status)
 
 
-@functools.lru_cache(maxsize=None)
+@functools.lru_cache(maxsize=1024)
 def _route_workspace(tokens, experts, k):
     need = _SIZE(0)
     _check(_lib.ios_route_experts_workspace(tokens, experts, k, ctypes.byref(need)))
