@@ -257,6 +257,15 @@ def test_grouped_product_of_many_groups():
     run_grouped(4000, 1024, 64, 48, BF16, skew=0.3)
 
 
+# few tiles of many columns: the K range split over clusters, few stages
+@ALL_TYPES
+@pytest.mark.parametrize('gather', [False, True])
+@pytest.mark.parametrize('total,groups,inner,channels', [(100, 1, 1024, 64), (128, 1, 2048, 200), (120, 1, 1023, 100), (210, 2, 4000, 130)])
+def test_grouped_product_split_over_clusters(dtype, gather, total, groups, inner, channels):
+    run_grouped(total, groups, inner, channels, dtype, gather=gather, scales=True, bias=True)
+    run_grouped(total, groups, inner, channels, dtype, gather=gather, gated=True, act='silu', out_dtype=F32)
+
+
 def test_grouped_product_of_many_tiles():
     """More tiles than a CTA finds when it starts: narrow ones, and those of pairs."""
     run_grouped(2000, 1024, 16, 2100, BF16, skew=0.2)
@@ -568,6 +577,31 @@ def test_layer_in_8_bits():
     # h is rounded to 8 bits: at most half a step of its row's largest / 127, in the root mean square over a row of normal
     # products far below 1 / 50 of the result's size
     assert (got.double() - value).norm() <= 0.02 * value.norm()
+
+
+def test_elements_past_32_bits():
+    """Matrices of more than 2^31 elements: the product's result, the quantiser's and the weighted sum's input."""
+    gen = generator(12)
+    rows, channels, inner = 540000, 4096, 16
+    x, w = make_operands(gen, (rows, inner), (2, channels, inner), BF16)
+    bounds = [0, 1000, rows]
+    y = rt.grouped_matmul(x, w, torch.tensor(bounds, dtype=torch.int32, device='cuda'))
+    assert y.numel() > 2 ** 31
+    tail = slice(rows - 300, rows)
+    check_grouped(y[tail], *grouped_reference(x[tail], w[1:], [0, 300], out_dtype=BF16))
+    check_grouped(y[:300], *grouped_reference(x[:300], w[:1], [0, 300], out_dtype=BF16))
+    q, scale = rt.quantize_rows(y)
+    expect, expect_scale = quantize_reference(y[tail])
+    assert torch.equal(q[tail].double(), expect)
+    assert ((scale[tail].double() - expect_scale).abs() <= U * expect_scale).all()
+    slots = torch.tensor([[rows - 1, rows - 2], [0, rows - 300]], dtype=torch.int32, device='cuda')
+    gates = torch.tensor([[0.5, 0.25], [2.0, 1.0]], device='cuda')
+    got = rt.combine_experts(y, gates, slots, out_dtype=F32).double()
+    parts = y[slots.long()].double() * gates.double()[:, :, None]
+    assert ((got - parts.sum(1)).abs() <= 3 * U * parts.abs().sum(1)).all()
+    again = rt.grouped_matmul(q, torch.ones(1, 8, channels, dtype=S8, device='cuda'), torch.tensor([0, rows], dtype=torch.int32, device='cuda'),
+                              row_scale=scale, out_dtype=F32)
+    assert torch.allclose(again[tail, 0].double(), q[tail].double().sum(1) * scale[tail].double(), rtol=4 * U)
 
 
 def test_captured_layer_on_a_side_stream_with_new_inputs():
