@@ -244,19 +244,14 @@ def _plain_combine(state):
 
 # ---- the framework's operators ---------------------------------------------------------------------------------------
 
-_loaded = []
-
-
 def _runtime():
-    if not _loaded:
-        package = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'inter-operator-scheduler_b200')
-        if not os.path.isdir(package):
-            package = os.path.abspath('inter-operator-scheduler_b200')
-        if package not in sys.path:
-            sys.path.insert(0, package)
-        from ios import ios_runtime
-        _loaded.append(ios_runtime)
-    return _loaded[0]
+    package = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'inter-operator-scheduler_b200')
+    if not os.path.isdir(package):
+        package = os.path.abspath('inter-operator-scheduler_b200')
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    from ios import ios_runtime
+    return ios_runtime
 
 
 def _own(state):
