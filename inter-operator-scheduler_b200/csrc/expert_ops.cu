@@ -354,11 +354,17 @@ cudaError_t route_typed(const RouteParams &p, cudaStream_t stream) {
 
 // ---- row quantiser -----------------------------------------------------------------------------
 
-constexpr float kLift = 18446744073709551616.0f;      // 2^64: rows of tiny values are lifted by it, so that 127 / largest stays finite
+// What a row is scaled by, a power of two, before its quotients are worked out: rows of tiny values are lifted, so that
+// 127 / largest stays finite, and rows of huge ones lowered, so that 254 times an element does.  (An element that the lowering
+// makes subnormal is below 2^-160 of the largest: it becomes 0 either way.)
+__device__ __forceinline__ float row_lift(float largest) {
+    return largest < 1e-30f ? 18446744073709551616.0f : largest > 1e30f ? 1.0f / 18446744073709551616.0f : 1.0f;      // 2^64, 2^-64
+}
 
 // The whole number nearest to 127 x / largest (halves to even), from the float product x * inverse and, where that
 // falls next to a half, from the exact comparison of 127 |x| with (n + 1/2) largest.  For 16-bit x both sides have at most 19
-// bits and their difference is exact in float32; for float32 they have 33 and it is exact in double precision.  (Exact halves
+// bits, and lifted as above they stay inside float32's range: its fused difference has the right sign; for float32 they have 33
+// and the difference is exact in double precision.  (Exact halves
 // are common: in bfloat16 one element in a thousand is half of its row's largest, which gives 63.5.)  NaN gives 0, an
 // infinity +-127.
 template <class T>
@@ -482,7 +488,7 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_rows_kernel(const 
     if (r >= p.total) return;
     const float largest = odd ? __uint_as_float(key) : Eight<T>::magnitude(key);
     if (member == 0) p.scale[r] = largest / 127.0f;
-    const float lift = largest < 1e-30f ? kLift : 1.0f;
+    const float lift = row_lift(largest);
     const float inverse = largest > 0.0f ? 127.0f / (largest * lift) : 0.0f;
     signed char *q = p.q + r * p.q_stride;
     // (the quotient is off by less than 127 * 2^-23; rows that need the exact form throughout get it: NaN compares as near, too)
@@ -534,7 +540,7 @@ __global__ void __launch_bounds__(256) quantize_any_kernel(const QuantizeParams 
 #pragma unroll
     for (int w = 0; w < 8; ++w) largest = fmaxf(largest, warp_max[w]);
     if (threadIdx.x == 0) p.scale[r] = largest / 127.0f;
-    const float lift = largest < 1e-30f ? kLift : 1.0f;
+    const float lift = row_lift(largest);
     const float inverse = largest > 0.0f ? 127.0f / (largest * lift) : 0.0f;
     signed char *q = p.q + r * p.q_stride;
     for (int c = threadIdx.x; c < p.inner; c += 256)
