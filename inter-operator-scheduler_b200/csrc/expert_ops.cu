@@ -8,6 +8,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 
 namespace ios {
 namespace {
@@ -326,17 +327,33 @@ int route_per_block(int tokens, int k) {
 }
 int route_blocks(int tokens, int k) { return (tokens + route_per_block(tokens, k) - 1) / route_per_block(tokens, k); }
 
+// The largest dynamic shared memory that a router kernel is launched with: kMaxExperts experts, kRoutePairs pairs (a single block:
+// 128 tokens of kMaxChosen, half of that).  The limit is set to this, once per kernel and device and never to a call's own size:
+// it belongs to the kernel, and another host thread may launch that between this thread's setting and its launch.
+constexpr size_t kRouteSmem = (size_t(kRouteThreads / 32 + 1) * kMaxExperts + 2 * size_t(kRoutePairs)) * sizeof(int);
+static_assert(kRouteSingleTokens * kMaxChosen <= kRoutePairs && 32 * kMaxChosen <= kRoutePairs && kRouteSmem + 1024 <= 227 * 1024, "fits an SM");
+template <class T, int PER, bool kSingle>
+cudaError_t allow_route_smem() {
+    static std::atomic<uint64_t> prepared{0};                // devices (of the first 64) that know
+    int device = 0;
+    cudaError_t err = cudaGetDevice(&device);
+    if (err != cudaSuccess) return err;
+    const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+    if (prepared.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    err = cudaFuncSetAttribute(route_pick_kernel<T, PER, kSingle>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kRouteSmem));
+    if (err == cudaSuccess) prepared.fetch_or(bit, std::memory_order_relaxed);
+    return err;
+}
+
 template <class T, int PER>
 cudaError_t route_run(const RouteParams &p, cudaStream_t stream) {
     const int per_block = route_per_block(p.tokens, p.k), blocks = route_blocks(p.tokens, p.k);
     const int threads = p.tokens <= 8 ? 256 : kRouteThreads;
     const size_t smem = (size_t(threads / 32 + 1) * p.experts + 2 * size_t(per_block) * p.k) * sizeof(int);
     const auto pick = blocks == 1 ? route_pick_kernel<T, PER, true> : route_pick_kernel<T, PER, false>;
-    if (smem > 48 * 1024) {
-        cudaError_t err = cudaFuncSetAttribute(pick, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-        if (err != cudaSuccess) return err;
-    }
-    cudaError_t err = launch(pick, blocks, threads, smem, stream, p, per_block);
+    cudaError_t err = blocks == 1 ? allow_route_smem<T, PER, true>() : allow_route_smem<T, PER, false>();
+    if (err != cudaSuccess) return err;
+    err = launch(pick, blocks, threads, smem, stream, p, per_block);
     if (err == cudaSuccess && blocks > 1)
         err = launch(route_place_kernel, blocks, kRouteThreads, 2 * size_t(p.experts) * sizeof(int), stream, p, per_block, blocks);
     return err;

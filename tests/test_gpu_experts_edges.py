@@ -2,6 +2,10 @@
 Calls of the expert-layer operators at the edges of what they take: huge magnitudes, sizes next to a launch limit, several
 host threads, row counts past a limit, waits that run out.  References and tolerances as in test_gpu_experts.py.
 """
+import subprocess
+import sys
+import threading
+
 import pytest
 
 from ios.contrib import ios_runtime as rt
@@ -10,7 +14,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip('torch')
 
-from test_gpu_experts import BF16, F16, F32, U, generator, quantize_reference  # noqa: E402
+from test_gpu_experts import BF16, F16, F32, U, check_route, generator, quantize_reference  # noqa: E402
 
 
 # ---- quantiser: magnitudes whose products with 254 pass float32 ------------------------------------
@@ -43,3 +47,45 @@ def test_quantized_rows_of_huge_values(dtype):
     x[1, 5], x[2, 6] = float('inf'), float('nan')
     for view in (x, x[:, 1:]):
         assert torch.equal(rt.quantize_rows(view)[0].double(), quantize_reference(view)[0])
+
+
+# ---- router: shared memory next to the default limit, several host threads -----------------------------
+
+@pytest.mark.parametrize('tokens,experts,k', [(108, 320, 8), (42, 352, 8), (120, 256, 16), (128, 1024, 32), (129, 1024, 32)])
+def test_first_route_of_a_process_at_any_size(tokens, experts, k):
+    """The first three need 48 KiB of shared memory with the kernel's own arrays, and less without; each is the first call."""
+    code = '''
+import sys
+sys.path[:0] = %r
+import torch
+from test_gpu_experts import check_route
+check_route(torch.randn(%d, %d, device="cuda"), %d, True)
+''' % ([path for path in sys.path if path], tokens, experts, k)
+    done = subprocess.run([sys.executable, '-c', code], capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_route_from_several_host_threads():
+    """Calls of one kernel with different shared-memory sizes, from threads that do not wait for one another."""
+    shapes = [(600, 1024, 8), (4000, 520, 8), (600, 520, 2), (300, 1000, 32)]
+    inputs = [torch.randn(t, e, generator=generator(t + e), device='cuda') for t, e, _ in shapes]
+    expect = [rt.route_experts(l, k) for l, (_, _, k) in zip(inputs, shapes)]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(1500):
+                    got = rt.route_experts(inputs[i], shapes[i][2])
+                torch.cuda.current_stream().synchronize()
+                assert all(torch.equal(a, b) for a, b in zip(got, expect[i]))
+        except Exception as error:
+            failed.append((shapes[i], error))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(shapes))]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not failed, failed
