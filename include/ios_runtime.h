@@ -99,7 +99,8 @@ IOS_API const char *ios_last_error(void);
  * "persistent" "1"/"0" (grids of several waves run as resident CTAs that walk the tiles / one CTA per tile),
  * "bulk_store" "1"/"0" (results leave through a bulk tensor store / straight from registers),
  * "split_k", "bn", "stages", "producers" (a positive number overrides the K split, the output-channel tile
- * width, the depth of the shared-memory pipeline, the lanes that issue TMA loads; "0" = automatic), "timeline" "1"/"0" (phase stamps of one CTA).
+ * width, the depth of the shared-memory pipeline, the lanes that issue TMA loads; "0" = automatic), "timeline" "1"/"0" (phase stamps of one CTA),
+ * "product_wait_us" (what a bounded wait inside a product on device tensors may take; "0" = 2 seconds).
  * Options apply to plans built afterwards on the calling process. */
 IOS_API int ios_set_option(const char *key, const char *value);
 IOS_API int ios_get_option(const char *key, char *value, int capacity);

@@ -33,8 +33,9 @@
 //   lane takes, each cost some 100 cycles, and 8192 x 4096 x 8192 in 8 bits took 300 us instead of 165.
 //
 // Warp roles: 0 = weight loads, 1 = MMA issuer, 2 = tensor memory, 3 = row loads, 4..11 (4..7) = epilogue, then
-// gathering, loader or splitting warps.  Every wait is bounded; on a time-out the device's error word is set, loads in flight
-// are waited for, tensor memory is freed and the kernel returns.
+// gathering, loader or splitting warps.  Every wait on an mbarrier is bounded, and every warp reaches the barriers that it shares with
+// others (the epilogue's once per tile, the last one) whether or not it gave up.  On a time-out the device's error word is set,
+// loads in flight are waited for, tensor memory is freed and the kernel returns.
 #include "expert_ops.h"
 #include "kernels.h"
 #include "tc_device.h"
@@ -90,6 +91,7 @@ struct MmGeom {
     int tmem_cols;
     uint32_t format;    // operand format field of the instruction descriptor
     int esize;
+    uint32_t wait_ns;   // what a wait may take
     int recv_off, turn_off, table_off, bar_off;   // byte offsets in shared memory
 };
 
@@ -282,10 +284,11 @@ __device__ __forceinline__ void commit(uint32_t elected, uint32_t bar) {
                      ::"r"(elected), "r"(bar)
                      : "memory");
 }
-// mbar_wait for a barrier that other CTAs of the cluster may arrive at
+// Bounded wait, for a barrier that (CLUSTER) other CTAs of the cluster may arrive at.  The clock runs on while the GPU does other
+// work, so what counts is the barrier's state some time after it has run out.
 template <bool CLUSTER>
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
-    if (!CLUSTER) return mbar_wait(bar, parity, nullptr);
+__device__ __forceinline__ bool passed(uint32_t bar, uint32_t parity) {
+    if (!CLUSTER) return mbar_try_wait(bar, parity);
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -294,7 +297,20 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
         : "=r"(done)
         : "r"(bar), "r"(parity)
         : "memory");
-    return done != 0 || mbar_wait_cluster(bar, parity, nullptr);
+    return done != 0;
+}
+template <bool CLUSTER>
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, uint32_t wait_ns) {
+    uint32_t start = 0, late = 0;
+    for (uint32_t spin = 1;; ++spin) {
+        if (passed<CLUSTER>(bar, parity)) return true;
+        if ((spin & 63u) != 0) continue;
+        if (late) return false;
+        uint32_t now;
+        asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(now));
+        if (spin == 64u) start = now;
+        else late = now - start > wait_ns;
+    }
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -549,7 +565,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             const Tile tile = tile_of(p, t, table, n, i, cta_channel);
             const uint32_t bytes = (PAIR ? 2 : 1) * kATileBytes + row_bytes_of(tile, 0) + (PAIR ? row_bytes_of(tile, tile.cols / 2) : 0);
             for (int k = k_begin; k < k_end; ++k) {
-                ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
+                ok = __all_sync(0xffffffffu, wait<false>(empty0 + 8u * s, phase, t.wait_ns) ? 1 : 0) != 0;
                 if (!ok) break;
                 const uint32_t dst = base + uint32_t(s) * stage_bytes, bar = full_at + 8u * s;
                 if (!PAIR || rank == 0) expect(elected, full0 + 8u * s, bytes);
@@ -582,7 +598,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             const int col0 = PAIR ? rank * (tile.cols / 2) : 0;              // a pair's CTAs hold half of the columns each
             const int loads = int(row_bytes_of(tile, col0)) / (t.box_rows * kRowBytes);
             for (int k = k_begin; k < k_end; ++k) {
-                ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
+                ok = __all_sync(0xffffffffu, wait<false>(empty0 + 8u * s, phase, t.wait_ns) ? 1 : 0) != 0;
                 if (!ok) break;
                 const uint32_t dst = base + uint32_t(s) * stage_bytes + kPlanes * kATileBytes, bar = full_at + 8u * s;
                 for (int b = 0; b < loads; ++b)
@@ -616,7 +632,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             const int4 src = make_int4(at[0], at[1], at[2], at[3]);
             for (int k = k_begin; k < k_end; ++k, ++step) {
                 if (!narrow || (step & (turns - 1)) == part) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
+                    ok = __all_sync(0xffffffffu, wait<false>(empty0 + 8u * s, phase, t.wait_ns) ? 1 : 0) != 0;
                     if (!ok) break;
                     if (loads)
                         load_rows4<PAIR>(1u, base + uint32_t(s) * stage_bytes + kPlanes * kATileBytes + uint32_t(group) * 4u * kRowBytes, &map_x,
@@ -683,7 +699,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             if (plain(k_begin)) fetch(now, now_last, k_begin);
             for (int k = k_begin; k < k_end; ++k) {
                 if (k + 1 < k_end && plain(k + 1)) fetch(next, next_last, k + 1);
-                ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
+                ok = __all_sync(0xffffffffu, wait<false>(empty0 + 8u * s, phase, t.wait_ns) ? 1 : 0) != 0;
                 if (!ok) break;
                 uint8_t *stage = generic + size_t(s) * stage_bytes + part * kR * kRowBytes + (lane & 3) * 4;
                 const auto store = [&](int r, uint32_t word) {
@@ -745,7 +761,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         for (int i = tile0, n = 0; i < total_tiles && ok; i += tile_step, ++n) {
             const Tile tile = tile_of(p, t, table, n, i, cta_channel);
             for (int k = k_begin; k < k_end; ++k) {
-                ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8u * s, phase, nullptr) ? 1 : 0) != 0;
+                ok = __all_sync(0xffffffffu, wait<false>(full0 + 8u * s, phase, t.wait_ns) ? 1 : 0) != 0;
                 if (!ok) break;
                 uint8_t *stage = generic + size_t(s) * stage_bytes;
                 const auto split = [&](uint8_t *at, uint32_t apart) {
@@ -787,10 +803,10 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 for (int k = k_begin; k < k_end;) {
                     const int stop = KIND == kX3 ? min(k + kChunkSteps, k_end) : k_end;
                     const uint32_t a = uint32_t(turn) & 1u, d = tmem + a * uint32_t(t.tn);
-                    ok = __all_sync(0xffffffffu, wait<PAIR>(acc_empty0 + 8u * a, ((uint32_t(turn) >> 1) & 1u) ^ 1u) ? 1 : 0) != 0;
+                    ok = __all_sync(0xffffffffu, wait<PAIR>(acc_empty0 + 8u * a, ((uint32_t(turn) >> 1) & 1u) ^ 1u, t.wait_ns) ? 1 : 0) != 0;
                     uint32_t acc = 0;
                     for (; ok && k < stop; ++k) {
-                        ok = __all_sync(0xffffffffu, wait<PAIR>((kSplit ? ready0 : full0) + 8u * s, phase) ? 1 : 0) != 0;
+                        ok = __all_sync(0xffffffffu, wait<PAIR>((kSplit ? ready0 : full0) + 8u * s, phase, t.wait_ns) ? 1 : 0) != 0;
                         if (!ok) break;
                         tc_fence_after();
                         const uint32_t a_low = a_low0 + uint32_t(s) * stage_low, b_low = a_low + b_low0;
@@ -833,7 +849,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         int turn = 0, round = 0;
         bool ok = true;
 #pragma unroll 1
-        for (int i = tile0, n = 0; i < total_tiles && ok; i += tile_step, ++n, ++round) {
+        for (int i = tile0, n = 0; i < total_tiles; i += tile_step, ++n, ++round) {
             const Tile tile = tile_of(p, t, table, n, i, cta_channel);
             const int warp_channel = tile.channel0 + quad * kWidth;
             const int channel = warp_channel + lane % kWidth;
@@ -856,17 +872,18 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 }
                 asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory");
             }
+            if (!ok) continue;                                        // a warp that gave up keeps the others' barrier whole, no more
             // ---- the sums of this CTA's K range ----
             uint32_t sums = lane_tmem + (uint32_t(turn) & 1u) * uint32_t(t.tn), held = acc_empty0 + 8u * (uint32_t(turn) & 1u);
             if (KIND != kX3) {
-                ok = wait<PAIR>(acc_full0 + 8u * (uint32_t(turn) & 1u), (uint32_t(turn) >> 1) & 1u);
+                ok = wait<PAIR>(acc_full0 + 8u * (uint32_t(turn) & 1u), (uint32_t(turn) >> 1) & 1u, t.wait_ns);
                 ++turn;
             } else {
                 // added up in tensor memory behind the two accumulators
                 sums = lane_tmem + 2u * uint32_t(t.tn);
                 for (int k = k_begin; k < k_end && ok; k += kChunkSteps, ++turn) {
                     const uint32_t a = uint32_t(turn) & 1u;
-                    ok = __all_sync(0xffffffffu, wait<PAIR>(acc_full0 + 8u * a, (uint32_t(turn) >> 1) & 1u) ? 1 : 0) != 0;
+                    ok = __all_sync(0xffffffffu, wait<PAIR>(acc_full0 + 8u * a, (uint32_t(turn) >> 1) & 1u, t.wait_ns) ? 1 : 0) != 0;
                     if (!ok) break;
                     tc_fence_after();
                     for (int c0 = share * 16; c0 < tile.cols; c0 += kShare * 16) {
@@ -885,9 +902,9 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                     if (lane == 0) mbar_arrive(acc_empty0 + 8u * a);          // (no pairs)
                 }
             }
-            if (ok && t.cluster > 1 && round > 0) ok = wait<true>(recv_free, uint32_t(round - 1) & 1u);
+            if (ok && t.cluster > 1 && round > 0) ok = wait<true>(recv_free, uint32_t(round - 1) & 1u, t.wait_ns);
             ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
-            if (!ok) break;
+            if (!ok) continue;
             tc_fence_after();
             const auto release = [&]() {                              // the accumulator may be written again
                 if (KIND == kX3) return;
@@ -914,8 +931,8 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 release();
                 __syncwarp();
                 if (lane < t.cluster) mbar_arrive_cluster(cluster_map(recv_full, uint32_t(lane)));
-                ok = __all_sync(0xffffffffu, wait<true>(recv_full, uint32_t(round) & 1u) ? 1 : 0) != 0;
-                if (!ok) break;
+                ok = __all_sync(0xffffffffu, wait<true>(recv_full, uint32_t(round) & 1u, t.wait_ns) ? 1 : 0) != 0;
+                if (!ok) continue;
                 // pairs of columns: a gated result takes two lanes' columns at once
                 const int mine = kShare == 1 ? per : (per / 2 + 1) / 2 * 2;          // columns of the first warp of a quarter
                 from = rank * per + share * mine;
@@ -1088,10 +1105,14 @@ int columns_for(const GroupedParams &p, int most) {
     return tn;
 }
 
+std::atomic<uint32_t> g_wait_us{0};                           // testing aid: what a wait may take; 0: the default
+
 // Chooses the tiling; touches no device.  Returns the CTAs to launch.
 int choose(const GroupedParams &p, int sm_count, bool tma, MmGeom *t, bool *pair) {
     const int esize = elem_size(p.type);
     t->esize = esize;
+    const uint32_t wait_us = g_wait_us.load(std::memory_order_relaxed);
+    t->wait_ns = wait_us ? wait_us * 1000u : uint32_t(kWaitBudgetNs);
     t->format = p.type == Elem::BF16 ? 1u : p.type == Elem::F16 ? 0u : p.type == Elem::S8 ? 1u : 2u;
     t->tile_channels = p.gated ? kTileM / 2 : kTileM;
     t->n_tiles = ceil_div(p.channels, t->tile_channels);
@@ -1179,6 +1200,8 @@ cudaError_t sm_count_of_current(int *count) {
 }
 
 }  // namespace
+
+void set_product_wait(int us) { g_wait_us.store(uint32_t(us), std::memory_order_relaxed); }
 
 bool grouped_too_large(const GroupedParams &p) {
     return p.total > 0 && (long long)ceil_div(p.total, columns_for(p, kLoaderCols)) * ceil_div(p.channels, kTileM / 2) > kMaxGroupTiles;

@@ -82,6 +82,8 @@ struct GroupedParams {
 cudaError_t launch_grouped(const GroupedParams &p, cudaStream_t stream);
 // more tiles than the kernel's table counts
 bool grouped_too_large(const GroupedParams &p);
+// Testing aid: what a wait inside a product may take, in microseconds (at most 2 seconds); 0: the default, 2 seconds.
+void set_product_wait(int us);
 // Waits for the stream; *code: the wait that ran out in a product on the current device since the last call, 0 for none.
 cudaError_t expert_mm_status(cudaStream_t stream, int *code);
 

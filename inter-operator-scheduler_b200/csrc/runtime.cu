@@ -27,6 +27,7 @@
 #include "../../include/ios_runtime.h"
 #include "graph.h"
 #include "kernels.h"
+#include "expert_ops.h"
 #include "plan.h"
 
 namespace ios {
@@ -872,6 +873,11 @@ int ios_set_option(const char *key, const char *value) {
         else if (k == "timeline") g_options.timeline = v == "1";
         else if (k == "stage_barriers" && (v == "0" || v == "1")) g_options.stage_barriers = v == "1";
         else if (k == "pdl_edges" && (v == "0" || v == "1")) g_options.pdl_edges = v == "1";
+        else if (k == "product_wait_us") {
+            const int us = std::atoi(value);
+            if (us < 0 || us > 2000000) throw ArgumentError("product_wait_us must be 0..2000000");
+            set_product_wait(us);
+        }
         else throw ArgumentError("unknown option " + k + "=" + v);
     });
 }

@@ -1,0 +1,13 @@
+"""
+Arguments of the operators on device tensors at the edges of what they take, on a machine without a GPU.
+"""
+import pytest
+
+from ios.contrib import ios_runtime as rt
+
+
+def test_what_a_wait_may_take_is_checked():
+    for bad in (-1, 2000001):
+        with pytest.raises(RuntimeError, match='product_wait_us'):
+            rt.set_option('product_wait_us', bad)
+    rt.set_option('product_wait_us', 0)

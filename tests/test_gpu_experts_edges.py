@@ -89,3 +89,69 @@ def test_route_from_several_host_threads():
     for thread in threads:
         thread.join()
     assert not failed, failed
+
+
+# ---- products whose waits run out -------------------------------------------------------------------
+
+@pytest.fixture
+def short_waits():
+    """Sets what a wait inside a product may take, in microseconds; the default comes back, and the record is read, at the end."""
+    yield lambda us: rt.set_option('product_wait_us', us)
+    rt.set_option('product_wait_us', 0)
+    try:
+        rt.device_ops_status()
+    except RuntimeError:
+        pass
+
+
+def ran_out():
+    try:
+        rt.device_ops_status()
+    except RuntimeError as error:
+        assert 'ran out' in str(error)
+        return True
+    return False
+
+
+def test_a_wait_that_runs_out_is_reported_and_ends(short_waits):
+    """One tile whose sums take far longer than its epilogue may wait: the rest of the product ends by itself."""
+    inner = 1 << 23
+    x = torch.ones(1, inner, dtype=BF16, device='cuda').expand(64, -1)
+    w = torch.ones(1, 1, inner, dtype=BF16, device='cuda').expand(1, 128, -1)
+    offsets = torch.tensor([0, 64], dtype=torch.int32, device='cuda')
+    scale = torch.ones(64, device='cuda')
+    short_waits(100)
+    rt.grouped_matmul(x, w, offsets, row_scale=scale)
+    assert ran_out()
+    short_waits(0)
+    small = rt.grouped_matmul(x[:, :4096], w[:, :, :4096], offsets, row_scale=scale)
+    assert (small == 4096).all()
+    assert not ran_out()
+
+
+@pytest.mark.parametrize('us', [100, 1500, 6000])
+@pytest.mark.parametrize('dtype,x_rows,total,inner,channels,gather', [
+    (BF16, 1, 6000, 1 << 20, 1500, False), (BF16, 256, 12000, 1 << 20, 1024, True), (BF16, 100, 100, 1 << 22, 128, False),
+    (F32, 2000, 2000, 1 << 18, 1500, False)], ids=['loaders', 'gathered-pairs', 'cluster', 'float'])
+def test_products_end_whichever_wait_runs_out(short_waits, us, dtype, x_rows, total, inner, channels, gather):
+    """Tiles of a millisecond or more, several per CTA, and scales that the epilogue warps share: some waits run out and some do
+    not, every kernel returns, and the next one is whole."""
+    gen = generator(total)
+    x = torch.empty(x_rows, inner, dtype=dtype, device='cuda').uniform_(-1, 1, generator=gen)
+    w = torch.empty(1, 1 if x_rows == 1 else channels, inner, dtype=dtype, device='cuda').uniform_(-1, 1, generator=gen)
+    if x_rows == 1:
+        x, w = x.expand(total, -1), w.expand(1, channels, -1)
+    args = dict(row_scale=torch.rand(x.shape[0], generator=gen, device='cuda'), out_dtype=F32)
+    if gather:
+        args['rows'] = torch.randint(0, x_rows, (total,), generator=gen, device='cuda', dtype=torch.int32)
+    offsets = torch.tensor([0, total], dtype=torch.int32, device='cuda')
+    expect = rt.grouped_matmul(x, w, offsets, **args)
+    assert not ran_out()
+    short_waits(us)
+    for _ in range(2):
+        got = rt.grouped_matmul(x, w, offsets, **args)
+        if not ran_out():
+            assert torch.equal(got, expect)
+    short_waits(0)
+    assert torch.equal(rt.grouped_matmul(x, w, offsets, **args), expect)
+    assert not ran_out()
