@@ -240,8 +240,10 @@ IOS_API int ios_static_scratch_status(void *cuda_stream);
  * inputs give the same bits.  Zero rows are no error; more than 2^30 rows or pairs are one (IOS_ERR_LIMIT). */
 enum { IOS_F32 = 0, IOS_F16 = 1, IOS_BF16 = 2, IOS_S8 = 3 };   /* element types */
 
-/* Waits for cuda_stream, then tells whether a bounded wait inside a product on `device` ran out since the last call of
- * this function (IOS_ERR_TIMEOUT: an output is incomplete) -- the calls below return before their work is done. */
+/* Waits for cuda_stream, then tells whether a bounded wait inside a product on `device`, on any stream, ran out since the
+ * calling host thread last asked (or, if it never did, since the library was loaded).  IOS_ERR_TIMEOUT: an output is
+ * incomplete.  Nothing else says so: the calls below return before their work is done.  What one thread is told, the others
+ * still are.  A wait may take two seconds, which a process that is stopped or descheduled that long can exceed. */
 IOS_API int ios_device_ops_status(int device, void *cuda_stream);
 
 /* The router.  For each token the k experts with the largest logits (equal logits: the lower index first; -inf and

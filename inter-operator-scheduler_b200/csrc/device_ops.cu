@@ -294,11 +294,13 @@ extern "C" int ios_combine_experts(const void *y, int type, long long y_rows, lo
 
 extern "C" int ios_device_ops_status(int device, void *cuda_stream) {
     int current = 0, code = 0;
+    if (device < 0 || device >= kMaxStatusDevices)
+        return fail(IOS_ERR_ARGUMENT, "device_ops_status: device must be 0..%d", kMaxStatusDevices - 1);
     if (cudaError_t err = cudaGetDevice(&current)) return DeviceScope::cuda("cudaGetDevice", err);
     if (cudaError_t err = cudaSetDevice(device)) return DeviceScope::cuda("cudaSetDevice", err);
-    const cudaError_t err = expert_mm_status(static_cast<cudaStream_t>(cuda_stream), &code);
+    const cudaError_t err = expert_mm_status(device, static_cast<cudaStream_t>(cuda_stream), &code);
     cudaSetDevice(current);
-    if (err != cudaSuccess) return DeviceScope::cuda("reading the time-out word", err);
+    if (err != cudaSuccess) return DeviceScope::cuda("reading the time-out counts", err);
     if (code != 0) return fail(IOS_ERR_TIMEOUT, "a bounded wait inside a product ran out (code %d): its output is incomplete", code);
     record_error("");
     return IOS_OK;

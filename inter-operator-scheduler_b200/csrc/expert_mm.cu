@@ -34,7 +34,7 @@
 //
 // Warp roles: 0 = weight loads, 1 = MMA issuer, 2 = tensor memory, 3 = row loads, 4..11 (4..7) = epilogue, then
 // gathering, loader or splitting warps.  Every wait on an mbarrier is bounded, and every warp reaches the barriers that it shares with
-// others (the epilogue's once per tile, the last one) whether or not it gave up.  On a time-out the device's error word is set,
+// others (the epilogue's once per tile, the last one) whether or not it gave up.  A time-out is counted in a word of the device,
 // loads in flight are waited for, tensor memory is freed and the kernel returns.
 #include "expert_ops.h"
 #include "kernels.h"
@@ -76,7 +76,10 @@ constexpr int kMaxGroupTiles = INT_MAX / kMaxExperts - 1;    // tiles of a group
 constexpr int kBarBytes = 3 * kMaxStages * 8 + 48;    // mbarriers: three per stage, six more
 constexpr size_t kSmemLimit = 227 * 1024, kStaticBytes = 4608;    // ... of which the kernel's static arrays may take
 
-__device__ int g_expert_error;                  // set by a wait that ran out, read by expert_mm_status
+// Waits that ran out since the library was loaded, by the code of the waiting role (see time_out); read by expert_mm_status and never
+// cleared: what one reader has seen is news to the next.
+constexpr int kWaitCodes = 8;
+__device__ unsigned g_expert_timeouts[kWaitCodes];
 
 struct MmGeom {
     int tn;             // columns a tile may have
@@ -324,7 +327,7 @@ __device__ __forceinline__ void store_cluster(uint32_t dst, float v) {
 // Records a wait that ran out.  The loads that this CTA has under way land within microseconds; those counted in another
 // CTA's barriers cannot be waited for from here, so a millisecond is let pass.
 __device__ __noinline__ void time_out(int code) {
-    atomicExch(&g_expert_error, code);
+    atomicAdd(&g_expert_timeouts[code], 1u);
     const uint64_t t0 = global_ns();
     while (global_ns() - t0 < 1000000) __nanosleep(1000);
 }
@@ -1251,14 +1254,18 @@ cudaError_t launch_grouped(const GroupedParams &given, cudaStream_t stream) {
 #undef IOS_RUN
 }
 
-cudaError_t expert_mm_status(cudaStream_t stream, int *code) {
-    cudaError_t err = cudaMemcpyFromSymbolAsync(code, g_expert_error, sizeof *code, 0, cudaMemcpyDeviceToHost, stream);
+cudaError_t expert_mm_status(int device, cudaStream_t stream, int *code) {
+    static thread_local unsigned seen[kMaxStatusDevices][kWaitCodes] = {};     // by this host thread
+    unsigned now[kWaitCodes];
+    cudaError_t err = cudaMemcpyFromSymbolAsync(now, g_expert_timeouts, sizeof now, 0, cudaMemcpyDeviceToHost, stream);
     if (err == cudaSuccess) err = cudaStreamSynchronize(stream);
-    if (err == cudaSuccess && *code != 0) {
-        const int zero = 0;
-        err = cudaMemcpyToSymbol(g_expert_error, &zero, sizeof zero);
+    if (err != cudaSuccess) return err;
+    *code = 0;
+    for (int c = kWaitCodes - 1; c > 0; --c) {
+        if (now[c] != seen[device][c]) *code = c;
+        seen[device][c] = now[c];
     }
-    return err;
+    return cudaSuccess;
 }
 
 }  // namespace ios

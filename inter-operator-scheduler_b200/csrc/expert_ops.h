@@ -84,7 +84,9 @@ cudaError_t launch_grouped(const GroupedParams &p, cudaStream_t stream);
 bool grouped_too_large(const GroupedParams &p);
 // Testing aid: what a wait inside a product may take, in microseconds (at most 2 seconds); 0: the default, 2 seconds.
 void set_product_wait(int us);
-// Waits for the stream; *code: the wait that ran out in a product on the current device since the last call, 0 for none.
-cudaError_t expert_mm_status(cudaStream_t stream, int *code);
+// Waits for the stream; *code: a wait that ran out in a product on the current device, `device`, since this host thread's last call
+// (its first: since the library was loaded), 0 for none.
+constexpr int kMaxStatusDevices = 64;
+cudaError_t expert_mm_status(int device, cudaStream_t stream, int *code);
 
 }  // namespace ios

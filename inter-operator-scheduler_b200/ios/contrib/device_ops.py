@@ -269,7 +269,10 @@ def combine_experts(y, gates, slots, out_dtype=None, out=None):
 
 
 def device_ops_status(device=None):
-    """Waits for torch's current stream of ``device`` and raises if a bounded wait inside a product ran out since the last call."""
+    """
+    Waits for torch's current stream of ``device`` and raises if a bounded wait inside a product there, on any stream, ran out
+    since the calling thread last asked (or ever): the output of that product is incomplete, which nothing else tells.
+    """
     if torch is None:
         _load()
     index = torch.cuda.current_device() if device is None else torch.device(device).index or 0

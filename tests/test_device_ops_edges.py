@@ -11,3 +11,9 @@ def test_what_a_wait_may_take_is_checked():
         with pytest.raises(RuntimeError, match='product_wait_us'):
             rt.set_option('product_wait_us', bad)
     rt.set_option('product_wait_us', 0)
+
+
+def test_status_of_no_device_is_refused():
+    for device in (-1, 64):
+        assert rt.load_ios_library().ios_device_ops_status(device, None) == 3
+        assert b'device_ops_status' in rt.load_ios_library().ios_last_error()

@@ -155,3 +155,32 @@ def test_products_end_whichever_wait_runs_out(short_waits, us, dtype, x_rows, to
     short_waits(0)
     assert torch.equal(rt.grouped_matmul(x, w, offsets, **args), expect)
     assert not ran_out()
+
+
+def test_every_thread_is_told_of_a_wait_that_ran_out(short_waits):
+    """One thread's question does not answer another's; nobody is told twice."""
+    inner = 1 << 23
+    x = torch.ones(1, inner, dtype=BF16, device='cuda').expand(64, -1)
+    w = torch.ones(1, 1, inner, dtype=BF16, device='cuda').expand(1, 128, -1)
+    told, asked = {}, [threading.Barrier(3) for _ in range(3)]
+
+    def ask(name):
+        ran_out()                                               # what lies before this test
+        asked[0].wait(60)
+        asked[1].wait(60)                                       # the product has run out of time meanwhile
+        told[name] = (ran_out(), ran_out())
+        asked[2].wait(60)
+
+    threads = [threading.Thread(target=ask, args=(name,)) for name in ('first', 'second')]
+    for thread in threads:
+        thread.start()
+    ran_out()
+    asked[0].wait(60)
+    short_waits(100)
+    rt.grouped_matmul(x, w, torch.tensor([0, 64], dtype=torch.int32, device='cuda'))
+    assert ran_out() and not ran_out()
+    asked[1].wait(60)
+    asked[2].wait(60)
+    for thread in threads:
+        thread.join()
+    assert told == {'first': (True, False), 'second': (True, False)}
