@@ -111,6 +111,7 @@ __device__ __forceinline__ float softmax_term(float v, float top) { return v == 
 
 constexpr int kRouteThreads = 1024;       // 32 warps hide one another's reductions; a call of a few tokens takes 256 threads
 constexpr int kRoutePairs = 8192;         // pairs that a block plans in shared memory
+constexpr int kRouteDirectBlocks = 128;   // blocks whose counts each block of the second pass sums for itself
 
 // The k best experts of tokens [first, last): one warp per token, logit e in register e / 32 of lane e % 32; the next
 // token's logits are on their way meanwhile.  Each pick takes one or two warp reductions and drops the winner.
@@ -275,8 +276,37 @@ __global__ void __launch_bounds__(kRouteThreads) route_pick_kernel(const RoutePa
         for (int i = used + int(threadIdx.x); i < pairs; i += blockDim.x) p.rows[i] = -1;
 }
 
+// Very long calls: the counts of every expert become, in place, the pairs of earlier blocks, its total stands behind them.  A lane per
+// expert, a warp per range of blocks.  (Blocks of the second pass that each read all counts would read blocks^2 x experts.)
+__global__ void __launch_bounds__(kRouteThreads) route_scan_kernel(const RouteParams p, int blocks) {
+    constexpr int kRanges = kRouteThreads / 32;
+    __shared__ int sums[kRanges][32];
+    const int lane = threadIdx.x & 31, range = threadIdx.x >> 5, e = int(blockIdx.x) * 32 + lane;
+    grid_dependency_entry();
+    const int b0 = int((long long)blocks * range / kRanges), b1 = int((long long)blocks * (range + 1) / kRanges);
+    int *counts = p.block_counts + e;
+    int sum = 0;
+    if (e < p.experts) {
+#pragma unroll 8
+        for (int b = b0; b < b1; ++b) sum += counts[(long long)b * p.experts];
+    }
+    sums[range][lane] = sum;
+    __syncthreads();
+    if (e >= p.experts) return;
+    int run = 0;
+    for (int r = 0; r < range; ++r) run += sums[r][lane];
+#pragma unroll 8
+    for (int b = b0; b < b1; ++b) {
+        const int c = counts[(long long)b * p.experts];
+        counts[(long long)b * p.experts] = run;
+        run += c;
+    }
+    if (range == kRanges - 1) counts[(long long)blocks * p.experts] = run;
+}
+
 // Second pass of a plan over many blocks: block b adds, per expert, the expert's start and the pairs of blocks < b.
-// Every block sums the counts of all blocks; the threads share that by expert and by range of blocks.
+// Every block sums the counts of all blocks; the threads share that by expert and by range of blocks.  Beyond
+// kRouteDirectBlocks, route_scan_kernel has summed them.
 __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteParams p, int per_block, int blocks) {
     extern __shared__ int shared[];                    // [experts] starts, [experts] pairs in earlier blocks
     int *start = shared, *earlier = shared + p.experts;
@@ -285,7 +315,12 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteP
     __syncthreads();
     const int ranges = max(1, int(blockDim.x) / p.experts);        // threads per expert
     const int e = int(threadIdx.x) % p.experts, range = int(threadIdx.x) / p.experts;
-    if (range < ranges) {
+    if (blocks > kRouteDirectBlocks) {
+        for (int i = threadIdx.x; i < p.experts; i += blockDim.x) {
+            start[i] = p.block_counts[(long long)blocks * p.experts + i];
+            earlier[i] = p.block_counts[(long long)blockIdx.x * p.experts + i];
+        }
+    } else if (range < ranges) {
         const int b0 = blocks * range / ranges, b1 = blocks * (range + 1) / ranges;
         int sum = 0, before = 0;
 #pragma unroll 8
@@ -318,12 +353,12 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteP
         p.rows[i] = -1;
 }
 
-// Tokens one block plans: a small call is one block and one launch; beyond that about 128 blocks, because every block of
-// the second pass reads the counts of all of them.
+// Tokens one block plans: a small call is one block and one launch; beyond that at most kRouteDirectBlocks blocks, because every
+// block of the second pass reads the counts of all of them, until kRoutePairs fill a block; then as many blocks as there are such.
 constexpr int kRouteSingleTokens = 128;
 int route_per_block(int tokens, int k) {
     if (tokens <= kRouteSingleTokens) return tokens;
-    return std::min(std::max(32, (tokens + 127) / 128), kRoutePairs / k);
+    return std::min(std::max(32, (tokens + kRouteDirectBlocks - 1) / kRouteDirectBlocks), kRoutePairs / k);
 }
 int route_blocks(int tokens, int k) { return (tokens + route_per_block(tokens, k) - 1) / route_per_block(tokens, k); }
 
@@ -354,6 +389,8 @@ cudaError_t route_run(const RouteParams &p, cudaStream_t stream) {
     cudaError_t err = blocks == 1 ? allow_route_smem<T, PER, true>() : allow_route_smem<T, PER, false>();
     if (err != cudaSuccess) return err;
     err = launch(pick, blocks, threads, smem, stream, p, per_block);
+    if (err == cudaSuccess && blocks > kRouteDirectBlocks)
+        err = launch(route_scan_kernel, (p.experts + 31) / 32, kRouteThreads, 0, stream, p, blocks);
     if (err == cudaSuccess && blocks > 1)
         err = launch(route_place_kernel, blocks, kRouteThreads, 2 * size_t(p.experts) * sizeof(int), stream, p, per_block, blocks);
     return err;
@@ -645,7 +682,7 @@ cudaError_t combine_typed(const CombineParams &p, cudaStream_t stream) {
 
 size_t route_workspace_bytes(int tokens, int experts, int k) {
     const int blocks = route_blocks(tokens, k);
-    return blocks == 1 ? 0 : size_t(blocks) * experts * sizeof(int);
+    return blocks == 1 ? 0 : size_t(blocks + (blocks > kRouteDirectBlocks ? 1 : 0)) * experts * sizeof(int);
 }
 
 cudaError_t launch_route(const RouteParams &p, cudaStream_t stream) {

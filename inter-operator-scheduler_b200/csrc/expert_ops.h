@@ -27,7 +27,7 @@ struct RouteParams {
     int *offsets;           // [experts + 1]
     int *rows;              // [tokens * k]
     int *slots;             // [tokens][k]
-    int *block_counts;      // workspace, [blocks][experts]; unused when one block does everything
+    int *block_counts;      // workspace, [blocks][experts], long calls: and their sums; unused when one block does everything
 };
 size_t route_workspace_bytes(int tokens, int experts, int k);
 cudaError_t launch_route(const RouteParams &p, cudaStream_t stream);

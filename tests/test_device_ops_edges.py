@@ -1,6 +1,8 @@
 """
 Arguments of the operators on device tensors at the edges of what they take, on a machine without a GPU.
 """
+import ctypes
+
 import pytest
 
 from ios.contrib import ios_runtime as rt
@@ -17,3 +19,11 @@ def test_status_of_no_device_is_refused():
     for device in (-1, 64):
         assert rt.load_ios_library().ios_device_ops_status(device, None) == 3
         assert b'device_ops_status' in rt.load_ios_library().ios_last_error()
+
+
+def test_route_workspace_of_long_calls():
+    """A row of counts per block of 8192 pairs, and beyond 128 blocks one more; linear in the tokens."""
+    lib, size = rt.load_ios_library(), ctypes.c_size_t(0)
+    for tokens, rows in ((131072, 128), (131073, 130), (1 << 27, (1 << 17) + 1)):
+        assert lib.ios_route_experts_workspace(tokens, 64, 8, ctypes.byref(size)) == 0
+        assert size.value == rows * 64 * 4

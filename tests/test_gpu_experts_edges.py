@@ -184,3 +184,27 @@ def test_every_thread_is_told_of_a_wait_that_ran_out(short_waits):
     for thread in threads:
         thread.join()
     assert told == {'first': (True, False), 'second': (True, False)}
+
+
+# ---- router: calls of more blocks than read one another's counts -----------------------------------------
+
+@pytest.mark.parametrize('tokens,experts,k,dtype', [
+    (131072, 64, 8, BF16), (131073, 64, 8, BF16), (300000, 100, 32, F32), (1100003, 4, 1, F16), (270000, 1024, 4, F32), (33000, 33, 32, BF16)])
+def test_route_of_many_tokens(tokens, experts, k, dtype):
+    logits = torch.randn(tokens, experts, generator=generator(tokens), device='cuda').to(dtype)
+    logits[::17] = -float('inf')
+    got = rt.route_experts(logits, k)
+    best, index = torch.sort(logits.float(), dim=1, descending=True, stable=True)
+    chosen = torch.where(best[:, :k] > -float('inf'), index[:, :k], -1)
+    assert torch.equal(got.experts.long(), chosen)
+    flat = torch.where(chosen < 0, experts, chosen).flatten()
+    order = torch.sort(flat, stable=True).indices
+    counts = torch.bincount(flat, minlength=experts + 1)[:experts]
+    used = int(counts.sum())
+    assert torch.equal(got.offsets.long(), torch.cat([counts.new_zeros(1), counts.cumsum(0)]))
+    assert torch.equal(got.rows[:used].long(), order[:used] // k) and (got.rows[used:] == -1).all()
+    slots = torch.full_like(flat, -1)
+    slots[order[:used]] = torch.arange(used, device='cuda')
+    assert torch.equal(got.slots.flatten().long(), slots)
+    gates = torch.softmax(best[:, :k].double(), 1).nan_to_num(0.0)
+    assert ((got.gates.double() - gates).abs() <= 90 * U * gates + 1e-30).all()
