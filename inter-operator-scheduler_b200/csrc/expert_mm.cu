@@ -355,10 +355,11 @@ __device__ __forceinline__ void split_tf32(uint32_t x, uint32_t *hi, uint32_t *l
     *lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(h)) + 0x1000u;
 }
 
+// sigmoid(v) = (v < 0 ? e : 1) / (1 + e) with e = exp(-|v|): exp(-v) passes float32 from v = -88 on, where the result is still one.
 __device__ __noinline__ float act_far(float v, int act) {
-    if (act == 4) return v / (1.0f + expf(-v));
-    if (act == 2) return 1.0f / (1.0f + expf(-v));
-    return tanhf(v);
+    if (act == 3) return tanhf(v);
+    const float e = expf(-fabsf(v));
+    return (act == 4 ? (v < 0.0f ? v * e : v) : (v < 0.0f ? e : 1.0f)) / (1.0f + e);
 }
 // the activation of N values; one branch for all of them.  Results that are rounded to 16 bits take the fast exponential.
 template <int N>
@@ -369,7 +370,10 @@ __device__ __forceinline__ void activate(float *v, int act, bool fast) {
         for (int c = 0; c < N; ++c) v[c] = fmaxf(v[c], 0.0f);
     } else if (act == 4 && fast) {
 #pragma unroll
-        for (int c = 0; c < N; ++c) v[c] = __fdividef(v[c], 1.0f + __expf(-v[c]));
+        for (int c = 0; c < N; ++c) {
+            const float e = __expf(-fabsf(v[c]));
+            v[c] = __fdividef(v[c] < 0.0f ? v[c] * e : v[c], 1.0f + e);
+        }
     } else {
 #pragma unroll
         for (int c = 0; c < N; ++c) v[c] = act_far(v[c], act);

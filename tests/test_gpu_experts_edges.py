@@ -14,7 +14,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip('torch')
 
-from test_gpu_experts import BF16, F16, F32, U, check_route, generator, quantize_reference  # noqa: E402
+from test_gpu_experts import BF16, F16, F32, U, check_route, generator, half_step, quantize_reference  # noqa: E402
 
 
 # ---- quantiser: magnitudes whose products with 254 pass float32 ------------------------------------
@@ -208,3 +208,25 @@ def test_route_of_many_tokens(tokens, experts, k, dtype):
     assert torch.equal(got.slots.flatten().long(), slots)
     gates = torch.softmax(best[:, :k].double(), 1).nan_to_num(0.0)
     assert ((got.gates.double() - gates).abs() <= 90 * U * gates + 1e-30).all()
+
+
+# ---- activations far from zero ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize('out_dtype', [BF16, F16, F32], ids=['bf16', 'fp16', 'fp32'])
+@pytest.mark.parametrize('act', ['silu', 'sigmoid'])
+def test_activations_far_from_zero(act, out_dtype):
+    """exp(-v) passes float32 below v = -88, the result does not.  The exponential is off by 2 + 1.2 |v| steps of 2^-23, the quotient and
+    the product by 3 more; below 2^-126 steps have one size, 2^-149, which |v| <= 104 multiplies."""
+    v = torch.cat([torch.arange(-104.0, 20.0, 0.25, device='cuda'), torch.tensor([-1e30, -200.0, 200.0, 1e30, 0.0, -0.0], device='cuda')]).to(BF16)
+    got = rt.grouped_matmul(torch.ones(1, 1, dtype=BF16, device='cuda'), v[None, :, None].contiguous(),
+                            torch.tensor([0, 1], dtype=torch.int32, device='cuda'), act=act, out_dtype=out_dtype)[0].double()
+    a = v.double()
+    expect = a * torch.sigmoid(a) if act == 'silu' else torch.sigmoid(a)
+    bound = (6 + 1.2 * a.abs().clamp(max=104)) * 2.0 ** -23 * expect.abs() + 2.0 ** -140
+    bound = bound + half_step(out_dtype) * (expect.abs() + bound) + torch.finfo(out_dtype).smallest_normal * torch.finfo(out_dtype).eps
+    inside = expect.abs() <= torch.finfo(out_dtype).max
+    assert ((got - expect).abs() <= bound)[inside].all()
+    special = torch.tensor([float('inf'), float('nan')], device='cuda').to(BF16)
+    got = rt.grouped_matmul(torch.ones(1, 1, dtype=BF16, device='cuda'), special[None, :, None].contiguous(),
+                            torch.tensor([0, 1], dtype=torch.int32, device='cuda'), act=act, out_dtype=out_dtype)[0]
+    assert got[0] == (float('inf') if act == 'silu' else 1.0) and torch.isnan(got[1])
