@@ -856,7 +856,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         int turn = 0, round = 0;
         bool ok = true;
 #pragma unroll 1
-        for (int i = tile0, n = 0; i < total_tiles; i += tile_step, ++n, ++round) {
+        for (int i = tile0, n = 0; i < total_tiles && ok; i += tile_step, ++n, ++round) {
             const Tile tile = tile_of(p, t, table, n, i, cta_channel);
             const int warp_channel = tile.channel0 + quad * kWidth;
             const int channel = warp_channel + lane % kWidth;
@@ -879,7 +879,6 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 }
                 asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory");
             }
-            if (!ok) continue;                                        // a warp that gave up keeps the others' barrier whole, no more
             // ---- the sums of this CTA's K range ----
             uint32_t sums = lane_tmem + (uint32_t(turn) & 1u) * uint32_t(t.tn), held = acc_empty0 + 8u * (uint32_t(turn) & 1u);
             if (KIND != kX3) {
@@ -911,7 +910,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             }
             if (ok && t.cluster > 1 && round > 0) ok = wait<true>(recv_free, uint32_t(round - 1) & 1u, t.wait_ns);
             ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
-            if (!ok) continue;
+            if (!ok) break;
             tc_fence_after();
             const auto release = [&]() {                              // the accumulator may be written again
                 if (KIND == kX3) return;
@@ -939,7 +938,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 __syncwarp();
                 if (lane < t.cluster) mbar_arrive_cluster(cluster_map(recv_full, uint32_t(lane)));
                 ok = __all_sync(0xffffffffu, wait<true>(recv_full, uint32_t(round) & 1u, t.wait_ns) ? 1 : 0) != 0;
-                if (!ok) continue;
+                if (!ok) break;
                 // pairs of columns: a gated result takes two lanes' columns at once
                 const int mine = kShare == 1 ? per : (per / 2 + 1) / 2 * 2;          // columns of the first warp of a quarter
                 from = rank * per + share * mine;
@@ -1025,7 +1024,14 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 if (lane < t.cluster) mbar_arrive_cluster(cluster_map(recv_free, uint32_t(lane)));
             }
         }
-        if (!ok && lane == 0) time_out(5);
+        if (!ok) {
+            if (lane == 0) time_out(5);
+            __syncwarp();
+            // the rest may still be at work: their barrier needs this warp in every tile to come
+            if (p.row_scale || (LOADS != kTma && p.rows))
+                for (int i = tile0 + (round + 1) * tile_step; i < total_tiles; i += tile_step)
+                    asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory");
+        }
     }
     __syncwarp();
     tc_fence_before();
