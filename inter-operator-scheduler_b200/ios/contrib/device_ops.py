@@ -44,6 +44,7 @@ _codes = {}           # torch type -> element type of the C interface
 _lib = None
 _raw_stream = None
 _FLOATS, _ALL, _INT8 = (0, 1, 2), (0, 1, 2, 3), (3,)
+_MOST_ROWS, _MOST = 1 << 30, (1 << 31) - 1      # rows of a call; any other size: the C interface counts in 32 bits
 
 
 def _load():
@@ -124,6 +125,10 @@ def _output(out, out_dtype, default, like, shape):
     return out, code, max(out.stride(0), shape[1]) if shape[0] == 1 else out.stride(0)
 
 
+def _too_large(what):
+    raise ValueError(f'more than 2^30 rows, or rows of 2^31 elements or more: {what}')
+
+
 def _act(act):
     code = _ACTS.get(act)
     if code is None:
@@ -156,6 +161,8 @@ def route_experts(logits, k, renormalize=True):
     code = _matrix(logits, 'logits', 2, _FLOATS)
     tokens, experts = logits.shape
     k = int(k)
+    if tokens * k > _MOST_ROWS or experts > _MOST:
+        _too_large(f'logits of shape {tuple(logits.shape)}, k = {k}')
     if not 1 <= k <= experts:
         raise ValueError(f'k must be in 1..{experts}, not {k}')
     pairs, need = tokens * k, _route_workspace(tokens, experts, k)
@@ -198,6 +205,8 @@ def grouped_matmul(x, weight, offsets, rows=None, bias=None, act='identity', gat
             raise ValueError(f'a gated product needs an even number of weight rows, not {per_group}')
         channels = per_group // 2
     total = x_rows if rows is None else _length(rows)
+    if total > _MOST_ROWS or per_group > _MOST or inner > _MOST or groups > _MOST:
+        _too_large(f'{total} rows, weight of shape {tuple(weight.shape)}')
     f32, i32 = torch.float32, torch.int32
     out, out_code, out_stride = _output(out, out_dtype, torch.bfloat16 if code == 3 else x.dtype, x, (total, channels))
     _check(_lib.ios_grouped_matmul(
@@ -223,6 +232,8 @@ def matmul_int8(a, b, row_scale=None, channel_scale=None, bias=None, act='identi
     channels, b_inner = b.shape
     if b_inner != inner:
         raise ValueError(f'a has rows of {inner} elements, b of {b_inner}')
+    if rows > _MOST_ROWS or channels > _MOST or inner > _MOST:
+        _too_large(f'a of shape {tuple(a.shape)}, b of shape {tuple(b.shape)}')
     f32 = torch.float32
     out, out_code, out_stride = _output(out, out_dtype, torch.bfloat16, a, (rows, channels))
     _check(_lib.ios_matmul_int8(
@@ -242,6 +253,8 @@ def quantize_rows(x, rows=None):
     index = x.get_device()
     x_rows, inner = x.shape
     total = x_rows if rows is None else _length(rows)
+    if total > _MOST_ROWS or inner > _MOST:
+        _too_large(f'{total} rows of {inner} elements')
     q, scale = x.new_empty((total, inner), dtype=torch.int8), x.new_empty((total,), dtype=torch.float32)
     _check(_lib.ios_quantize_rows(
         x.data_ptr(), code, x_rows, x.stride(0), inner, _dense(rows, 'rows', (total,), torch.int32, index), total, q.data_ptr(), inner,
@@ -260,6 +273,8 @@ def combine_experts(y, gates, slots, out_dtype=None, out=None):
     index = y.get_device()
     y_rows, channels = y.shape
     shape = tokens, k = slots.shape
+    if tokens > _MOST_ROWS or k > _MOST or channels > _MOST:
+        _too_large(f'y of shape {tuple(y.shape)}, slots of shape {tuple(shape)}')
     out, out_code, out_stride = _output(out, out_dtype, y.dtype, y, (tokens, channels))
     _check(_lib.ios_combine_experts(
         y.data_ptr(), code, y_rows, y.stride(0), _needed(gates, 'gates', shape, torch.float32, index),

@@ -14,7 +14,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip('torch')
 
-from test_gpu_experts import BF16, F16, F32, U, check_route, generator, half_step, quantize_reference  # noqa: E402
+from test_gpu_experts import BF16, F16, F32, S8, U, check_route, generator, half_step, quantize_reference  # noqa: E402
 
 
 # ---- quantiser: magnitudes whose products with 254 pass float32 ------------------------------------
@@ -230,3 +230,24 @@ def test_activations_far_from_zero(act, out_dtype):
     got = rt.grouped_matmul(torch.ones(1, 1, dtype=BF16, device='cuda'), special[None, :, None].contiguous(),
                             torch.tensor([0, 1], dtype=torch.int32, device='cuda'), act=act, out_dtype=out_dtype)[0]
     assert got[0] == (float('inf') if act == 'silu' else 1.0) and torch.isnan(got[1])
+
+
+# ---- sizes past 32 bits ------------------------------------------------------------------------------------
+
+def test_sizes_past_32_bits_are_refused():
+    """(A row count of 2^32 + 4 is 4 in 32 bits: the rest of the result would be left unwritten.)"""
+    many, offsets = 2 ** 32 + 4, torch.zeros(2, dtype=torch.int32, device='cuda')
+    row, row8 = torch.zeros(1, 16, dtype=BF16, device='cuda'), torch.zeros(1, 16, dtype=S8, device='cuda')
+    for call in (lambda: rt.route_experts(row.expand(many, -1), 1), lambda: rt.matmul_int8(row8.expand(many, -1), row8),
+                 lambda: rt.matmul_int8(row8, row8.expand(many, -1)), lambda: rt.quantize_rows(row.expand(many, -1)),
+                 lambda: rt.grouped_matmul(row.expand(many, -1), row[None], offsets),
+                 lambda: rt.grouped_matmul(row, row[None].expand(1, many, -1), offsets),
+                 lambda: rt.grouped_matmul(row, row[None].expand(many, -1, -1), offsets),
+                 lambda: rt.route_experts(row.expand(2 ** 30, -1), 2)):
+        with pytest.raises(ValueError, match='more than'):
+            call()
+    wide = torch.zeros(1, 2 ** 31 + 8, dtype=S8, device='cuda')
+    with pytest.raises(ValueError, match='more than'):
+        rt.matmul_int8(wide, wide)
+    with pytest.raises(ValueError, match='more than'):
+        rt.quantize_rows(torch.zeros(1, 2 ** 31, dtype=F16, device='cuda'))
