@@ -290,5 +290,12 @@ def device_ops_status(device=None):
     """
     if torch is None:
         _load()
-    index = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    index = None
+    if device is not None:
+        device = torch.device(device)
+        if device.type != 'cuda':
+            raise ValueError(f'{device} is not a GPU')
+        index = device.index
+    if index is None:                            # None, or 'cuda' without a number
+        index = torch.cuda.current_device()
     _check(_lib.ios_device_ops_status(index, _raw_stream(index)))

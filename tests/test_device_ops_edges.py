@@ -27,3 +27,25 @@ def test_route_workspace_of_long_calls():
     for tokens, rows in ((131072, 128), (131073, 130), (1 << 27, (1 << 17) + 1)):
         assert lib.ios_route_experts_workspace(tokens, 64, 8, ctypes.byref(size)) == 0
         assert size.value == rows * 64 * 4
+
+
+def test_status_asks_about_the_device_that_is_meant(monkeypatch):
+    """'cuda' without a number is the current device, as everywhere in torch."""
+    torch = pytest.importorskip('torch')
+    from ios.contrib import device_ops
+    asked = []
+
+    class Library:
+        def ios_device_ops_status(self, index, stream):
+            asked.append((index, stream))
+            return 0
+
+    monkeypatch.setattr(device_ops, 'torch', torch)
+    monkeypatch.setattr(device_ops, '_lib', Library())
+    monkeypatch.setattr(device_ops, '_raw_stream', lambda index: 100 + index)
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: 3)
+    for device in (None, 'cuda', torch.device('cuda'), 'cuda:2', torch.device('cuda', 0), 1):
+        rt.device_ops_status(device)
+    assert asked == [(index, 100 + index) for index in (3, 3, 3, 2, 0, 1)]
+    with pytest.raises(ValueError, match='not a GPU'):
+        rt.device_ops_status('cpu')
