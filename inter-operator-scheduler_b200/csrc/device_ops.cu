@@ -99,7 +99,7 @@ int run_grouped(const GroupedParams &p, const char *what, void *stream) {
         record_error("");
         return IOS_OK;
     }
-    if (!p.x || !p.w || !p.y) return fail(IOS_ERR_ARGUMENT, "%s: x, w and y must not be NULL", what);
+    if ((!p.x && p.x_rows > 0) || !p.w || !p.y) return fail(IOS_ERR_ARGUMENT, "%s: x, w and y must not be NULL", what);
     DeviceScope scope;
     if (int status = scope.enter(p.y)) return status;
     if (int status = scope.same(p.x, "x")) return status;
@@ -236,7 +236,7 @@ extern "C" int ios_quantize_rows(const void *x, int type, long long x_rows, long
         record_error("");
         return IOS_OK;
     }
-    if (!x || !q || !scale) return fail(IOS_ERR_ARGUMENT, "quantize_rows: x, q and scale must not be NULL");
+    if ((!x && x_rows > 0) || !q || !scale) return fail(IOS_ERR_ARGUMENT, "quantize_rows: x, q and scale must not be NULL");
     DeviceScope scope;
     if (int status = scope.enter(q)) return status;
     if (int status = scope.same(x, "x")) return status;

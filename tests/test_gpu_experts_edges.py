@@ -14,7 +14,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip('torch')
 
-from test_gpu_experts import BF16, F16, F32, S8, U, check_route, generator, half_step, quantize_reference  # noqa: E402
+from test_gpu_experts import BF16, F16, F32, S8, U, check_route, generator, half_step, make_operands, quantize_reference  # noqa: E402
 
 
 # ---- quantiser: magnitudes whose products with 254 pass float32 ------------------------------------
@@ -251,3 +251,27 @@ def test_sizes_past_32_bits_are_refused():
         rt.matmul_int8(wide, wide)
     with pytest.raises(ValueError, match='more than'):
         rt.quantize_rows(torch.zeros(1, 2 ** 31, dtype=F16, device='cuda'))
+
+
+# ---- rows that name none of no rows --------------------------------------------------------------------------
+
+@pytest.mark.parametrize('dtype', [BF16, F16, F32, S8], ids=['bf16', 'fp16', 'fp32', 'int8'])
+@pytest.mark.parametrize('gated', [False, True])
+def test_product_of_rows_that_are_not_there(dtype, gated):
+    """x without rows: every entry of `rows` reads as zeros, whatever the weights hold."""
+    gen = generator(5)
+    _, w = make_operands(gen, (1, 64), (2, 48, 64), dtype)
+    if dtype != S8:
+        w[0, 0] = float('nan')
+    x, bias = w.new_empty(0, 64), torch.randn(2, 48, generator=gen, device='cuda')
+    offsets, rows = (torch.tensor(v, dtype=torch.int32, device='cuda') for v in ([0, 3, 40], [-1, 0, 2 ** 31 - 1] + [-1] * 37))
+    got = rt.grouped_matmul(x, w, offsets, rows=rows, bias=bias, act='relu', gated=gated, out_dtype=F32, row_scale=x.new_empty(0, dtype=F32),
+                            channel_scale=torch.ones(2, 48, device='cuda'))
+    v = torch.repeat_interleave(bias, torch.tensor([3, 37], device='cuda'), 0)
+    assert torch.equal(got, v[:, :24].clamp(min=0) * v[:, 24:] if gated else v.clamp(min=0))
+
+
+@pytest.mark.parametrize('inner', [64, 63])
+def test_quantized_rows_that_are_not_there(inner):
+    q, scale = rt.quantize_rows(torch.empty(0, inner, device='cuda'), rows=torch.tensor([-1, 0, 5], dtype=torch.int32, device='cuda'))
+    assert tuple(q.shape) == (3, inner) and (q == 0).all() and (scale == 0).all()
