@@ -275,3 +275,25 @@ def test_product_of_rows_that_are_not_there(dtype, gated):
 def test_quantized_rows_that_are_not_there(inner):
     q, scale = rt.quantize_rows(torch.empty(0, inner, device='cuda'), rows=torch.tensor([-1, 0, 5], dtype=torch.int32, device='cuda'))
     assert tuple(q.shape) == (3, inner) and (q == 0).all() and (scale == 0).all()
+
+
+# ---- derivatives, versions ---------------------------------------------------------------------------------------
+
+def test_tangents_are_refused():
+    """Forward-mode derivatives of any argument, also under torch.no_grad(), which does not switch them off."""
+    from torch.autograd import forward_ad
+    x, w, logits = torch.randn(4, 8, device='cuda'), torch.randn(1, 6, 8, device='cuda'), torch.randn(4, 3, device='cuda')
+    offsets, bias = torch.tensor([0, 4], dtype=torch.int32, device='cuda'), torch.randn(1, 6, device='cuda')
+    plan = rt.route_experts(logits, 2)
+    y = torch.randn(8, 8, device='cuda')
+    expect = rt.grouped_matmul(x, w, offsets, bias=bias)
+    with forward_ad.dual_level(), torch.no_grad():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: rt.route_experts(dual(logits), 2), lambda: rt.grouped_matmul(dual(x), w, offsets),
+                     lambda: rt.grouped_matmul(x, dual(w), offsets), lambda: rt.grouped_matmul(x, w, offsets, bias=dual(bias)),
+                     lambda: rt.quantize_rows(dual(x)), lambda: rt.combine_experts(dual(y), plan.gates, plan.slots),
+                     lambda: rt.combine_experts(y, dual(plan.gates), plan.slots)):
+            with pytest.raises(ValueError, match='tangent'):
+                call()
+        assert torch.equal(rt.grouped_matmul(forward_ad.unpack_dual(dual(x)).primal, w, offsets, bias=bias), expect)
