@@ -120,7 +120,10 @@ def _length(rows, name='rows'):
 
 
 def _output(out, out_dtype, default, like, shape):
-    """(tensor, code of its type, row stride): a new one of `out_dtype`, else `default`, or the caller's after a check."""
+    """
+    (tensor, code of its type, row stride): a new one of `out_dtype`, else `default`, or the caller's after a check, marked
+    as changed for whatever autograd has saved it for.
+    """
     if out is None:
         dtype = default if out_dtype is None else out_dtype
         code = _codes.get(dtype)
@@ -131,6 +134,7 @@ def _output(out, out_dtype, default, like, shape):
     if out.shape != shape or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError(f'out must be a {out.dtype if out_dtype is None else out_dtype} tensor of shape {shape}')
     _same_device(out, 'out', like.get_device())
+    torch.autograd.graph.increment_version(out)
     return out, code, max(out.stride(0), shape[1]) if shape[0] == 1 else out.stride(0)
 
 

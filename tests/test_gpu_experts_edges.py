@@ -297,3 +297,21 @@ def test_tangents_are_refused():
             with pytest.raises(ValueError, match='tangent'):
                 call()
         assert torch.equal(rt.grouped_matmul(forward_ad.unpack_dual(dual(x)).primal, w, offsets, bias=bias), expect)
+
+
+def test_a_result_written_into_a_saved_tensor_is_noticed():
+    """torch refuses a backward pass through a tensor that an `out` has overwritten since."""
+    x, w = torch.randn(4, 8, device='cuda'), torch.randn(1, 6, 8, device='cuda')
+    offsets = torch.tensor([0, 4], dtype=torch.int32, device='cuda')
+    plan = rt.route_experts(torch.randn(4, 3, device='cuda'), 2)
+    q = torch.ones(4, 16, dtype=S8, device='cuda')
+    for write, shape in ((lambda out: rt.grouped_matmul(x, w, offsets, out=out), (4, 6)), (lambda out: rt.matmul_int8(q, q, out=out), (4, 4)),
+                         (lambda out: rt.combine_experts(torch.randn(8, 8, device='cuda'), plan.gates, plan.slots, out=out), (4, 8))):
+        leaf, out = torch.ones(shape, device='cuda', requires_grad=True), torch.ones(shape, device='cuda')
+        product = (leaf * out).sum()
+        write(out)
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            product.backward()
+    with torch.inference_mode():
+        out = torch.empty(4, 6, device='cuda')
+        assert torch.equal(rt.grouped_matmul(x, w, offsets, out=out), rt.grouped_matmul(x, w, offsets))
