@@ -93,6 +93,13 @@ int check_grouped(const GroupedParams &p, const char *what) {
     return IOS_OK;
 }
 
+int check_route_limits(int tokens, int experts, int k) {
+    if (experts > kMaxExperts || k > kMaxChosen)
+        return fail(IOS_ERR_LIMIT, "route_experts: at most %d experts and %d of them per token", kMaxExperts, kMaxChosen);
+    if ((long long)tokens * k > kMaxRows) return fail(IOS_ERR_LIMIT, "route_experts: more than 2^30 pairs");
+    return IOS_OK;
+}
+
 int run_grouped(const GroupedParams &p, const char *what, void *stream) {
     if (int status = check_grouped(p, what)) return status;
     if (p.total == 0) {
@@ -118,8 +125,9 @@ int run_grouped(const GroupedParams &p, const char *what, void *stream) {
 using namespace ios;
 
 extern "C" int ios_route_experts_workspace(int tokens, int experts, int k, size_t *bytes) {
-    if (!bytes || tokens < 0 || experts <= 0 || experts > kMaxExperts || k <= 0 || k > kMaxChosen)
-        return fail(IOS_ERR_ARGUMENT, "route_experts_workspace: bytes must not be NULL, tokens >= 0, experts in 1..%d, k in 1..%d", kMaxExperts, kMaxChosen);
+    if (!bytes || tokens < 0 || experts <= 0 || k <= 0 || k > experts)
+        return fail(IOS_ERR_ARGUMENT, "route_experts_workspace: bytes must not be NULL, tokens >= 0 and 1 <= k <= experts are needed");
+    if (int status = check_route_limits(tokens, experts, k)) return status;
     *bytes = tokens == 0 ? 0 : route_workspace_bytes(tokens, experts, k);
     record_error("");
     return IOS_OK;
@@ -131,9 +139,7 @@ extern "C" int ios_route_experts(const void *logits, int type, int tokens, int e
     if (!float_type(type)) return fail(IOS_ERR_ARGUMENT, "route_experts: logits must be float32, float16 or bfloat16");
     if (tokens < 0 || experts <= 0 || k <= 0 || k > experts || stride < 0)
         return fail(IOS_ERR_ARGUMENT, "route_experts: tokens >= 0, 1 <= k <= experts and stride >= 0 are needed");
-    if (experts > kMaxExperts || k > kMaxChosen)
-        return fail(IOS_ERR_LIMIT, "route_experts: at most %d experts and %d of them per token", kMaxExperts, kMaxChosen);
-    if ((long long)tokens * k > kMaxRows) return fail(IOS_ERR_LIMIT, "route_experts: more than 2^30 pairs");
+    if (int status = check_route_limits(tokens, experts, k)) return status;
     if (!offsets || (tokens > 0 && (!logits || !chosen || !gates || !rows || !slots)))
         return fail(IOS_ERR_ARGUMENT, "route_experts: logits and the outputs must not be NULL");
     const size_t need = tokens == 0 ? 0 : route_workspace_bytes(tokens, experts, k);

@@ -49,3 +49,11 @@ def test_status_asks_about_the_device_that_is_meant(monkeypatch):
     assert asked == [(index, 100 + index) for index in (3, 3, 3, 2, 0, 1)]
     with pytest.raises(ValueError, match='not a GPU'):
         rt.device_ops_status('cpu')
+
+
+def test_route_workspace_refuses_what_route_refuses():
+    """(2^31 - 1 tokens passed 32 bits on the way and came out as a size of some sort.)"""
+    lib, size = rt.load_ios_library(), ctypes.c_size_t(7)
+    for status, args in ((6, (2 ** 31 - 1, 1024, 1)), (6, (2 ** 30, 8, 2)), (6, (1, 1025, 1)), (6, (1, 64, 33)), (3, (10, 4, 8)), (3, (-1, 4, 2))):
+        assert lib.ios_route_experts_workspace(*args, ctypes.byref(size)) == status, args
+        assert b'route_experts' in lib.ios_last_error() and size.value == 7
