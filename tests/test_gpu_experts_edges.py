@@ -315,3 +315,25 @@ def test_a_result_written_into_a_saved_tensor_is_noticed():
     with torch.inference_mode():
         out = torch.empty(4, 6, device='cuda')
         assert torch.equal(rt.grouped_matmul(x, w, offsets, out=out), rt.grouped_matmul(x, w, offsets))
+
+
+# ---- 8-bit products: sums of 32 bits ------------------------------------------------------------------------------
+
+# few rows (K split over a cluster), tiles of one CTA, pairs of CTAs, rows at odd addresses, the longest rows
+@pytest.mark.parametrize('rows,inner,channels', [(3, 4096, 300), (20, 4095, 300), (300, 4096, 1100), (1500, 4096, 2100), (3, 131070, 40), (400, 131071, 40)])
+def test_matmul_int8_sums_pass_24_bits(rows, inner, channels):
+    """
+    Odd products that pass 2^24 and cancel: the result is below 2^24, so float32 holds it exactly, but a float32 sum on the
+    way, where only even numbers are left, does not reach it.
+    """
+    gen, half = generator(inner + rows), inner // 2
+    a, b = (torch.randint(50, 64, (n, half), generator=gen, device='cuda', dtype=S8) * 2 + 1 for n in (rows, channels))
+    rest = inner - 2 * half
+    a = torch.cat([a, -a, torch.ones(rows, rest, dtype=S8, device='cuda')], 1)
+    b = torch.cat([b, b, torch.ones(channels, rest, dtype=S8, device='cuda')], 1)
+    b[:, inner - 3] -= 3
+    expect = a.double() @ b.double().t()
+    assert expect.abs().max() < 2 ** 24 and half * 101 ** 2 > 2 ** 24
+    in_float32 = (a[0].cpu().float() * b[0].cpu().float()).numpy().cumsum(dtype='float32')[-1]
+    assert in_float32 != expect[0, 0].item()
+    assert torch.equal(rt.matmul_int8(a, b, out_dtype=F32).double(), expect)
