@@ -28,6 +28,9 @@ int fail(int status, const char *format, ...) {
 }
 
 constexpr int kMaxRows = 1 << 30;       // row numbers and what is added to them stay inside an int
+// Elements of a 16-bit product.  Its sums are waited for once, at the end of the rows: that many at odd addresses take 0.7 s of the 2
+// that a wait may take, four times as many ran out of time (float32 waits at every step, 8-bit rows are shorter).
+constexpr int kMaxInner16 = 1 << 25;
 
 bool float_type(int t) { return t == IOS_F32 || t == IOS_F16 || t == IOS_BF16; }
 
@@ -88,6 +91,7 @@ int check_grouped(const GroupedParams &p, const char *what) {
     if (p.y_stride < p.channels) return fail(IOS_ERR_ARGUMENT, "%s: rows of y overlap (stride %lld, %d channels)", what, p.y_stride, p.channels);
     if (p.type == Elem::S8 && p.inner >= 131072)
         return fail(IOS_ERR_LIMIT, "%s: 8-bit products of 131072 or more elements can pass the 32 bits of their sum", what);
+    if (elem_size(p.type) == 2 && p.inner > kMaxInner16) return fail(IOS_ERR_LIMIT, "%s: 16-bit products of more than 2^25 elements take too long for one wait", what);
     if (p.total > kMaxRows || grouped_too_large(p)) return fail(IOS_ERR_LIMIT, "%s: %d rows of %d channels are too many for one call", what, p.total, p.channels);
     if (!p.rows && p.x_rows < p.total) return fail(IOS_ERR_ARGUMENT, "%s: x has %lld rows, y %d", what, p.x_rows, p.total);
     return IOS_OK;

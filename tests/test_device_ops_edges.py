@@ -57,3 +57,10 @@ def test_route_workspace_refuses_what_route_refuses():
     for status, args in ((6, (2 ** 31 - 1, 1024, 1)), (6, (2 ** 30, 8, 2)), (6, (1, 1025, 1)), (6, (1, 64, 33)), (3, (10, 4, 8)), (3, (-1, 4, 2))):
         assert lib.ios_route_experts_workspace(*args, ctypes.byref(size)) == status, args
         assert b'route_experts' in lib.ios_last_error() and size.value == 7
+
+
+def test_16_bit_products_of_too_long_rows_are_refused():
+    lib = rt.load_ios_library()
+    for kind in (1, 2):
+        assert lib.ios_grouped_matmul(4096, kind, 1, 0, 4096, 1, 8, 2 ** 25 + 1, 0, 0, 4096, None, 1, None, None, None, 0, 0, 4096, 0, 8, None) == 6
+        assert b'2^25' in lib.ios_last_error()

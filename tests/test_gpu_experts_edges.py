@@ -337,3 +337,19 @@ def test_matmul_int8_sums_pass_24_bits(rows, inner, channels):
     in_float32 = (a[0].cpu().float() * b[0].cpu().float()).numpy().cumsum(dtype='float32')[-1]
     assert in_float32 != expect[0, 0].item()
     assert torch.equal(rt.matmul_int8(a, b, out_dtype=F32).double(), expect)
+
+
+# ---- the longest rows -----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize('odd', [0, 1])
+def test_the_longest_16_bit_rows_are_summed_in_time(odd):
+    """2^25 elements in one CTA each, through the slowest loads: the epilogue waits for all of them at once."""
+    inner, channels = (1 << 25) - odd, 128 * 100
+    row = torch.ones(1, inner + odd, dtype=BF16, device='cuda')[:, odd:]
+    x = torch.ones(1, inner, dtype=BF16, device='cuda').expand(128, -1)
+    row[0, 1::2] = -1
+    row[0, 7:1001:2] = 1                                        # 497 of them: 994 more, and an odd row has one 1 more than -1
+    assert not ran_out()
+    got = rt.grouped_matmul(x, row[None].expand(1, channels, -1), torch.tensor([0, 128], dtype=torch.int32, device='cuda'), out_dtype=F32)
+    assert not ran_out()
+    assert (got == 994 + odd).all()
