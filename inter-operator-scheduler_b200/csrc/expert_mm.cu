@@ -346,7 +346,7 @@ __device__ __noinline__ uint32_t load_edge(const uint8_t *row, long long off, lo
     return out;
 }
 
-// x = hi + lo + (at most 2^-22 |x|) for the tensor core, which drops the low 13 bits of an operand: hi is rounded to the
+// x = hi + lo + (at most 2^-22 |x|, or 2^-137 where lo is subnormal) for the tensor core, which drops the low 13 bits of an operand: hi is rounded to the
 // bits it keeps, lo is what is missing plus half a step of its own.  (Whole-number arithmetic: cvt.rna.tf32 runs at an eighth of
 // its rate.)  Values that would round to infinity are cut instead; an infinity's lo is NaN.
 __device__ __forceinline__ void split_tf32(uint32_t x, uint32_t *hi, uint32_t *lo) {

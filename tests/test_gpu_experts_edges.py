@@ -353,3 +353,43 @@ def test_the_longest_16_bit_rows_are_summed_in_time(odd):
     got = rt.grouped_matmul(x, row[None].expand(1, channels, -1), torch.tensor([0, 128], dtype=torch.int32, device='cuda'), out_dtype=F32)
     assert not ran_out()
     assert (got == 994 + odd).all()
+
+
+# ---- float32 elements whose smaller half is subnormal ---------------------------------------------------------------------
+
+@pytest.mark.parametrize('power', [100, 114, 118, 122, 126, 135])
+@pytest.mark.parametrize('pad', [0, 1])
+def test_float32_products_of_tiny_elements(power, pad):
+    """An element split in two loses at most 2^-22 of itself, or 2^-137, half of the last step that its smaller half has."""
+    gen = generator(power)
+    inner = 200
+    x = (torch.randn(70, inner + pad, generator=gen, device='cuda').double() * 2.0 ** -power).float()[:, pad:]
+    w = (torch.randn(1, 90, inner + pad, generator=gen, device='cuda').double() * 2.0 ** min(power, 120)).float()[:, :, pad:]
+    offsets = torch.tensor([0, 70], dtype=torch.int32, device='cuda')
+    got = rt.grouped_matmul(x, w, offsets).double()
+    a, b = x.double(), w[0].double()
+    size = a.abs() @ b.abs().t()
+    bound = (inner / 8 + 32) * 2.0 ** -23 * size + 3 * 2.0 ** -22 * size + 2.0 ** -137 * b.abs().sum(1)[None]
+    assert ((got - a @ b.t()).abs() <= 1.01 * bound + 2.0 ** -149).all()
+
+
+# ---- router: values of 16 bits that are no ordinary numbers ----------------------------------------------------------------
+
+@pytest.mark.parametrize('dtype', [BF16, F16], ids=['bf16', 'fp16'])
+@pytest.mark.parametrize('tokens', [60, 700])
+def test_route_of_odd_16_bit_values(dtype, tokens):
+    inf, nan, info = float('inf'), float('nan'), torch.finfo(dtype)
+    logits = torch.randint(-2, 3, (tokens, 40), generator=generator(6), device='cuda').to(dtype)      # many equal logits
+    logits[1] = -inf
+    logits[2] = nan
+    logits[3] = -nan
+    logits[4, 2:] = -inf
+    logits[5] = 0.0
+    logits[5, ::2] = -0.0                               # the two zeros tie
+    logits[6] = info.min
+    logits[7, 39], logits[7, 5] = inf, info.max
+    logits[8, 4:9] = inf
+    logits[9, ::3], logits[9, 1::3] = nan, -nan
+    logits[10] = torch.arange(40, device='cuda').to(dtype) * info.smallest_normal * info.eps           # subnormal ones have an order, too
+    for renormalize in (True, False):
+        check_route(logits, 8, renormalize)
