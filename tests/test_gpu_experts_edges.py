@@ -14,7 +14,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip('torch')
 
-from test_gpu_experts import BF16, F16, F32, S8, U, check_route, generator, half_step, make_operands, quantize_reference  # noqa: E402
+from test_gpu_experts import BF16, F16, F32, S8, U, check_route, generator, half_step, layer, make_operands, quantize_reference  # noqa: E402
 
 
 # ---- quantiser: magnitudes whose products with 254 pass float32 ------------------------------------
@@ -393,3 +393,53 @@ def test_route_of_odd_16_bit_values(dtype, tokens):
     logits[10] = torch.arange(40, device='cuda').to(dtype) * info.smallest_normal * info.eps           # subnormal ones have an order, too
     for renormalize in (True, False):
         check_route(logits, 8, renormalize)
+
+
+# ---- beside the graph path ----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize('precision', ['tf32x3', 'bf16'])
+def test_layers_and_an_engine_at_once(precision):
+    """Both use tensor memory and clusters: an engine in one thread, layers on a stream in another, neither changes a bit."""
+    import numpy as np
+    import ios
+    import ios_oracle as oracle
+    from helpers import seeded
+    rt.set_option('precision', precision)
+    try:
+        graph = ios.models.inception_v3()
+        graph.greedy_schedule()
+        config, _ = seeded(graph, 0)
+        engine = rt.Engine(graph, 1)
+    finally:
+        rt.set_option('precision', 'tf32x3')
+    image = oracle.normal_input(config, 1, 0)
+    expect = engine.run(image)
+    gen = generator(31)
+    inputs = []
+    for tokens, experts, k, inner, outer, dtype in ((4, 16, 4, 1024, 512, BF16), (700, 8, 2, 512, 768, F16), (33, 8, 2, 256, 192, F32)):
+        x = torch.randn(tokens, inner, generator=gen, device='cuda').to(dtype)
+        w_in = (torch.randn(experts, 2 * outer, inner, generator=gen, device='cuda') * inner ** -0.5).to(dtype)
+        w_out = (torch.randn(experts, inner, outer, generator=gen, device='cuda') * outer ** -0.5).to(dtype)
+        inputs.append((x, torch.randn(tokens, experts, generator=gen, device='cuda'), w_in, w_out, k))
+    alone = [layer(*args) for args in inputs]
+    torch.cuda.synchronize()
+    failed, done = [], threading.Event()
+
+    def images():
+        try:
+            for _ in range(150):
+                assert np.array_equal(engine.run(image), expect)
+        except Exception as error:
+            failed.append(error)
+        done.set()
+
+    thread = threading.Thread(target=images)
+    thread.start()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        while not done.is_set():
+            for args, value in zip(inputs, alone):
+                assert torch.equal(layer(*args), value)
+    thread.join()
+    engine.close()
+    assert not failed, failed
+    assert not ran_out()
