@@ -236,7 +236,8 @@ IOS_API int ios_static_scratch_status(void *cuda_stream);
  * row stride in elements and unit column stride, any alignment of the element type.  The work is enqueued on
  * cuda_stream (a cudaStream_t of that device, NULL = default stream) and NOT synchronised; nothing is allocated or
  * kept between calls, so calls may overlap and may be captured into graphs.  Outputs must not overlap inputs.
- * Sums, softmax terms and scales are float32 (8-bit products: int32).  Everything runs in a fixed order: the same
+ * Sums, softmax terms and scales are float32 (8-bit products: int32; 16-bit products add in the tensor core, which
+ * truncates: 2e-6 of a sum of 1408 elements, more in longer ones).  Everything runs in a fixed order: the same
  * inputs give the same bits.  Zero rows are no error; more than 2^30 rows or pairs are one (IOS_ERR_LIMIT). */
 enum { IOS_F32 = 0, IOS_F16 = 1, IOS_BF16 = 2, IOS_S8 = 3 };   /* element types */
 
@@ -269,7 +270,7 @@ IOS_API int ios_route_experts(const void *logits, int type, int tokens, int expe
  * x[x_rows, inner] and w[groups, channels (* 2), inner] have one type (IOS_F32: three TF32 products, fp32-grade;
  * IOS_F16, IOS_BF16: inner <= 2^25; IOS_S8: inner < 131072), y[total_rows, channels] is IOS_F32 / IOS_F16 / IOS_BF16.  row_scale[x_rows],
  * channel_scale and bias (groups x channels or 2 * channels, dense) are float32 or NULL.  act: 0 identity, 1 relu,
- * 2 sigmoid, 3 tanh, 4 silu.  offsets[groups + 1] is read on the device and must not decrease; it may stop short of
+ * 2 sigmoid, 3 tanh, 4 silu; relu of NaN is 0, as in the convolutions.  offsets[groups + 1] is read on the device and must not decrease; it may stop short of
  * total_rows, rows of y before the first group and behind the last are left as they were.  An entry of rows outside
  * [0, x_rows) reads as a row of zeros.  groups <= 1024.  Any strides and alignments are taken; rows of x and w that start on
  * 16-byte boundaries (and groups of w that do not overlap) are several times faster than others.  IOS_F32: a sum that an

@@ -25,8 +25,13 @@
 // * float32: three products a_hi b_hi + a_hi b_lo + a_lo b_hi of TF32 numbers; the operands are split in shared memory, after
 //   they have landed (or by the loader warps): 16384 rows, 2048 -> 1024, at 130 TFLOP/s, bound by three stages being loaded,
 //   split and multiplied in turn.  The tensor core truncates where it adds, which costs 1e-6 of a sum over 128 elements; so the
-//   sums of every K step, 32 elements, are added up in tensor memory, rounded to nearest: 3e-7 of the result at any length,
-//   and no slower.
+//   sums of every K step, 32 elements, are added up in tensor memory, rounded to nearest, and no slower.  Off by, relative to a
+//   result of normal numbers: 0.9e-7 at 8 elements, 2.4e-7 from 32 on, 3.2e-7 at 32768 (a float32 product on the CUDA cores, 256 rows:
+//   0.5e-7 at 8, 1e-7 at 32, 2e-7 at 128, 8e-7 at 2048).
+// * 16-bit operands: the sums of a tile's K range stay in one accumulator of 32 bits, whose additions truncate.  That costs 2e-6 of the
+//   result at 1408 elements, 4e-6 at 2048 where a few channels are ten times the others, and grows with the length (a library product: 2e-6
+//   at 2048, 9e-6 at 8192).  Far below half a step of a 16-bit result, of which it moves 2 in a thousand to the neighbour;
+//   visible in float32 results.  Adding up step by step as above would need a third accumulator, which 256-column tiles leave no room for.
 // * gated: 16 rows of the gate half and the 16 rows of the same channels of the other half alternate in the tile (one box of
 //   a five-dimensional view), so that a lane and the lane 16 further on hold the two factors of one result.
 // * Loads and tensor-core instructions are issued from warp-uniform code by a predicated lane.  Issued from a branch that one
@@ -361,7 +366,9 @@ __device__ __noinline__ float act_far(float v, int act) {
     const float e = expf(-fabsf(v));
     return (act == 4 ? (v < 0.0f ? v * e : v) : (v < 0.0f ? e : 1.0f)) / (1.0f + e);
 }
-// the activation of N values; one branch for all of them.  Results that are rounded to 16 bits take the fast exponential.
+// the activation of N values; one branch for all of them.  Results that are rounded to 16 bits take the fast exponential, which is off
+// by 2 + 1.2 |v| steps of 2^-23: 1.5e-5 of the result at the most, a thirtieth of half a float16 step, where silu is all but zero, and
+// 1e-6 around v = 5.  (32768 rows, 256 -> 2048, bfloat16: 91 us; with the exact exponential 104 in place, 264 called.)
 template <int N>
 __device__ __forceinline__ void activate(float *v, int act, bool fast) {
     if (act == 0) return;
@@ -1157,6 +1164,9 @@ int choose(const GroupedParams &p, int sm_count, bool tma, MmGeom *t, bool *pair
     const size_t recv = t->cluster > 1 ? size_t(t->tn) * kTileM * sizeof(float) : 0;
     const size_t table = kListed * sizeof(int4) + (2 * size_t(p.groups + 1) * sizeof(int) + 15) / 16 * 16;
     const size_t turn = 8 * kTurnBytes;
+    // The stages take what is left: no second CTA with tensor memory of this kernel fits beside one, and what a CTA leaves of its SM (27 KB,
+    // float32 43 KB and 8 thousand registers) is too little for a CTA of another kernel's cluster.  So no two clusters can hold one SM's tensor
+    // memory each and wait for the other's.
     const size_t fixed = 1024 + recv + turn + table + kBarBytes + kStaticBytes;
     t->stages = int(std::min<size_t>(kMaxStages, (kSmemLimit - fixed) / stage));
     static_assert((kSmemLimit - 1024 - kNarrowCols * kTileM * 4 - 8 * kTurnBytes - kListed * 16 - 2 * (kMaxExperts + 4) * 4 - kBarBytes - kStaticBytes) /

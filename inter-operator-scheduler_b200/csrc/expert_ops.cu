@@ -109,7 +109,9 @@ template <> struct Rank<__nv_bfloat16> {
 // exp(v - top), with +inf logits sharing the weight among themselves instead of producing NaN
 __device__ __forceinline__ float softmax_term(float v, float top) { return v == top ? 1.0f : expf(v - top); }
 
-constexpr int kRouteThreads = 1024;       // 32 warps hide one another's reductions; a call of a few tokens takes 256 threads
+// 32 warps, a token each at a time; a call of up to 8 tokens takes 8 warps, whose barriers cost less (4 tokens, 64 experts, k = 8: 3.1 us
+// for 4.4; 32 tokens with 8 warps: 6.4 for 5.5)
+constexpr int kRouteThreads = 1024;
 constexpr int kRoutePairs = 8192;         // pairs that a block plans in shared memory
 constexpr int kRouteDirectBlocks = 128;   // blocks whose counts each block of the second pass sums for itself
 
@@ -218,8 +220,9 @@ __device__ int exclusive_scan(int *count, int n) {
 // matching equal experts across its lanes, so nothing depends on timing.
 // kSingle: the grid is one block and the plan is finished here; otherwise slots[] holds ranks inside the block and
 // route_place_kernel adds what lies before it.
-// (16384 tokens, 128 experts, k = 8, bfloat16: 15 us, bound by the latency of the picks' reductions, not by the 4 MB read;
-// the second pass takes 9 us.)
+// (16384 tokens, 128 experts, k = 8, bfloat16: 16 us from cold caches, bound by instructions, not by the 4 MB read: 490 a token, most
+// of them the picks' comparing and selecting; instructions issue in 65 % of the cycles and the ALU is busy in 67 %.  The second pass
+// takes 9.5 us, waiting for loads: the counts of all blocks, then what the first pass left of each pair.)
 template <class T, int PER, bool kSingle>
 __global__ void __launch_bounds__(kRouteThreads) route_pick_kernel(const RouteParams p, int per_block) {
     extern __shared__ int shared[];                    // [warps][experts] counts, [experts] totals, then chosen and rank of the pairs
@@ -355,6 +358,9 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteP
 
 // Tokens one block plans: a small call is one block and one launch; beyond that at most kRouteDirectBlocks blocks, because every
 // block of the second pass reads the counts of all of them, until kRoutePairs fill a block; then as many blocks as there are such.
+// (One block, k = 8: 64 tokens of 64 experts take 7.5 us, as in two launches; 128 tokens 12.0 for 7.7, yet a call outside a graph 14.4
+// for 16.3, because the host's part of a launch is longer; 128 tokens of 256 experts 20.9 for 10.1, a call 21.0 for 16.3; 200 tokens
+// of 64 experts would take 17.5 for 7.9.)
 constexpr int kRouteSingleTokens = 128;
 int route_per_block(int tokens, int k) {
     if (tokens <= kRouteSingleTokens) return tokens;
@@ -572,7 +578,8 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_rows_kernel(const 
     }
 }
 
-// Rows of any length, alignment and stride: a row per block, read twice, element by element.
+// Rows of any length, alignment and stride: a row per block, read twice, element by element.  (8192 rows of 4095 bfloat16: 53 us, of
+// 20000: 234; float32 55 and 332.  Bound by instructions, as above, and by loads of one element.)
 template <class T>
 __global__ void __launch_bounds__(256) quantize_any_kernel(const QuantizeParams p) {
     __shared__ float warp_max[8];

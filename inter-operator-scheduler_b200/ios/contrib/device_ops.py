@@ -2,7 +2,7 @@
 Operators on device tensors: a mixture-of-experts layer and its 8-bit products.
 
 Unlike the graph entry points, which take host arrays, these take tensors that already live on a GPU (``torch.Tensor``)
-and return tensors on the same device.  The work goes to torch's current stream of that device and is not waited for;
+and return tensors on the same device; an ``out`` must not overlap what the call reads.  The work goes to torch's current stream of that device and is not waited for;
 the calls may be captured into CUDA graphs.  They compute no gradients, and refuse tensors that ask for one or carry a tangent.
 
 A layer, from its router logits to its output::
