@@ -268,11 +268,11 @@ IOS_API int ios_route_experts(const void *logits, int type, int tokens, int expe
  * src = rows[r] if rows is given, else r.  gated != 0: w, channel_scale and bias have 2 * channels rows per group and
  *     y[r, n] = act(v[n]) * v[channels + n]          (v: the value inside act(...) above).
  * x[x_rows, inner] and w[groups, channels (* 2), inner] have one type (IOS_F32: three TF32 products, fp32-grade;
- * IOS_F16, IOS_BF16: inner <= 2^25; IOS_S8: inner < 131072), y[total_rows, channels] is IOS_F32 / IOS_F16 / IOS_BF16.  row_scale[x_rows],
- * channel_scale and bias (groups x channels or 2 * channels, dense) are float32 or NULL.  act: 0 identity, 1 relu,
- * 2 sigmoid, 3 tanh, 4 silu; relu of NaN is 0, as in the convolutions.  offsets[groups + 1] is read on the device and must not decrease; it may stop short of
- * total_rows, rows of y before the first group and behind the last are left as they were.  An entry of rows outside
- * [0, x_rows) reads as a row of zeros.  groups <= 1024.  Any strides and alignments are taken; rows of x and w that start on
+ * IOS_F16, IOS_BF16: inner <= 2^25; IOS_S8: inner < 131072), y[total_rows, channels] is IOS_F32 / IOS_F16 / IOS_BF16.
+ * row_scale[x_rows], channel_scale and bias (groups x channels or 2 * channels, dense) are float32 or NULL.  act: 0 identity,
+ * 1 relu, 2 sigmoid, 3 tanh, 4 silu; relu of NaN is 0, as in the convolutions.  offsets[groups + 1] is read on the device and
+ * must not decrease; it may stop short of total_rows, rows of y before the first group and behind the last are left as they
+ * were.  An entry of rows outside [0, x_rows) reads as a row of zeros; x may have none.  groups <= 1024.  Any strides and alignments are taken; rows of x and w that start on
  * 16-byte boundaries (and groups of w that do not overlap) are several times faster than others.  IOS_F32: a sum that an
  * infinity enters may come out as NaN; an element is held to 2^-22 of itself, below 2^-115 to 2^-137. */
 IOS_API int ios_grouped_matmul(const void *x, int type, long long x_rows, long long x_stride, const void *w, int groups,

@@ -2,8 +2,9 @@
 Operators on device tensors: a mixture-of-experts layer and its 8-bit products.
 
 Unlike the graph entry points, which take host arrays, these take tensors that already live on a GPU (``torch.Tensor``)
-and return tensors on the same device; an ``out`` must not overlap what the call reads.  The work goes to torch's current stream of that device and is not waited for;
-the calls may be captured into CUDA graphs.  They compute no gradients, and refuse tensors that ask for one or carry a tangent.
+and return tensors on the same device; an ``out`` must not overlap what the call reads.  The work goes to torch's current
+stream of that device and is not waited for; the calls may be captured into CUDA graphs.  They compute no gradients, and refuse
+tensors that ask for one or carry a tangent.
 
 A layer, from its router logits to its output::
 
@@ -43,7 +44,7 @@ torch = None          # looked up on the first call: the rest of the package doe
 _codes = {}           # torch type -> element type of the C interface
 _lib = None
 _raw_stream = None
-_forward_ad = None    # torch.autograd.forward_ad; its level is below zero wherever no tensor can carry a tangent
+_forward_ad = None    # torch.autograd.forward_ad; where its level is below zero, no tensor carries a tangent
 _FLOATS, _ALL, _INT8 = (0, 1, 2), (0, 1, 2, 3), (3,)
 _MOST_ROWS, _MOST = 1 << 30, (1 << 31) - 1      # rows of a call; any other size: the C interface counts in 32 bits
 
@@ -80,7 +81,7 @@ def _matrix(tensor, name, dims, codes):
         raise ValueError(f'{name} must have {dims} axes, not {tensor.dim()}')
     if not tensor.is_cuda:
         raise ValueError(f'{name} must be on a GPU')
-    if (tensor.requires_grad and torch.is_grad_enabled()) or _forward_ad._current_level >= 0:
+    if (tensor.requires_grad and torch.is_grad_enabled()) or getattr(_forward_ad, '_current_level', 0) >= 0:
         _no_derivative(tensor, name)
     if tensor.stride(-1) != 1 and tensor.shape[-1] > 1:
         raise ValueError(f'the last axis of {name} must be dense (its stride is {tensor.stride(-1)})')
@@ -97,7 +98,7 @@ def _dense(tensor, name, shape, dtype, index):
         raise ValueError(f'{name} is on {tensor.device}, the operands are on cuda:{index}')
     if not tensor.is_contiguous():
         raise ValueError(f'{name} must be contiguous')
-    if (tensor.requires_grad and torch.is_grad_enabled()) or _forward_ad._current_level >= 0:
+    if (tensor.requires_grad and torch.is_grad_enabled()) or getattr(_forward_ad, '_current_level', 0) >= 0:
         _no_derivative(tensor, name)
     return tensor.data_ptr()
 

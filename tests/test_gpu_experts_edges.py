@@ -232,6 +232,14 @@ def test_activations_far_from_zero(act, out_dtype):
     assert got[0] == (float('inf') if act == 'silu' else 1.0) and torch.isnan(got[1])
 
 
+@pytest.mark.parametrize('out_dtype', [BF16, F32], ids=['bf16', 'fp32'])
+def test_relu_of_nan_is_zero(out_dtype):
+    w = torch.tensor([float('nan'), -1.0, 2.0, float('inf')], device='cuda').to(BF16)[None, :, None]
+    got = rt.grouped_matmul(torch.ones(1, 1, dtype=BF16, device='cuda'), w, torch.tensor([0, 1], dtype=torch.int32, device='cuda'), act='relu',
+                            out_dtype=out_dtype)
+    assert got.tolist() == [[0.0, 0.0, 2.0, float('inf')]]
+
+
 # ---- sizes past 32 bits ------------------------------------------------------------------------------------
 
 def test_sizes_past_32_bits_are_refused():
